@@ -1,0 +1,476 @@
+// fp8.cu — the 8-bit operators of the C ABI: block quantisation, the linear layer on quantised operands, writing
+// and reading an 8-bit K/V cache, attention over it.  They need no engine: each call works on the current device and
+// the caller's stream and allocates nothing.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "../../include/pi05.h"
+#include "fp8.cuh"
+#include "kv8_attention.cuh"
+
+using namespace p5;
+
+namespace {
+
+int fail(char* err, size_t err_len, int code, const char* fmt, ...) {
+  if (err && err_len) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(err, err_len, fmt, ap);
+    va_end(ap);
+  }
+  return code;
+}
+int launched(const char* what, char* err, size_t err_len) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  return PI05_OK;
+}
+bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// ------------------------------------------------------------------ quantisation
+// A half warp takes one block of 128 values, 8 a lane.  Memory-bound: each lane loads ITEMS blocks' pieces before it
+// works on the first.
+template <typename X, bool VEC, int ITEMS>
+__global__ void fp8_quantize_kernel(const X* x, long ldx, int cols, uint32_t blocks, uint32_t items, uint8_t* q, long ldq,
+                                    uint8_t* scales, long lds) {
+  const int lane = threadIdx.x & 15;
+  const uint32_t first = (blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4)) * ITEMS;
+  float f[ITEMS][8];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t it = first + k;
+    const uint32_t row = it / blocks;
+    const int c0 = (int)(it % blocks) * FP8_BLOCK + 8 * lane;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[k][i] = 0.f;
+    if (it < items && c0 < cols) {
+      const X* src = x + (long)row * ldx + c0;
+      if (VEC) {
+        if (sizeof(X) == 2) {
+          unpack8(*reinterpret_cast<const uint4*>(src), f[k]);
+        } else {
+          const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+          f[k][0] = a.x, f[k][1] = a.y, f[k][2] = a.z, f[k][3] = a.w;
+          f[k][4] = b.x, f[k][5] = b.y, f[k][6] = b.z, f[k][7] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c0 + i < cols) f[k][i] = (float)src[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t it = first + k;
+    int byte;
+    const uint2 code = fp8_encode8<16>(f[k], byte);
+    if (it >= items) continue;
+    const uint32_t row = it / blocks, blk = it % blocks;
+    const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
+    uint8_t* dst = q + (long)row * ldq + c0;
+    if (c0 + 8 <= cols) {
+      *reinterpret_cast<uint2*>(dst) = code;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < cols) dst[i] = (uint8_t)((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
+    }
+    if (lane == 0) scales[(long)row * lds + blk] = (uint8_t)byte;
+  }
+}
+
+// ------------------------------------------------------------------ the cache
+struct KvRows {
+  const bf16 *k, *v;  // write: sources
+  bf16 *ko, *vo;      // read: destinations
+  long b_stride, t_stride;
+  uint8_t *k8, *ks, *v8, *vs;
+  const int *start, *count, *slots;
+  int n_slots, capacity, batch, T, kv_heads;
+};
+
+// rows [0, n) of sample b that have a place in the cache start at position p0 (may be negative)
+__device__ __forceinline__ bool kv_span(const KvRows& a, int b, int& slot, long& p0, int& n) {
+  slot = a.slots ? a.slots[b] : b;
+  p0 = a.start ? a.start[b] : 0;
+  n = a.count ? max(0, min(a.count[b], a.T)) : a.T;
+  return slot >= 0 && slot < a.n_slots;
+}
+
+// One thread an 8-value piece of a head row, HD / 8 neighbouring lanes a row; grid (pieces, batch, K | V).
+// Where two samples of a call name the same slot and position the later sample's row is kept.
+template <int HD, bool WRITE>
+__global__ void kv8_rows_kernel(const KvRows a) {
+  constexpr int LANES = HD / 8;
+  const int b = blockIdx.y;
+  int slot, n;
+  long p0;
+  bool ok = kv_span(a, b, slot, p0, n);
+  __shared__ int later;
+  if (WRITE) {
+    if (threadIdx.x == 0) later = 0;
+    __syncthreads();
+    if (a.slots)
+      for (int o = b + 1 + threadIdx.x; o < a.batch; o += blockDim.x)
+        if (a.slots[o] == slot) later = 1;
+    __syncthreads();
+  }
+  const long i = (long)blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;  // head row of the sample
+  const int piece = threadIdx.x % LANES;
+  const long t = i / a.kv_heads;
+  const int h = (int)(i % a.kv_heads);
+  const long pos = p0 + t;
+  ok = ok && t < n && pos >= 0 && pos < a.capacity;
+  if (WRITE && ok && later) {
+    for (int o = b + 1; o < a.batch; ++o) {
+      int so, no;
+      long po;
+      if (kv_span(a, o, so, po, no) && so == slot && pos >= po && pos < po + no) ok = false;
+    }
+  }
+  const long head = ((long)slot * a.capacity + pos) * a.kv_heads + h;
+  const long at = (long)b * a.b_stride + t * a.t_stride + (long)h * HD + 8 * piece;
+  uint8_t* codes = (blockIdx.z ? a.v8 : a.k8);
+  uint8_t* bytes = (blockIdx.z ? a.vs : a.ks);
+  if (WRITE) {
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (ok) unpack8(*reinterpret_cast<const uint4*>((blockIdx.z ? a.v : a.k) + at), f);
+    int byte;
+    const uint2 code = fp8_encode8<LANES>(f, byte);
+    if (ok) {
+      *reinterpret_cast<uint2*>(codes + head * HD + 8 * piece) = code;
+      if (piece == 0) bytes[head] = (uint8_t)byte;
+    }
+  } else if (ok) {
+    const uint2 code = *reinterpret_cast<const uint2*>(codes + head * HD + 8 * piece);
+    const float s = fp8_scale_value(bytes[head]);
+    const float2 x0 = fp8_to_f2((uint16_t)code.x), x1 = fp8_to_f2((uint16_t)(code.x >> 16));
+    const float2 x2 = fp8_to_f2((uint16_t)code.y), x3 = fp8_to_f2((uint16_t)(code.y >> 16));
+    *reinterpret_cast<uint4*>((blockIdx.z ? a.vo : a.ko) + at) =
+        make_uint4(pack_bf2(x0.x * s, x0.y * s), pack_bf2(x1.x * s, x1.y * s), pack_bf2(x2.x * s, x2.y * s),
+                   pack_bf2(x3.x * s, x3.y * s));
+  }
+}
+
+template <bool WRITE>
+int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char* err, size_t err_len) {
+  if (a.batch < 1 || a.batch > 65535 || a.T < 1 || a.kv_heads < 1 || a.n_slots < 1 || a.capacity < 1 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return fail(err, err_len, PI05_ERR_ARG,
+                "%s: needs 1 <= batch <= 65535, T, kv_heads, n_slots, capacity >= 1, head_dim 64, 128 or 256", what);
+  const void* x0 = WRITE ? (const void*)a.k : a.ko;
+  const void* x1 = WRITE ? (const void*)a.v : a.vo;
+  if (!x0 || !x1 || !a.k8 || !a.ks || !a.v8 || !a.vs || !aligned(x0, 16) || !aligned(x1, 16) || !aligned(a.k8, 16) ||
+      !aligned(a.v8, 16) || a.b_stride % 8 || a.t_stride % 8 || a.t_stride < (long)a.kv_heads * head_dim || a.b_stride < 0)
+    return fail(err, err_len, PI05_ERR_ARG,
+                "%s: k, v and the caches must be 16-byte aligned device pointers, rows at least kv_heads * head_dim "
+                "elements and a multiple of 8 apart", what);
+  if (!a.slots && a.batch > a.n_slots)
+    return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
+  const long head_rows = (long)a.T * a.kv_heads;
+  const int threads = 256, per = threads / (head_dim / 8);
+  const long gx = (head_rows + per - 1) / per;
+  if (gx > 0x7fffffffL) return fail(err, err_len, PI05_ERR_ARG, "%s: too many rows", what);
+  const dim3 grid((unsigned)gx, a.batch, 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 64)
+    kv8_rows_kernel<64, WRITE><<<grid, threads, 0, st>>>(a);
+  else if (head_dim == 128)
+    kv8_rows_kernel<128, WRITE><<<grid, threads, 0, st>>>(a);
+  else
+    kv8_rows_kernel<256, WRITE><<<grid, threads, 0, st>>>(a);
+  return launched(what, err, err_len);
+}
+
+// ------------------------------------------------------------------ linear layer
+struct Fp8Linear {
+  const uint8_t *x, *xs, *w, *ws;
+  long ldx, ldxs, ldw, ldws;
+  const bf16 *bias, *res, *gate;
+  void* out;
+  int T, F, K, epi;
+};
+
+__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 64 x 64 tile, four warps of 32 x 32; each 128-wide block's partial sum is scaled into the fp32 result.
+__global__ void __launch_bounds__(128) fp8_linear_simple_kernel(const Fp8Linear a) {
+  __shared__ __align__(16) uint8_t sx[64][144], sw[64][144];
+  const int t0 = blockIdx.y * 64, f0 = blockIdx.x * 64;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
+  float acc[2][4][4] = {};
+  const int blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
+  for (int kb = 0; kb < blocks; ++kb) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += 128) {
+      const int r = i >> 3, k = kb * 128 + (i & 7) * 16;
+      uint4 u = make_uint4(0, 0, 0, 0), v = u;
+      if (k < a.K) {  // rows are 16 bytes apart, so a piece that starts in a row ends in its pitch
+        if (t0 + r < a.T) u = *reinterpret_cast<const uint4*>(a.x + (long)(t0 + r) * a.ldx + k);
+        if (f0 + r < a.F) v = *reinterpret_cast<const uint4*>(a.w + (long)(f0 + r) * a.ldw + k);
+        if (k + 16 > a.K) {
+          uint8_t *pu = reinterpret_cast<uint8_t*>(&u), *pv = reinterpret_cast<uint8_t*>(&v);
+          for (int e = a.K - k; e < 16; ++e) pu[e] = pv[e] = 0;
+        }
+      }
+      *reinterpret_cast<uint4*>(&sx[r][(i & 7) * 16]) = u;
+      *reinterpret_cast<uint4*>(&sw[r][(i & 7) * 16]) = v;
+    }
+    __syncthreads();
+    float part[2][4][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t af[2][4], bfr[4][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const uint8_t* p = &sx[wm + 16 * m + g][kk * 32 + 4 * c];
+        af[m][0] = *reinterpret_cast<const uint32_t*>(p);
+        af[m][1] = *reinterpret_cast<const uint32_t*>(p + 8 * 144);
+        af[m][2] = *reinterpret_cast<const uint32_t*>(p + 16);
+        af[m][3] = *reinterpret_cast<const uint32_t*>(p + 8 * 144 + 16);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint8_t* p = &sw[wn + 8 * n + g][kk * 32 + 4 * c];
+        bfr[n][0] = *reinterpret_cast<const uint32_t*>(p);
+        bfr[n][1] = *reinterpret_cast<const uint32_t*>(p + 16);
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mma_e4m3_16832(part[m][n], af[m], bfr[n][0], bfr[n][1]);
+    }
+    float sxv[2][2], swv[4][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = t0 + wm + 16 * m + g + 8 * j;
+        sxv[m][j] = t < a.T ? fp8_scale_value(a.xs[(long)t * a.ldxs + kb]) : 0.f;
+      }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int f = f0 + wn + 8 * n + 2 * c + j;
+        swv[n][j] = f < a.F ? fp8_scale_value(a.ws[(long)f * a.ldws + kb]) : 0.f;
+      }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][n][e] += part[m][n][e] * (sxv[m][e >> 1] * swv[n][e & 1]);
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = t0 + wm + 16 * m + g + 8 * j, f = f0 + wn + 8 * n + 2 * c;
+        if (t >= a.T || f >= a.F) continue;
+        float y[2] = {acc[m][n][2 * j], acc[m][n][2 * j + 1]};
+        const int nf = min(2, a.F - f);
+        if (a.bias)
+          for (int e = 0; e < nf; ++e) y[e] += bf(a.bias[f + e]);
+        if (a.epi == 4) {
+          static_cast<bf16*>(a.out)[(long)t * (a.F / 2) + f / 2] = tobf(gelu_tanh(y[0]) * y[1]);
+          continue;
+        }
+        for (int e = 0; e < nf; ++e) {
+          const long i = (long)t * a.F + f + e;
+          float v = y[e];
+          if (a.epi == 5) {
+            static_cast<float*>(a.out)[i] = v;
+            continue;
+          }
+          if (a.epi == 1) v = gelu_tanh(v);
+          if (a.epi == 2) v += bf(a.res[i]);
+          if (a.epi == 3) v = bf(a.res[i]) + v * bf(a.gate[f + e]);
+          static_cast<bf16*>(a.out)[i] = tobf(v);
+        }
+      }
+}
+
+// ------------------------------------------------------------------ attention
+int num_sms() {
+  static int n = [] {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return 148;
+    return v;
+  }();
+  return n;
+}
+
+int attn_splits(int batch, int T, int heads, int kv_heads, int capacity) {
+  const long tiles = (long)batch * kv_heads * (((long)T * (heads / kv_heads) + 7) / 8);
+  const int max_useful = std::max(1, capacity / 256);
+  return (int)std::max<long>(1, std::min<long>({(long)max_useful, 2L * num_sms() / tiles, 64L}));
+}
+
+template <int HD>
+int attention(const Kv8Args& a, int batch, cudaStream_t st, char* err, size_t err_len) {
+  const dim3 grid((a.T * a.G + 7) / 8, batch * a.kv_heads, a.splits);
+  kv8_attn_rows_kernel<HD, 1, 4><<<grid, 128, 0, st>>>(a);
+  if (a.splits > 1) {
+    const long rows = (long)batch * a.T * a.heads;
+    kv8_attn_combine_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, batch);
+  }
+  return launched("pi05_kv8_attention", err, err_len);
+}
+
+}  // namespace
+
+extern "C" PI05_API int pi05_fp8_quantize(int64_t rows, int64_t cols, const void* x, int x_type, int64_t ldx, void* q,
+                                          int64_t ldq, uint8_t* scales, int64_t ld_scales, void* stream, char* err,
+                                          size_t err_len) {
+  const int64_t blocks = (cols + FP8_BLOCK - 1) / FP8_BLOCK;
+  if (rows < 1 || cols < 1 || cols > 0x7fffff00L || rows > 0x7fffffffL || rows * blocks > 0x7fffffffL || (x_type != 0 && x_type != 1))
+    return fail(err, err_len, PI05_ERR_ARG,
+                "pi05_fp8_quantize: needs rows, cols >= 1, fewer than 2^31 blocks of 128, x_type 0 (bf16) or 1 (fp32)");
+  const int xb = x_type ? 4 : 2;
+  if (!x || !q || !scales || !aligned(x, xb) || !aligned(q, 16) || ldq % 16 || ldx < cols || ldq < cols || ld_scales < blocks)
+    return fail(err, err_len, PI05_ERR_ARG,
+                "pi05_fp8_quantize: q must be 16-byte aligned with rows a multiple of 16 bytes apart, rows of x, q and "
+                "scales at least cols, cols and ceil(cols / 128) elements apart");
+  // 16-byte loads where every row starts on a 16-byte boundary and ends on a whole 8-value piece
+  const bool vec = aligned(x, 16) && (ldx * xb) % 16 == 0 && cols % 8 == 0;
+  constexpr int ITEMS = 4;
+  const uint32_t items = (uint32_t)(rows * blocks), per = 256 / 16 * ITEMS;
+  const unsigned grid = (items + per - 1) / per;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* q8 = static_cast<uint8_t*>(q);
+  const uint32_t nb = (uint32_t)blocks;
+  if (x_type == 0) {
+    const bf16* xp = static_cast<const bf16*>(x);
+    if (vec) fp8_quantize_kernel<bf16, true, ITEMS><<<grid, 256, 0, st>>>(xp, ldx, (int)cols, nb, items, q8, ldq, scales, ld_scales);
+    else fp8_quantize_kernel<bf16, false, ITEMS><<<grid, 256, 0, st>>>(xp, ldx, (int)cols, nb, items, q8, ldq, scales, ld_scales);
+  } else {
+    const float* xp = static_cast<const float*>(x);
+    if (vec) fp8_quantize_kernel<float, true, ITEMS><<<grid, 256, 0, st>>>(xp, ldx, (int)cols, nb, items, q8, ldq, scales, ld_scales);
+    else fp8_quantize_kernel<float, false, ITEMS><<<grid, 256, 0, st>>>(xp, ldx, (int)cols, nb, items, q8, ldq, scales, ld_scales);
+  }
+  return launched("pi05_fp8_quantize", err, err_len);
+}
+
+extern "C" PI05_API int pi05_fp8_linear(int T, int F, int K, const void* x, int64_t ldx, const uint8_t* x_scales,
+                                        int64_t ld_xs, const void* w, int64_t ldw, const uint8_t* w_scales, int64_t ld_ws,
+                                        const void* bias, const void* res, const void* gate, int epi, void* out,
+                                        void* stream, char* err, size_t err_len) {
+  if (T < 1 || F < 1 || K < 1 || T > (1 << 24) || F > (1 << 24) || K > (1 << 24) || epi < 0 || epi > 5 || (epi == 4 && F % 2))
+    return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: needs 1 <= T, F, K <= 2^24, epi 0..5, an even F for epi 4");
+  const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  if (!x || !x_scales || !w || !w_scales || !out || ((epi == 2 || epi == 3) && !res) || (epi == 3 && !gate))
+    return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: missing operand (res for epi 2 and 3, gate for epi 3)");
+  if (!aligned(x, 16) || !aligned(w, 16) || ldx % 16 || ldw % 16 || ldx < K || ldw < K || !aligned(x_scales, 4) ||
+      !aligned(w_scales, 4) || ld_xs % 4 || ld_ws % 4 || ld_xs < blocks || ld_ws < blocks || ldx >= (1LL << 39) || ldw >= (1LL << 39) ||
+      !aligned(out, 16) || !aligned(bias, 16) || !aligned(res, 16) || !aligned(gate, 16))
+    return fail(err, err_len, PI05_ERR_ARG,
+                "pi05_fp8_linear: x and w must be 16-byte aligned with rows a multiple of 16 bytes apart, their scales "
+                "4-byte aligned with rows a multiple of 4 bytes apart, out, bias, res and gate 16-byte aligned");
+  const Fp8Linear a = {static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(w), w_scales, ldx, ld_xs, ldw, ld_ws,
+                       static_cast<const bf16*>(bias), static_cast<const bf16*>(res), static_cast<const bf16*>(gate), out, T, F, K, epi};
+  if ((T + 63) / 64 > 65535) return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: too many tokens");
+  fp8_linear_simple_kernel<<<dim3((F + 63) / 64, (T + 63) / 64), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launched("pi05_fp8_linear", err, err_len);
+}
+
+extern "C" PI05_API int pi05_kv8_write(int batch, int T, int kv_heads, int head_dim, const void* k, const void* v,
+                                       int64_t sample_stride, int64_t token_stride, int n_slots, int capacity, void* k8,
+                                       uint8_t* k_scales, void* v8, uint8_t* v_scales, const int32_t* start,
+                                       const int32_t* count, const int32_t* slots, void* stream, char* err, size_t err_len) {
+  const KvRows a = {static_cast<const bf16*>(k), static_cast<const bf16*>(v), nullptr, nullptr, sample_stride, token_stride,
+                    static_cast<uint8_t*>(k8), k_scales, static_cast<uint8_t*>(v8), v_scales, start, count, slots,
+                    n_slots, capacity, batch, T, kv_heads};
+  return kv8_rows<true>("pi05_kv8_write", a, head_dim, stream, err, err_len);
+}
+
+extern "C" PI05_API int pi05_kv8_read(int batch, int T, int kv_heads, int head_dim, void* k, void* v, int64_t sample_stride,
+                                      int64_t token_stride, int n_slots, int capacity, const void* k8,
+                                      const uint8_t* k_scales, const void* v8, const uint8_t* v_scales,
+                                      const int32_t* start, const int32_t* count, const int32_t* slots, void* stream,
+                                      char* err, size_t err_len) {
+  const KvRows a = {nullptr, nullptr, static_cast<bf16*>(k), static_cast<bf16*>(v), sample_stride, token_stride,
+                    (uint8_t*)k8, (uint8_t*)k_scales, (uint8_t*)v8, (uint8_t*)v_scales, start, count, slots,
+                    n_slots, capacity, batch, T, kv_heads};
+  return kv8_rows<false>("pi05_kv8_read", a, head_dim, stream, err, err_len);
+}
+
+extern "C" PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
+  if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || capacity < 1 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return PI05_ERR_ARG;
+  const int64_t splits = attn_splits(batch, T, heads, kv_heads, capacity);
+  return splits == 1 ? 0 : splits * batch * T * heads * ((int64_t)head_dim * 4 + 8);
+}
+
+extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_heads, int head_dim, const void* q,
+                                           int64_t q_sample_stride, int64_t q_token_stride, int n_slots, int capacity,
+                                           const void* k8, const uint8_t* k_scales, const void* v8, const uint8_t* v_scales,
+                                           const int32_t* lens, const int32_t* slots, int causal, float scale, void* out,
+                                           int64_t out_sample_stride, int64_t out_token_stride, void* workspace,
+                                           int64_t workspace_bytes, void* stream, char* err, size_t err_len) {
+  if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || n_slots < 1 || capacity < 1 ||
+      (int64_t)batch * kv_heads > 65535 || (int64_t)T * (heads / kv_heads) > (1 << 30) || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return fail(err, err_len, PI05_ERR_ARG,
+                "pi05_kv8_attention: needs batch, T, n_slots, capacity >= 1, heads a multiple of kv_heads, head_dim 64, 128 "
+                "or 256, batch * kv_heads <= 65535");
+  const int64_t width = (int64_t)heads * head_dim;
+  if (!q || !k8 || !k_scales || !v8 || !v_scales || !lens || !out || !aligned(q, 16) || !aligned(k8, 16) || !aligned(v8, 16) ||
+      !aligned(out, 16) || q_sample_stride % 8 || q_token_stride % 8 || out_sample_stride % 8 || out_token_stride % 8 ||
+      q_token_stride < width || out_token_stride < width || q_sample_stride < 0 || out_sample_stride < 0 ||
+      (batch > 1 && out_sample_stride < out_token_stride * (T - 1) + width))
+    return fail(err, err_len, PI05_ERR_ARG,
+                "pi05_kv8_attention: q, out and the caches must be 16-byte aligned device pointers, tokens of q and out "
+                "at least heads * head_dim elements and a multiple of 8 apart, samples of out not overlapping");
+  if (!slots && batch > n_slots) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: batch exceeds the cache's slots");
+  if (!(scale == scale) || scale - scale != 0.f) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: scale must be finite");
+  Kv8Args a = {};
+  a.q = static_cast<const bf16*>(q);
+  a.q_b = q_sample_stride;
+  a.q_t = q_token_stride;
+  a.k = static_cast<const uint8_t*>(k8);
+  a.ks = k_scales;
+  a.v = static_cast<const uint8_t*>(v8);
+  a.vs = v_scales;
+  a.lens = lens;
+  a.slots = slots;
+  a.out = static_cast<bf16*>(out);
+  a.o_b = out_sample_stride;
+  a.o_t = out_token_stride;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.n_slots = n_slots;
+  a.capacity = capacity;
+  a.T = T;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.G = heads / kv_heads;
+  a.causal = causal != 0;
+  a.splits = attn_splits(batch, T, heads, kv_heads, capacity);
+  const int64_t need = pi05_kv8_attention_workspace(batch, T, heads, kv_heads, head_dim, capacity);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+      return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + (int64_t)a.splits * batch * T * heads * head_dim);
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 64) return attention<64>(a, batch, st, err, err_len);
+  if (head_dim == 128) return attention<128>(a, batch, st, err, err_len);
+  return attention<256>(a, batch, st, err, err_len);
+}

@@ -267,6 +267,63 @@ PI05_API int pi05_linear_static(int T, int F, int K, const void* x, const void* 
  * No counterpart in the reference's ABI. */
 PI05_API int pi05_linear_static_status(void* stream, char* err, size_t err_len);
 
+/* ---- 8-bit operators: quantisation, linear layer, K/V cache, attention --------------------------------------
+ * For callers that serve with 8-bit weights and activations or hold many prefix caches (a bf16 prefix of the default
+ * model is 17.8 MB an environment, this cache 9 MB).  They need no engine: like pi05_linear_static each call takes the
+ * caller's stream (a cudaStream_t, NULL = legacy default stream) and device pointers of the current device, allocates
+ * nothing, is asynchronous, may be captured into a CUDA graph, and writes a message to err when it refuses.  Calls share
+ * no state, so they may overlap on the GPU as long as their buffers (a workspace among them) are their own.
+ * No counterpart in the reference's ABI (its engine was bf16, π05_네이티브엔진.md:102-105).
+ *
+ * Format: an e4m3 code c (finite, 1 byte) and one exponent byte s for each block stand for c * 2^(s - 127); s - 127 is
+ * the smallest e with max|x| <= 448 * 2^e (s = 0 for a block of zeros), codes are rounded to nearest even.  A block with
+ * a NaN or an infinity has s = 255 and codes 0 and reads as NaN.  Code 0x7f / 0xff (NaN) is never written and not valid
+ * as input.
+ *
+ * pi05_fp8_quantize: rows x cols values (x_type 0 bf16, 1 fp32; row r at x + r * ldx elements) -> q[r][cols], rows ldq
+ *   bytes apart (a multiple of 16, base 16-byte aligned), and scales[r][ceil(cols / 128)], rows ld_scales bytes apart.
+ *   Bytes between a row's end and its pitch are left as they were.
+ * pi05_fp8_linear: out[T][F'] = epilogue(x[T][K] . w[F][K]^T) on two quantised operands; scales' rows a multiple of 4 bytes
+ *   apart, base 4-byte aligned.  epi as pi05_op_linear: 0 store, 1 gelu, 2 residual (res[T][F]), 3 gated residual (res +
+ *   gate[F] * y), 4 GeGLU (w rows interleaved gate/up, F' = F/2), 5 fp32 out; bias[F] optional.  bias, res, gate and out are
+ *   bf16 (out of epi 5 fp32), contiguous, 16-byte aligned; out may be res.  Accumulated in fp32, rounded once at the end.
+ *   1 <= T, F, K <= 2^24, any K. */
+PI05_API int pi05_fp8_quantize(int64_t rows, int64_t cols, const void* x, int x_type, int64_t ldx, void* q, int64_t ldq,
+                               uint8_t* scales, int64_t ld_scales, void* stream, char* err, size_t err_len);
+PI05_API int pi05_fp8_linear(int T, int F, int K, const void* x, int64_t ldx, const uint8_t* x_scales, int64_t ld_xs,
+                             const void* w, int64_t ldw, const uint8_t* w_scales, int64_t ld_ws, const void* bias,
+                             const void* res, const void* gate, int epi, void* out, void* stream, char* err, size_t err_len);
+/* The 8-bit K/V cache: codes k8, v8 [n_slots][capacity][kv_heads][head_dim] and scales [n_slots][capacity][kv_heads], one
+ * scale for each head of a position, all contiguous, codes 16-byte aligned; head_dim 64, 128 or 256.  Sample b of a call
+ * works on slot slots[b] (slots NULL: b).  start, count, lens, slots: int32 in device memory, read by the kernels: a slot
+ * outside [0, n_slots) is passed over, as are positions outside [0, capacity).
+ * pi05_kv8_write: rows t < count[b] (count NULL: T; clamped to [0, T]) of k, v (bf16, sample b's token t at
+ *   b * sample_stride + t * token_stride elements, its kv_heads * head_dim values contiguous, 16-byte aligned) go to positions
+ *   start[b] + t (start NULL: t).  Everything else in the cache stays as it was.  Where two samples name the same
+ *   slot and position the later sample's row is kept.
+ * pi05_kv8_read: the reverse; rows that are passed over stay as they were in k and v.
+ * pi05_kv8_attention: out[b][t][h] = sum_j p_j V_j, p = softmax over j < lens[b] (clamped to [0, capacity]) of
+ *   scale * q[b][t][h] . K_j; causal != 0: token t sees j < lens[b] - T + t + 1 (the last token sees all, as after a write of
+ *   the T tokens).  A row that sees nothing gives 0.  heads is a multiple of kv_heads; query head h reads K/V head
+ *   h / (heads / kv_heads).  q and out bf16, token t of sample b at b * sample stride + t * token stride elements, heads
+ *   contiguous, 16-byte aligned.  workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
+ *   of no importance before and after. */
+PI05_API int pi05_kv8_write(int batch, int T, int kv_heads, int head_dim, const void* k, const void* v, int64_t sample_stride,
+                            int64_t token_stride, int n_slots, int capacity, void* k8, uint8_t* k_scales, void* v8,
+                            uint8_t* v_scales, const int32_t* start, const int32_t* count, const int32_t* slots, void* stream,
+                            char* err, size_t err_len);
+PI05_API int pi05_kv8_read(int batch, int T, int kv_heads, int head_dim, void* k, void* v, int64_t sample_stride,
+                           int64_t token_stride, int n_slots, int capacity, const void* k8, const uint8_t* k_scales,
+                           const void* v8, const uint8_t* v_scales, const int32_t* start, const int32_t* count,
+                           const int32_t* slots, void* stream, char* err, size_t err_len);
+PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int heads, int kv_heads, int head_dim, int capacity);
+PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_heads, int head_dim, const void* q,
+                                int64_t q_sample_stride, int64_t q_token_stride, int n_slots, int capacity, const void* k8,
+                                const uint8_t* k_scales, const void* v8, const uint8_t* v_scales, const int32_t* lens,
+                                const int32_t* slots, int causal, float scale, void* out, int64_t out_sample_stride,
+                                int64_t out_token_stride, void* workspace, int64_t workspace_bytes, void* stream, char* err,
+                                size_t err_len);
+
 /* Reference batch-API names (π05_네이티브엔진.md:288-303).  pi05_create_batch configures the engine from the
  * weight file's cfg lines (NULL path: default configuration with pi05_init_random_weights(0)). */
 PI05_API pi05_engine* pi05_create_batch(const char* weights_path, int device, int max_batch);
