@@ -5,12 +5,14 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
 
 #include "../../include/pi05.h"
 #include "fp8.cuh"
+#include "fp8_gemm.cuh"
 #include "kv8_attention.cuh"
 
 using namespace p5;
@@ -190,120 +192,143 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
 }
 
 // ------------------------------------------------------------------ linear layer
-struct Fp8Linear {
-  const uint8_t *x, *xs, *w, *ws;
-  long ldx, ldxs, ldw, ldws;
-  const bf16 *bias, *res, *gate;
-  void* out;
-  int T, F, K, epi;
-};
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn g_encode = nullptr;
+std::mutex g_mu;
+int g_sms[64];  // SMs of a device, 0 before its first call
 
-__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// [rows][K] codes, rows ld bytes apart, in boxes of one 128-byte K block x box_rows
+bool tmap(CUtensorMap* m, const void* base, long rows, int K, long ld, int box_rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 64 x 64 tile, four warps of 32 x 32; each 128-wide block's partial sum is scaled into the fp32 result.
-__global__ void __launch_bounds__(128) fp8_linear_simple_kernel(const Fp8Linear a) {
-  __shared__ __align__(16) uint8_t sx[64][144], sw[64][144];
-  const int t0 = blockIdx.y * 64, f0 = blockIdx.x * 64;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
-  float acc[2][4][4] = {};
-  const int blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
-  for (int kb = 0; kb < blocks; ++kb) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 8; i += 128) {
-      const int r = i >> 3, k = kb * 128 + (i & 7) * 16;
-      uint4 u = make_uint4(0, 0, 0, 0), v = u;
-      if (k < a.K) {  // rows are 16 bytes apart, so a piece that starts in a row ends in its pitch
-        if (t0 + r < a.T) u = *reinterpret_cast<const uint4*>(a.x + (long)(t0 + r) * a.ldx + k);
-        if (f0 + r < a.F) v = *reinterpret_cast<const uint4*>(a.w + (long)(f0 + r) * a.ldw + k);
-        if (k + 16 > a.K) {
-          uint8_t *pu = reinterpret_cast<uint8_t*>(&u), *pv = reinterpret_cast<uint8_t*>(&v);
-          for (int e = a.K - k; e < 16; ++e) pu[e] = pv[e] = 0;
-        }
-      }
-      *reinterpret_cast<uint4*>(&sx[r][(i & 7) * 16]) = u;
-      *reinterpret_cast<uint4*>(&sw[r][(i & 7) * 16]) = v;
+template <int EPI>
+bool linear_attributes() {
+  auto set = [](const void* f, int bytes) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  };
+  return set((const void*)fp8_few_kernel<32, EPI>, Fp8FewCfg<32>::SMEM) &&
+         set((const void*)fp8_few_kernel<64, EPI>, Fp8FewCfg<64>::SMEM) &&
+         set((const void*)fp8_few_kernel<128, EPI>, Fp8FewCfg<128>::SMEM) &&
+         set((const void*)fp8_pair_kernel<EPI>, Fp8PairCfg::SMEM);
+}
+
+// once per device, with that device current
+int setup(char* err, size_t err_len, int* sms) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(err, err_len, PI05_ERR_CUDA, "no current device");
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_sms[dev]) {
+    if (!g_encode) {
+      void* fn = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn ||
+          q != cudaDriverEntryPointSuccess)
+        return fail(err, err_len, PI05_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+      g_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    __syncthreads();
-    float part[2][4][4] = {};
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t af[2][4], bfr[4][2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const uint8_t* p = &sx[wm + 16 * m + g][kk * 32 + 4 * c];
-        af[m][0] = *reinterpret_cast<const uint32_t*>(p);
-        af[m][1] = *reinterpret_cast<const uint32_t*>(p + 8 * 144);
-        af[m][2] = *reinterpret_cast<const uint32_t*>(p + 16);
-        af[m][3] = *reinterpret_cast<const uint32_t*>(p + 8 * 144 + 16);
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint8_t* p = &sw[wn + 8 * n + g][kk * 32 + 4 * c];
-        bfr[n][0] = *reinterpret_cast<const uint32_t*>(p);
-        bfr[n][1] = *reinterpret_cast<const uint32_t*>(p + 16);
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) mma_e4m3_16832(part[m][n], af[m], bfr[n][0], bfr[n][1]);
-    }
-    float sxv[2][2], swv[4][2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = t0 + wm + 16 * m + g + 8 * j;
-        sxv[m][j] = t < a.T ? fp8_scale_value(a.xs[(long)t * a.ldxs + kb]) : 0.f;
-      }
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int f = f0 + wn + 8 * n + 2 * c + j;
-        swv[n][j] = f < a.F ? fp8_scale_value(a.ws[(long)f * a.ldws + kb]) : 0.f;
-      }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][n][e] += part[m][n][e] * (sxv[m][e >> 1] * swv[n][e & 1]);
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2 || !linear_attributes<FP8_STORE>() ||
+        !linear_attributes<FP8_GELU>() || !linear_attributes<FP8_RESID>() || !linear_attributes<FP8_GATED>() ||
+        !linear_attributes<FP8_GEGLU>() || !linear_attributes<FP8_F32>())
+      return fail(err, err_len, PI05_ERR_CUDA, "preparing the 8-bit kernels failed: %s", cudaGetErrorString(cudaGetLastError()));
+    g_sms[dev] = n;
   }
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = t0 + wm + 16 * m + g + 8 * j, f = f0 + wn + 8 * n + 2 * c;
-        if (t >= a.T || f >= a.F) continue;
-        float y[2] = {acc[m][n][2 * j], acc[m][n][2 * j + 1]};
-        const int nf = min(2, a.F - f);
-        if (a.bias)
-          for (int e = 0; e < nf; ++e) y[e] += bf(a.bias[f + e]);
-        if (a.epi == 4) {
-          static_cast<bf16*>(a.out)[(long)t * (a.F / 2) + f / 2] = tobf(gelu_tanh(y[0]) * y[1]);
-          continue;
-        }
-        for (int e = 0; e < nf; ++e) {
-          const long i = (long)t * a.F + f + e;
-          float v = y[e];
-          if (a.epi == 5) {
-            static_cast<float*>(a.out)[i] = v;
-            continue;
-          }
-          if (a.epi == 1) v = gelu_tanh(v);
-          if (a.epi == 2) v += bf(a.res[i]);
-          if (a.epi == 3) v = bf(a.res[i]) + v * bf(a.gate[f + e]);
-          static_cast<bf16*>(a.out)[i] = tobf(v);
-        }
-      }
+  *sms = g_sms[dev];
+  return PI05_OK;
+}
+
+cudaError_t launch_cluster(const void* fn, unsigned grid, int threads, int smem, unsigned cluster, cudaStream_t st, void** params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, fn, params);
+}
+
+struct LinearPlan {
+  int few_bn;  // 0: the pair kernel
+  int bn, splits;
+};
+
+// Picks the kernel and its tile by an estimate of SM clocks: waves of tiles x K blocks x clocks of a block.  A block
+// costs what its operand bytes take into one SM's shared memory (about 45 B a clock) and a tile its fill and
+// epilogue.
+LinearPlan linear_plan(int T, int F, int blocks, int sms) {
+  LinearPlan best = {0, 0, 1};
+  double best_cost = 1e300;
+  for (int bn = 240; bn >= 128; bn -= 16) {
+    const double units = (double)((T + 255) / 256) * ((F + bn - 1) / bn);
+    const double waves = ceil(units / (sms / 2));
+    const double cost = 5000 + waves * (blocks * 2.3 * bn + 300);
+    if (cost < best_cost) best_cost = cost, best = {0, bn, 1};
+  }
+  for (int bn = 32; bn <= 128; bn *= 2) {
+    if (bn > 32 && T <= bn / 2) break;
+    const double tiles = (double)((F + 127) / 128) * ((T + bn - 1) / bn);
+    for (int s = 1; s <= 8 && s <= blocks; s *= 2) {
+      const double waves = ceil(tiles * s / sms);
+      const double cost = waves * (3500 + ((blocks + s - 1) / s) * (364 + 2.84 * bn) + (s > 1 ? 1500 : 0));
+      if (cost < best_cost) best_cost = cost, best = {bn, bn, s};
+    }
+  }
+  return best;
+}
+
+template <int BN, int EPI>
+cudaError_t launch_few(Fp8Args& a, const void* x, long ldx, const void* w, long ldw, int K, cudaStream_t st, bool& mapped) {
+  CUtensorMap tw, tx;
+  mapped = tmap(&tw, w, a.F, K, ldw, 128) && tmap(&tx, x, a.T, K, ldx, BN);
+  if (!mapped) return cudaSuccess;
+  a.tiles_f = (a.F + 127) / 128;
+  a.tiles_t = (a.T + BN - 1) / BN;
+  void* params[] = {&tw, &tx, &a};
+  return launch_cluster((const void*)fp8_few_kernel<BN, EPI>, (unsigned)((long)a.tiles_f * a.tiles_t * a.splits), 256,
+                        Fp8FewCfg<BN>::SMEM, a.splits, st, params);
+}
+
+template <int EPI>
+int linear(Fp8Args& a, const void* x, long ldx, const void* w, long ldw, int K, int sms, cudaStream_t st, char* err, size_t err_len) {
+  const LinearPlan p = linear_plan(a.T, a.F, a.blocks, sms);
+  a.splits = p.splits;
+  a.bn = p.bn;
+  bool mapped = true;
+  cudaError_t e;
+  if (p.few_bn == 32) {
+    e = launch_few<32, EPI>(a, x, ldx, w, ldw, K, st, mapped);
+  } else if (p.few_bn == 64) {
+    e = launch_few<64, EPI>(a, x, ldx, w, ldw, K, st, mapped);
+  } else if (p.few_bn == 128) {
+    e = launch_few<128, EPI>(a, x, ldx, w, ldw, K, st, mapped);
+  } else {
+    CUtensorMap tx, tw;
+    mapped = tmap(&tx, x, a.T, K, ldx, 128) && tmap(&tw, w, a.F, K, ldw, a.bn / 2);
+    a.tiles_t = (a.T + 255) / 256;
+    a.tiles_f = (a.F + a.bn - 1) / a.bn;
+    a.group_t = std::min(a.tiles_t, 8);
+    const unsigned clusters = (unsigned)std::min<long>((long)a.tiles_t * a.tiles_f, sms / 2);
+    void* params[] = {&tx, &tw, &a};
+    e = mapped ? launch_cluster((const void*)fp8_pair_kernel<EPI>, 2 * clusters, Fp8PairCfg::THREADS, Fp8PairCfg::SMEM, 2, st, params)
+               : cudaSuccess;
+  }
+  if (!mapped) return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: tensor map rejected the operands");
+  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_fp8_linear: %s", cudaGetErrorString(e));
+  return launched("pi05_fp8_linear", err, err_len);
 }
 
 // ------------------------------------------------------------------ attention
@@ -383,11 +408,45 @@ extern "C" PI05_API int pi05_fp8_linear(int T, int F, int K, const void* x, int6
     return fail(err, err_len, PI05_ERR_ARG,
                 "pi05_fp8_linear: x and w must be 16-byte aligned with rows a multiple of 16 bytes apart, their scales "
                 "4-byte aligned with rows a multiple of 4 bytes apart, out, bias, res and gate 16-byte aligned");
-  const Fp8Linear a = {static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(w), w_scales, ldx, ld_xs, ldw, ld_ws,
-                       static_cast<const bf16*>(bias), static_cast<const bf16*>(res), static_cast<const bf16*>(gate), out, T, F, K, epi};
-  if ((T + 63) / 64 > 65535) return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: too many tokens");
-  fp8_linear_simple_kernel<<<dim3((F + 63) / 64, (T + 63) / 64), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return launched("pi05_fp8_linear", err, err_len);
+  if (((int64_t)T + 31) / 32 * (((int64_t)F + 127) / 128) > 0x0fffffff)
+    return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: too many output tiles");
+  int sms = 0;
+  const int rc = setup(err, err_len, &sms);
+  if (rc != PI05_OK) return rc;
+  Fp8Args a = {};
+  a.xs = x_scales;
+  a.ws = w_scales;
+  a.ld_xs = ld_xs;
+  a.ld_ws = ld_ws;
+  a.bias = static_cast<const bf16*>(bias);
+  a.res = static_cast<const bf16*>(res);
+  a.gate = static_cast<const bf16*>(gate);
+  a.out = out;
+  a.T = T;
+  a.F = F;
+  a.blocks = blocks;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (epi) {
+    case FP8_STORE: return linear<FP8_STORE>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+    case FP8_GELU: return linear<FP8_GELU>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+    case FP8_RESID: return linear<FP8_RESID>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+    case FP8_GATED: return linear<FP8_GATED>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+    case FP8_GEGLU: return linear<FP8_GEGLU>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+    default: return linear<FP8_F32>(a, x, ldx, w, ldw, K, sms, st, err, err_len);
+  }
+}
+
+// Waits for `stream`, then reads and clears the status word that the kernels' bounded waits write.
+extern "C" PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len) {
+  cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+  int word = 0;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&word, g_fp8_status, sizeof word);
+  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_fp8_status: %s", cudaGetErrorString(e));
+  if (word == 0) return PI05_OK;
+  const int zero = 0;
+  e = cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof zero);
+  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_fp8_status: %s", cudaGetErrorString(e));
+  return fail(err, err_len, PI05_ERR_DEVICE, "pi05_fp8_*/pi05_kv8_*: a device-side wait gave up (status %d); that call's output is incomplete", word);
 }
 
 extern "C" PI05_API int pi05_kv8_write(int batch, int T, int kv_heads, int head_dim, const void* k, const void* v,

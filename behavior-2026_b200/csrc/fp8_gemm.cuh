@@ -1,0 +1,592 @@
+// fp8_gemm.cuh — the linear layer on block-quantised operands (fp8.cuh) on the 5th-generation tensor cores:
+//   y[t][f] = sum over blocks b of 2^(xs[t][b] + ws[f][b] - 254) sum_{k in b} x[t][k] w[f][k],  out = epilogue(y)
+//
+// tcgen05.mma kind::mxf8f6f4 multiplies e4m3 by e4m3 at twice the bf16 rate and applies a power-of-two scale to each
+// row of either operand for every 32 values of K by itself, so the 128-wide blocks cost no pass over the accumulator:
+// the four K = 32 steps of a block name the same scale.  The scales are read from tensor memory: for the rows 32 j + i of
+// an operand, lane i (the same in each of the four 32-lane quarters) of column j holds one 32-bit word whose four bytes are
+// the row's scales of four consecutive blocks, and the instruction descriptor names the byte.  Such a word is what four
+// consecutive bytes of the caller's scale rows are, so four warps, one for each lane quarter, load the words and
+// tcgen05.st them, a "chunk" of four blocks (512 of K) at a time.
+#pragma once
+#include "fp8.cuh"
+
+namespace p5 {
+
+// device-side status of this file's bounded waits (0: none gave up)
+__device__ int g_fp8_status;
+
+struct Fp8Args {
+  const uint8_t *xs, *ws;  // scales: [T][ld_xs], [F][ld_ws]
+  long ld_xs, ld_ws;
+  const bf16 *bias, *res, *gate;
+  void* out;
+  int T, F, blocks;  // blocks = ceil(K / 128)
+  int tiles_t, tiles_f, group_t;
+  int bn;      // pair kernel: features of a tile
+  int splits;  // few-token kernel: CTAs of a cluster along K
+};
+
+// instruction descriptor of kind::mxf8f6f4: e4m3 x e4m3, ue8m0 scales, both operands K-major; `sf` is the
+// byte of both operands' scale words
+__device__ __forceinline__ uint32_t fp8_idesc(int M, int N, int sf) {
+  return ((uint32_t)sf << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24) | ((uint32_t)sf << 29);
+}
+__device__ __forceinline__ void tc_mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma2_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+// the scales of blocks 4 chunk .. 4 chunk + 3 of row r as one word; 2^0 where there is no such row or block
+__device__ __forceinline__ uint32_t fp8_scale_word(const uint8_t* s, long ld, int r, int rows, int chunk, int blocks) {
+  if (r >= rows) return 0x7f7f7f7fu;
+  const uint8_t* p = s + (long)r * ld + 4 * chunk;
+  if (4 * chunk + 4 <= blocks) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= (4 * chunk + i < blocks ? (uint32_t)p[i] : 0x7fu) << (8 * i);
+  return w;
+}
+
+// After a wait that gave up: the producer lets its last loads land (with a limit) before the CTA can leave.
+__device__ __forceinline__ void fp8_drain(uint64_t* full, int stages, int issued, volatile int* flags, int* status) {
+  if (!flags[0]) return;
+  for (int i = max(0, issued - stages); i < issued; ++i)
+    mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u, status, P5_ERR_WAIT_FULL);
+}
+
+enum Fp8Epi : int { FP8_STORE = 0, FP8_GELU = 1, FP8_RESID = 2, FP8_GATED = 3, FP8_GEGLU = 4, FP8_F32 = 5 };
+
+// Epilogue of eight consecutive features f.. of token t (t < T; f + 8 may pass F), fp32 throughout and rounded once.
+// 16-byte accesses where the rows allow them: F % 8 == 0 (f is a multiple of 8, the bases are 16-byte aligned).
+template <int EPI>
+__device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], int t, int f) {
+  if (f >= a.F) return;
+  if (a.F % 8 == 0) {
+    if (a.bias) {
+      float b[8];
+      unpack8(*reinterpret_cast<const uint4*>(a.bias + f), b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    const long at = (long)t * a.F + f;
+    if (EPI == FP8_F32) {
+      float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
+      d[0] = make_float4(v[0], v[1], v[2], v[3]);
+      d[1] = make_float4(v[4], v[5], v[6], v[7]);
+      return;
+    }
+    if (EPI == FP8_GEGLU) {
+      *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + at / 2) = make_uint2(
+          pack_bf2(gelu_tanh(v[0]) * v[1], gelu_tanh(v[2]) * v[3]), pack_bf2(gelu_tanh(v[4]) * v[5], gelu_tanh(v[6]) * v[7]));
+      return;
+    }
+    if (EPI == FP8_GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = gelu_tanh(v[i]);
+    }
+    if (EPI == FP8_GATED) {
+      float g[8];
+      unpack8(*reinterpret_cast<const uint4*>(a.gate + f), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= g[i];
+    }
+    if (EPI == FP8_RESID || EPI == FP8_GATED) {
+      float r[8];
+      unpack8(*reinterpret_cast<const uint4*>(a.res + at), r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + at) =
+        make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+#pragma unroll
+    for (int j = i; j < i + 2; ++j) {
+      if (f + j >= a.F) continue;
+      if (a.bias) v[j] += bf(a.bias[f + j]);
+      const long at = (long)t * a.F + f + j;
+      if (EPI == FP8_F32) static_cast<float*>(a.out)[at] = v[j];
+      if (EPI == FP8_GELU) v[j] = gelu_tanh(v[j]);
+      if (EPI == FP8_GATED) v[j] *= bf(a.gate[f + j]);
+      if (EPI == FP8_RESID || EPI == FP8_GATED) v[j] += bf(a.res[at]);
+      if (EPI != FP8_F32 && EPI != FP8_GEGLU) static_cast<bf16*>(a.out)[at] = tobf(v[j]);
+    }
+    if (EPI == FP8_GEGLU && f + i + 1 < a.F)
+      static_cast<bf16*>(a.out)[((long)t * a.F + f + i) / 2] = tobf(gelu_tanh(v[i]) * v[i + 1]);
+  }
+}
+
+// ------------------------------------------------------------------ few tokens
+// D[128 features][BN tokens] of one tile by a cluster of `splits` CTAs, each with its share of the K blocks: the weights
+// are on the 128-row side, so a handful of tokens still reads each weight once and at full width.  The fp32 partial tiles
+// meet over distributed shared memory: CTA p receives the token slice p of every partial in one bulk copy each and adds
+// them in rank order (reruns give the same bits).
+//   warp 0  TMA producer, warp 1  MMA issuer, warp 2  TMEM, warps 4-7  scales, then the accumulator
+template <int BN>
+struct Fp8FewCfg {
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN >= 128 ? 5 : (BN >= 64 ? 7 : 8);
+  static constexpr int TILE = BN * 128 * 4;  // fp32 partial tile [token][feature]
+  static constexpr int SF_SLOTS = 4, SF_COL = BN, SF_PITCH = 8;  // scale words: 4 columns of A, BN / 32 of B
+  static constexpr uint32_t TMEM_COLS = BN >= 128 ? 256 : (BN >= 64 ? 128 : 64);
+  static constexpr int SMEM = 1024 + STAGES * STAGE + TILE + 512;
+  static_assert(TILE <= STAGES * STAGE && SF_COL + SF_SLOTS * SF_PITCH <= (int)TMEM_COLS && SMEM <= 232448, "");
+};
+
+template <int BN, int EPI>
+__global__ void __launch_bounds__(256, 1)
+    fp8_few_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Fp8Args a) {
+  using C = Fp8FewCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* ring = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint8_t* recv = ring + C::STAGES * C::STAGE;  // [splits][BN / splits][128] fp32
+  uint64_t* full = reinterpret_cast<uint64_t*>(recv + C::TILE);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* sf_full = empty + C::STAGES;
+  uint64_t* sf_empty = sf_full + C::SF_SLOTS;
+  uint64_t* done = sf_empty + C::SF_SLOTS;
+  uint64_t* got = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(got + 1);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort
+  int* status = &g_fp8_status;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int tile = blockIdx.x / a.splits;
+  const int f0 = (tile % a.tiles_f) * 128, t0 = (tile / a.tiles_f) * BN;
+  const int per = (a.blocks + a.splits - 1) / a.splits;
+  const int kb0 = min((int)rank * per, a.blocks), n = min(kb0 + per, a.blocks) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < C::SF_SLOTS; ++s) {
+      mbar_init(&sf_full[s], 4);
+      mbar_init(&sf_empty[s], 1);
+    }
+    mbar_init(done, 1);
+    mbar_init(got, 1);
+    flags[0] = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tw);
+    tma_prefetch_desc(&tx);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  cluster_sync();  // every CTA's barriers exist before a peer's copy can arrive
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int c_first = kb0 >> 2;  // chunks of four blocks, counted from the start of K
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < n && !flags[0]; ++i) {
+        const int s = i % C::STAGES;
+        if (!mbar_wait(&empty[s], ((uint32_t)(i / C::STAGES) & 1u) ^ 1u, status, P5_ERR_WAIT_EMPTY)) {
+          flags[0] = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[s], C::STAGE);
+        tma_load_2d(ring + s * C::STAGE, &tw, &full[s], (kb0 + i) * 128, f0);
+        tma_load_2d(ring + s * C::STAGE + C::A_BYTES, &tx, &full[s], (kb0 + i) * 128, t0);
+        issued = i + 1;
+      }
+      fp8_drain(full, C::STAGES, issued, flags, status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int cur = -1, slot = 0;
+      for (int i = 0; i < n && !flags[0]; ++i) {
+        const int s = i % C::STAGES, kb = kb0 + i;
+        if ((kb >> 2) != cur) {
+          cur = kb >> 2;
+          const int ci = cur - c_first;
+          slot = ci % C::SF_SLOTS;
+          if (!mbar_wait(&sf_full[slot], (uint32_t)(ci / C::SF_SLOTS) & 1u, status, P5_ERR_WAIT_FULL)) {
+            flags[0] = 1;
+            break;
+          }
+        }
+        if (!mbar_wait(&full[s], (uint32_t)(i / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
+          flags[0] = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t wa = smem_u32(ring + s * C::STAGE), xa = wa + C::A_BYTES;
+        const uint32_t sf = tmem + (uint32_t)(C::SF_COL + slot * C::SF_PITCH);
+        const uint32_t idesc = fp8_idesc(128, BN, kb & 3);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_mxf8(tmem, sw128_kmajor_desc(wa + kk * 32), sw128_kmajor_desc(xa + kk * 32), idesc, sf, sf + 4,
+                      (i > 0 || kk > 0) ? 1u : 0u);
+        tc_commit(&empty[s]);
+        if ((kb & 3) == 3 || i == n - 1) tc_commit(&sf_empty[slot]);
+      }
+      tc_commit(done);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- scale words, a chunk ahead of the wait for its slot
+    const uint32_t t_sf = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SF_COL;
+    const int chunks = n > 0 ? ((kb0 + n - 1) >> 2) - c_first + 1 : 0;
+    for (int ci = 0; ci < chunks; ++ci) {
+      const int slot = ci % C::SF_SLOTS;
+      uint32_t wv[4], xv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wv[j] = fp8_scale_word(a.ws, a.ld_ws, f0 + 32 * j + lane, a.F, c_first + ci, a.blocks);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        xv[j] = j < BN / 32 ? fp8_scale_word(a.xs, a.ld_xs, t0 + 32 * j + lane, a.T, c_first + ci, a.blocks) : 0u;
+      const bool ok = !flags[0] && mbar_wait(&sf_empty[slot], ((uint32_t)(ci / C::SF_SLOTS) & 1u) ^ 1u, status, P5_ERR_WAIT_EMPTY);
+      if (__any_sync(0xffffffffu, !ok)) {
+        flags[0] = 1;
+        break;
+      }
+      tc_fence_after();
+      tmem_st4(t_sf + (uint32_t)(slot * C::SF_PITCH), wv[0], wv[1], wv[2], wv[3]);
+      tmem_st4(t_sf + (uint32_t)(slot * C::SF_PITCH) + 4u, xv[0], xv[1], xv[2], xv[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sf_full[slot]);
+    }
+    // ---- partial tile -> shared memory [token][feature] (the ring is idle once every MMA is done)
+    const bool ok = mbar_wait(done, 0, status, P5_ERR_WAIT_ACCUM) && n > 0;
+    tc_fence_after();
+    float* dst = reinterpret_cast<float*>(a.splits == 1 ? recv : ring) + (warp & 3) * 32 + lane;
+    const uint32_t t_acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      uint32_t r[32];
+      __syncwarp();
+      tmem_ld32(t_acc + (uint32_t)c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dst[(c + i) * 128] = ok ? __uint_as_float(r[i]) : 0.f;
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, C::TMEM_COLS);
+
+  const int slice = BN / a.splits;  // tokens that this CTA finishes
+  if (a.splits > 1) {
+    const uint32_t bytes = (uint32_t)slice * 512u;
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(got, bytes * (uint32_t)a.splits);
+    if (threadIdx.x < (unsigned)a.splits)
+      bulk_copy_to_peer(map_peer(smem_u32(recv) + rank * bytes, threadIdx.x), smem_u32(ring) + threadIdx.x * bytes, bytes,
+                        map_peer(smem_u32(got), threadIdx.x));
+    if (!mbar_wait_cl(got, 0, status, P5_ERR_WAIT_SPLITK)) flags[0] = 1;
+    __syncthreads();
+    cluster_arrive_relaxed();
+  }
+  const float* part = reinterpret_cast<const float*>(recv);
+  if (!flags[0]) {
+    for (int i = threadIdx.x; i < slice * 16; i += 256) {
+      const int j = i >> 4, fo = (i & 15) * 8;
+      const int t = t0 + (int)rank * slice + j;
+      if (t >= a.T) continue;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int p = 0; p < a.splits; ++p) {
+        const float4* s = reinterpret_cast<const float4*>(part + (long)(p * slice + j) * 128 + fo);
+        const float4 u = s[0], w = s[1];
+        v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w, v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
+      }
+      fp8_epilogue8<EPI>(a, v, t, f0 + fo);
+    }
+  }
+  __syncwarp();
+  if (a.splits > 1) cluster_wait_acquire();  // no CTA leaves while a peer's copy may still read its shared memory
+}
+
+// ------------------------------------------------------------------ many tokens
+// A cluster of two CTAs owns 256 tokens x bn features (bn <= 240, a multiple of 16): each stages 128 token rows and
+// bn / 2 weight rows per K block, and one thread of the even CTA issues tcgen05.mma.cta_group::2 over both, as in
+// gemm_pair.cuh (the same ring, relay and commit protocol).  bn stops at 240 because two accumulators of 240 columns leave
+// 32 columns of tensor memory for two chunks of scale words (4 columns of tokens, 8 of features); 256 columns would
+// leave room for one accumulator only, and its epilogue could not run under the next tile's products.
+//   warp 0 TMA, warp 1 MMA (odd CTA: relay), warp 2 TMEM, warps 4-11 epilogue, warps 12-15 scales
+struct Fp8PairCfg {
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = 120 * 128, STAGE = A_BYTES + 16384;
+  static constexpr int STAGES = 6;
+  static constexpr int MAX_BN = 240, SF_COL = 480, SF_PITCH = 16, SF_SLOTS = 2;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 512;
+  static constexpr int THREADS = 512;
+};
+
+template <int EPI>
+__global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Fp8Args a) {
+  using C = Fp8PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* ring = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::STAGE);  // own TMA landed
+  uint64_t* empty = full + C::STAGES;        // pair MMAs done with the stage (multicast commit)
+  uint64_t* pair = empty + C::STAGES;        // even CTA: the odd CTA's stage landed (relay)
+  uint64_t* tfull = pair + C::STAGES;        // [2] accumulator complete (multicast commit)
+  uint64_t* tempty = tfull + 2;              // [2] even CTA: accumulator drained by 16 epilogue warps
+  uint64_t* sf_full = tempty + 2;            // [2] even CTA: scale words of both CTAs in place (8 warps)
+  uint64_t* sf_empty = sf_full + C::SF_SLOTS;  // [2] MMAs done with the scale words (multicast commit)
+  uint64_t* done = sf_empty + C::SF_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort
+  int* status = &g_fp8_status;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool even = rank == 0;
+  const int cid = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  const int n_units = a.tiles_t * a.tiles_f;
+  const uint32_t b_bytes = (uint32_t)(a.bn / 2) * 128u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&pair[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 16);
+      mbar_init(&sf_full[i], 8);
+      mbar_init(&sf_empty[i], 1);
+    }
+    mbar_init(done, 1);
+    flags[0] = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tx);
+    tma_prefetch_desc(&tw);
+  }
+  cluster_sync();
+  if (warp == 2) {
+    tmem_alloc2(tmem_slot, 512);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto decode = [&](int u, int& tt, int& tf) {  // tiles walk down group_t token tiles, then to the next features
+    const int per_group = a.group_t * a.tiles_f;
+    const int group = u / per_group, first = group * a.group_t;
+    const int gt = min(a.group_t, a.tiles_t - first), in = u % per_group;
+    tt = first + in % gt;
+    tf = in / gt;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+        int tt, tf;
+        decode(u, tt, tf);
+        const int xrow = tt * 256 + (int)rank * 128, wrow = tf * a.bn + (int)rank * (a.bn / 2);
+        for (int i = 0; i < a.blocks; ++i, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&empty[s], ((uint32_t)(it / C::STAGES) & 1u) ^ 1u, status, P5_ERR_WAIT_EMPTY)) {
+            flags[0] = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], C::A_BYTES + b_bytes);
+          tma_load_2d(ring + s * C::STAGE, &tx, &full[s], i * 128, xrow);
+          tma_load_2d(ring + s * C::STAGE + C::A_BYTES, &tw, &full[s], i * 128, wrow);
+        }
+      }
+      fp8_drain(full, C::STAGES, it, flags, status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      if (even) {
+        int it = 0, j = 0, ci = 0, slot = 0;
+        for (int u = cid; u < n_units && !flags[0]; u += nclusters, ++j) {
+          const int acc = j & 1;
+          if (!mbar_wait_cl(&tempty[acc], ((uint32_t)(j >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ACCUM)) {
+            flags[0] = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(acc * C::MAX_BN);
+          for (int i = 0; i < a.blocks; ++i, ++it) {
+            const int s = it % C::STAGES;
+            const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
+            if ((i & 3) == 0) {
+              slot = ci & 1;
+              if (!mbar_wait_cl(&sf_full[slot], (uint32_t)(ci >> 1) & 1u, status, P5_ERR_WAIT_FULL)) {
+                flags[0] = 1;
+                break;
+              }
+              ++ci;
+            }
+            if (!mbar_wait(&full[s], ph, status, P5_ERR_WAIT_FULL) || !mbar_wait(&pair[s], ph, status, P5_ERR_WAIT_FULL)) {
+              flags[0] = 1;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t xa = smem_u32(ring + s * C::STAGE), wa = xa + C::A_BYTES;
+            const uint32_t sf = tmem + (uint32_t)(C::SF_COL + slot * C::SF_PITCH);
+            const uint32_t idesc = fp8_idesc(256, a.bn, i & 3);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma2_mxf8(d, sw128_kmajor_desc(xa + kk * 32), sw128_kmajor_desc(wa + kk * 32), idesc, sf, sf + 4,
+                           (i > 0 || kk > 0) ? 1u : 0u);
+            tc_commit2_mc(&empty[s], 3);
+            if ((i & 3) == 3 || i == a.blocks - 1) tc_commit2_mc(&sf_empty[slot], 3);
+          }
+          if (flags[0]) break;
+          tc_commit2_mc(&tfull[acc], 3);
+        }
+        tc_commit2_mc(done, 3);
+      } else {
+        const uint32_t pair0 = map_peer(smem_u32(pair), 0);
+        int it = 0;
+        for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+          for (int i = 0; i < a.blocks; ++i, ++it) {
+            const int s = it % C::STAGES;
+            if (!mbar_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
+              flags[0] = 1;
+              break;
+            }
+            mbar_arrive_cluster_relaxed(pair0 + (uint32_t)s * 8u);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 12) {
+    // ---- scale words of this CTA's 128 tokens and of all bn features
+    const uint32_t t_sf = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SF_COL;
+    const uint32_t full0 = map_peer(smem_u32(sf_full), 0);
+    const int chunks = (a.blocks + 3) >> 2;
+    int ci = 0;
+    for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+      int tt, tf;
+      decode(u, tt, tf);
+      const int xrow = tt * 256 + (int)rank * 128, wrow = tf * a.bn;
+      for (int k = 0; k < chunks; ++k, ++ci) {
+        const int slot = ci & 1;
+        uint32_t xv[4], wv[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[j] = fp8_scale_word(a.xs, a.ld_xs, xrow + 32 * j + lane, a.T, k, a.blocks);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wv[j] = fp8_scale_word(a.ws, a.ld_ws, wrow + 32 * j + lane, a.F, k, a.blocks);
+        const bool ok = !flags[0] && mbar_wait_cl(&sf_empty[slot], ((uint32_t)(ci >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_EMPTY);
+        if (__any_sync(0xffffffffu, !ok)) {
+          flags[0] = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t ta = t_sf + (uint32_t)(slot * C::SF_PITCH);
+        tmem_st4(ta, xv[0], xv[1], xv[2], xv[3]);
+        tmem_st4(ta + 4u, wv[0], wv[1], wv[2], wv[3]);
+        tmem_st4(ta + 8u, wv[4], wv[5], wv[6], wv[7]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (even)
+            mbar_arrive(&sf_full[slot]);
+          else
+            mbar_arrive_cluster(full0 + (uint32_t)slot * 8u);
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: this CTA's 128 tokens, each half of the warps one half of the features
+    const int sub = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
+    const uint32_t tempty0 = map_peer(smem_u32(tempty), 0);
+    // halves in multiples of 8 columns
+    const int c_begin = half ? (a.bn / 16) * 8 : 0, c_end = half ? a.bn : (a.bn / 16) * 8;
+    int j = 0;
+    for (int u = cid; u < n_units; u += nclusters, ++j) {
+      int tt, tf;
+      decode(u, tt, tf);
+      const int acc = j & 1;
+      const bool ok = !flags[0] && mbar_wait(&tfull[acc], (uint32_t)(j >> 1) & 1u, status, P5_ERR_WAIT_ACCUM);
+      if (!ok) flags[0] = 1;
+      tc_fence_after();
+      const uint32_t t_acc = tmem + lane_addr + (uint32_t)(acc * C::MAX_BN);
+      const int t = tt * 256 + (int)rank * 128 + sub * 32 + lane, fb = tf * a.bn;
+#pragma unroll 1
+      for (int c = c_begin; c < c_end; c += 40) {
+        uint32_t r[5][8];
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 5; ++q)
+          if (c + 8 * q < c_end) tmem_ld8(t_acc + (uint32_t)(c + 8 * q), r[q]);
+        tmem_wait_ld();
+        if (ok && t < a.T) {
+#pragma unroll
+          for (int q = 0; q < 5; ++q) {
+            if (c + 8 * q >= c_end) continue;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[q][i]);
+            fp8_epilogue8<EPI>(a, v, t, fb + c + 8 * q);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (even)
+          mbar_arrive(&tempty[acc]);
+        else
+          mbar_arrive_cluster(tempty0 + (uint32_t)acc * 8u);
+      }
+      if (!ok) break;
+    }
+  }
+
+  // ---- exit: the issuer's last commit has landed in both CTAs, then both meet
+  __syncthreads();
+  if (threadIdx.x == 0) mbar_wait_cl(done, 0, status, P5_ERR_WAIT_ACCUM);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc2(tmem, 512);
+  }
+}
+
+}  // namespace p5

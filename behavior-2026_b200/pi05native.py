@@ -31,7 +31,7 @@ EXPORTS = [
     "pi05_tokenizer_free", "pi05_tokenizer_vocab_size", "pi05_tokenizer_encode", "pi05_tokenize_prompt",
     "pi05_set_noise_cholesky", "pi05_set_inpaint", "pi05_set_inpaint_known", "pi05_set_kv_mix", "pi05_prefill_embeds", "pi05_verify_planted",
     "pi05_fp8_quantize", "pi05_fp8_linear", "pi05_kv8_write", "pi05_kv8_read", "pi05_kv8_attention_workspace",
-    "pi05_kv8_attention",
+    "pi05_kv8_attention", "pi05_fp8_status",
 ]
 
 
@@ -151,6 +151,7 @@ def _load():
     i64, tail = ctypes.c_int64, [vp, ctypes.c_char_p, ctypes.c_size_t]
     L.pi05_fp8_quantize.argtypes = [i64, i64, vp, i32, i64, vp, i64, vp, i64] + tail
     L.pi05_fp8_linear.argtypes = [i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, i32, vp] + tail
+    L.pi05_fp8_status.argtypes = tail
     for f in (L.pi05_kv8_write, L.pi05_kv8_read):
         f.argtypes = [i32, i32, i32, i32, vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp] + tail
     L.pi05_kv8_attention_workspace.argtypes = [i32] * 6
@@ -880,6 +881,14 @@ def fp8_linear(x, x_scales, w, w_scales, epi="store", bias=None, res=None, gate=
               w.data_ptr(), _fp8_pitch(w), w_scales.data_ptr(), _fp8_pitch(w_scales), _fp8_addr(bias), _fp8_addr(res),
               _fp8_addr(gate), Engine.EPI[epi], out.data_ptr())
     return out
+
+
+def fp8_status(device=None):
+    """pi05_fp8_status: waits for the current torch stream of `device`; raises Pi05Error(ERR_DEVICE) if a device-side wait of
+    an 8-bit operator there has given up since the last call."""
+    import torch
+
+    _fp8_call(lib.pi05_fp8_status, torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device))
 
 
 def _kv8_cache(what, dev, k8, k_scales, v8, v_scales, slots, batch):

@@ -293,6 +293,10 @@ PI05_API int pi05_fp8_quantize(int64_t rows, int64_t cols, const void* x, int x_
 PI05_API int pi05_fp8_linear(int T, int F, int K, const void* x, int64_t ldx, const uint8_t* x_scales, int64_t ld_xs,
                              const void* w, int64_t ldw, const uint8_t* w_scales, int64_t ld_ws, const void* bias,
                              const void* res, const void* gate, int epi, void* out, void* stream, char* err, size_t err_len);
+/* The kernels' waits are bounded.  pi05_fp8_status waits for `stream`, then reports (PI05_ERR_DEVICE, message in err) and
+ * clears a wait that gave up in a pi05_fp8_* or pi05_kv8_* call on the current device since the last report (that call's
+ * output is incomplete); PI05_OK when there was none.  Not to be called while a stream is being captured. */
+PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
 /* The 8-bit K/V cache: codes k8, v8 [n_slots][capacity][kv_heads][head_dim] and scales [n_slots][capacity][kv_heads], one
  * scale for each head of a position, all contiguous, codes 16-byte aligned; head_dim 64, 128 or 256.  Sample b of a call
  * works on slot slots[b] (slots NULL: b).  start, count, lens, slots: int32 in device memory, read by the kernels: a slot

@@ -17,7 +17,7 @@ E4M3, BF = torch.float8_e4m3fn, torch.bfloat16
 @pytest.fixture(autouse=True)
 def _check_device(pn):
     yield
-    torch.cuda.synchronize()
+    pn.fp8_status()  # no bounded wait gave up
 
 
 def gen(seed):
