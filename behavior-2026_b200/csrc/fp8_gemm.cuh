@@ -32,23 +32,52 @@ struct Fp8Args {
 __device__ __forceinline__ uint32_t fp8_idesc(int M, int N, int sf) {
   return ((uint32_t)sf << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24) | ((uint32_t)sf << 29);
 }
+// The issuing warp runs its loop as a whole and one elected lane issues: in a branch that a single lane takes the
+// operands cannot stay in uniform registers, and moving them there for each instruction made every MMA cost about
+// 180 clocks whatever its N (256 x 128 and 256 x 240 tiles took the same time).
 __device__ __forceinline__ void tc_mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void tc_mma2_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                              uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
+}
+// tc_commit and tc_commit2_mc by the elected lane of a whole warp
+__device__ __forceinline__ void tc_commit_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit2_mc_warp(uint64_t* bar, uint16_t mask) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          smem_u32(bar)),
+      "h"(mask)
+      : "memory");
+}
+// a bounded wait by a whole warp: every lane gets the same answer
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
+__device__ __forceinline__ bool mbar_wait_cl_warp(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_cl(bar, parity, status, code));
 }
 __device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -67,10 +96,16 @@ __device__ __forceinline__ uint32_t fp8_scale_word(const uint8_t* s, long ld, in
   if (4 * chunk + 4 <= blocks) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= (4 * chunk + i < blocks ? (uint32_t)p[i] : 0x7fu) << (8 * i);
+  for (int i = 0; i < 4; ++i) w |= (uint32_t)(4 * chunk + i < blocks ? p[i] : 0x7f) << (8 * i);
   return w;
 }
 
+// the same of blocks 4 chunk .. 4 chunk + 15; `vec`: the rows start on 16-byte boundaries
+__device__ __forceinline__ uint4 fp8_scale_quad(const uint8_t* s, long ld, int r, int rows, int chunk, int blocks, bool vec) {
+  if (r < rows && vec && 4 * chunk + 16 <= blocks) return *reinterpret_cast<const uint4*>(s + (long)r * ld + 4 * chunk);
+  return make_uint4(fp8_scale_word(s, ld, r, rows, chunk, blocks), fp8_scale_word(s, ld, r, rows, chunk + 1, blocks),
+                    fp8_scale_word(s, ld, r, rows, chunk + 2, blocks), fp8_scale_word(s, ld, r, rows, chunk + 3, blocks));
+}
 // After a wait that gave up: the producer lets its last loads land (with a limit) before the CTA can leave.
 __device__ __forceinline__ void fp8_drain(uint64_t* full, int stages, int issued, volatile int* flags, int* status) {
   if (!flags[0]) return;
@@ -177,7 +212,7 @@ __global__ void __launch_bounds__(256, 1)
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort
   int* status = &g_fp8_status;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int tile = blockIdx.x / a.splits;
   const int f0 = (tile % a.tiles_f) * 128, t0 = (tile / a.tiles_f) * BN;
@@ -207,7 +242,7 @@ __global__ void __launch_bounds__(256, 1)
   tc_fence_before();
   cluster_sync();  // every CTA's barriers exist before a peer's copy can arrive
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int c_first = kb0 >> 2;  // chunks of four blocks, counted from the start of K
 
   if (warp == 0) {
@@ -228,37 +263,32 @@ __global__ void __launch_bounds__(256, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int cur = -1, slot = 0;
-      for (int i = 0; i < n && !flags[0]; ++i) {
-        const int s = i % C::STAGES, kb = kb0 + i;
-        if ((kb >> 2) != cur) {
-          cur = kb >> 2;
-          const int ci = cur - c_first;
-          slot = ci % C::SF_SLOTS;
-          if (!mbar_wait(&sf_full[slot], (uint32_t)(ci / C::SF_SLOTS) & 1u, status, P5_ERR_WAIT_FULL)) {
-            flags[0] = 1;
-            break;
-          }
-        }
-        if (!mbar_wait(&full[s], (uint32_t)(i / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
-          flags[0] = 1;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t wa = smem_u32(ring + s * C::STAGE), xa = wa + C::A_BYTES;
-        const uint32_t sf = tmem + (uint32_t)(C::SF_COL + slot * C::SF_PITCH);
-        const uint32_t idesc = fp8_idesc(128, BN, kb & 3);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc_mma_mxf8(tmem, sw128_kmajor_desc(wa + kk * 32), sw128_kmajor_desc(xa + kk * 32), idesc, sf, sf + 4,
-                      (i > 0 || kk > 0) ? 1u : 0u);
-        tc_commit(&empty[s]);
-        if ((kb & 3) == 3 || i == n - 1) tc_commit(&sf_empty[slot]);
+    int cur = -1, slot = 0;
+    for (int i = 0; i < n; ++i) {
+      const int s = i % C::STAGES, kb = kb0 + i;
+      bool ok = true;
+      if ((kb >> 2) != cur) {
+        cur = kb >> 2;
+        const int ci = cur - c_first;
+        slot = ci % C::SF_SLOTS;
+        ok = mbar_wait_warp(&sf_full[slot], (uint32_t)(ci / C::SF_SLOTS) & 1u, status, P5_ERR_WAIT_FULL);
       }
-      tc_commit(done);
+      if (!ok || !mbar_wait_warp(&full[s], (uint32_t)(i / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
+        flags[0] = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t wa = smem_u32(ring) + s * C::STAGE, xa = wa + C::A_BYTES;
+      const uint32_t sf = tmem + (uint32_t)(C::SF_COL + slot * C::SF_PITCH);
+      const uint32_t idesc = fp8_idesc(128, BN, kb & 3);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        tc_mma_mxf8(tmem, sw128_kmajor_desc(wa + kk * 32), sw128_kmajor_desc(xa + kk * 32), idesc, sf, sf + 4,
+                    (i > 0 || kk > 0) ? 1u : 0u);
+      tc_commit_warp(&empty[s]);
+      if ((kb & 3) == 3 || i == n - 1) tc_commit_warp(&sf_empty[slot]);
     }
-    __syncwarp();
+    tc_commit_warp(done);
   } else if (warp >= 4) {
     // ---- scale words, a chunk ahead of the wait for its slot
     const uint32_t t_sf = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SF_COL;
@@ -338,15 +368,18 @@ __global__ void __launch_bounds__(256, 1)
 // ------------------------------------------------------------------ many tokens
 // A cluster of two CTAs owns 256 tokens x bn features (bn <= 240, a multiple of 16): each stages 128 token rows and
 // bn / 2 weight rows per K block, and one thread of the even CTA issues tcgen05.mma.cta_group::2 over both, as in
-// gemm_pair.cuh (the same ring, relay and commit protocol).  bn stops at 240 because two accumulators of 240 columns leave
-// 32 columns of tensor memory for two chunks of scale words (4 columns of tokens, 8 of features); 256 columns would
-// leave room for one accumulator only, and its epilogue could not run under the next tile's products.
+// gemm_pair.cuh (the same ring, relay and commit protocol).  Tensor memory holds two accumulators of bn columns and, in the
+// rest, chunks of scale words (4 columns of tokens, 8 of features); bn = 256 would leave room for one accumulator only,
+// and its epilogue could not run under the next tile's products.
 //   warp 0 TMA, warp 1 MMA (odd CTA: relay), warp 2 TMEM, warps 4-11 epilogue, warps 12-15 scales
 struct Fp8PairCfg {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = 120 * 128, STAGE = A_BYTES + 16384;
   static constexpr int STAGES = 6;
-  static constexpr int MAX_BN = 240, SF_COL = 480, SF_PITCH = 16, SF_SLOTS = 2;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 512;
+  static constexpr int MAX_BN = 240, SF_PITCH = 12, MAX_SLOTS = 8;
+  // chunks of scale words that fit in tensor memory beside two accumulators of bn columns (2 at 240, 5 at 224, 8 from 208 down)
+  __host__ __device__ static constexpr int slots(int bn) { return (512 - 2 * bn) / SF_PITCH < MAX_SLOTS ? (512 - 2 * bn) / SF_PITCH : MAX_SLOTS; }
+  static constexpr int SF_BYTES = 2 * 384 * 16;  // scales of 16 blocks of every row, two buffers
+  static constexpr int SMEM = 1024 + STAGES * STAGE + SF_BYTES + 512;
   static constexpr int THREADS = 512;
 };
 
@@ -357,24 +390,27 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* ring = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::STAGE);  // own TMA landed
+  uint4* sf_rows = reinterpret_cast<uint4*>(ring + C::STAGES * C::STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::STAGE + C::SF_BYTES);  // own TMA landed
   uint64_t* empty = full + C::STAGES;        // pair MMAs done with the stage (multicast commit)
   uint64_t* pair = empty + C::STAGES;        // even CTA: the odd CTA's stage landed (relay)
   uint64_t* tfull = pair + C::STAGES;        // [2] accumulator complete (multicast commit)
   uint64_t* tempty = tfull + 2;              // [2] even CTA: accumulator drained by 16 epilogue warps
-  uint64_t* sf_full = tempty + 2;            // [2] even CTA: scale words of both CTAs in place (8 warps)
-  uint64_t* sf_empty = sf_full + C::SF_SLOTS;  // [2] MMAs done with the scale words (multicast commit)
-  uint64_t* done = sf_empty + C::SF_SLOTS;
+  uint64_t* sf_full = tempty + 2;                // [slots] this CTA's scale words in place (4 warps)
+  uint64_t* sf_empty = sf_full + C::MAX_SLOTS;   // [slots] MMAs done with the scale words (multicast commit)
+  uint64_t* rows_full = sf_empty + C::MAX_SLOTS;  // [2] sf_rows buffer written by the four scale warps
+  uint64_t* done = rows_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort
   int* status = &g_fp8_status;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool even = rank == 0;
   const int cid = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   const int n_units = a.tiles_t * a.tiles_f;
   const uint32_t b_bytes = (uint32_t)(a.bn / 2) * 128u;
+  const int slots = C::slots(a.bn);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -385,7 +421,10 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
       mbar_init(&tempty[i], 16);
-      mbar_init(&sf_full[i], 8);
+      mbar_init(&rows_full[i], 4);
+    }
+    for (int i = 0; i < C::MAX_SLOTS; ++i) {
+      mbar_init(&sf_full[i], 4);
       mbar_init(&sf_empty[i], 1);
     }
     mbar_init(done, 1);
@@ -402,7 +441,7 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   auto decode = [&](int u, int& tt, int& tf) {  // tiles walk down group_t token tiles, then to the next features
     const int per_group = a.group_t * a.tiles_f;
@@ -433,102 +472,136 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
       fp8_drain(full, C::STAGES, it, flags, status);
     }
     __syncwarp();
+  } else if (warp == 1 && even) {
+    int it = 0, j = 0, slot = -1;
+    uint32_t sf_ph = 1;
+    bool ok = true;
+    for (int u = cid; u < n_units && ok; u += nclusters, ++j) {
+      const int acc = j & 1;
+      ok = mbar_wait_cl_warp(&tempty[acc], ((uint32_t)(j >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ACCUM);
+      tc_fence_after();
+      const uint32_t d = tmem + (uint32_t)(acc * a.bn);
+      for (int i = 0; i < a.blocks && ok; ++i, ++it) {
+        const int s = it % C::STAGES;
+        const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
+        if ((i & 3) == 0) {
+          if (++slot == slots) slot = 0;
+          if (slot == 0) sf_ph ^= 1u;
+          ok = mbar_wait_warp(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL);
+        }
+        ok = ok && mbar_wait_warp(&full[s], ph, status, P5_ERR_WAIT_FULL) && mbar_wait_warp(&pair[s], ph, status, P5_ERR_WAIT_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t xa = smem_u32(ring) + s * C::STAGE, wa = xa + C::A_BYTES;
+        const uint32_t sf = tmem + (uint32_t)(2 * a.bn + slot * C::SF_PITCH);
+        const uint32_t idesc = fp8_idesc(256, a.bn, i & 3);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma2_mxf8(d, sw128_kmajor_desc(xa + kk * 32), sw128_kmajor_desc(wa + kk * 32), idesc, sf, sf + 4,
+                       (i > 0 || kk > 0) ? 1u : 0u);
+        tc_commit2_mc_warp(&empty[s], 3);
+        if ((i & 3) == 3 || i == a.blocks - 1) tc_commit2_mc_warp(&sf_empty[slot], 3);
+      }
+      if (ok) tc_commit2_mc_warp(&tfull[acc], 3);
+    }
+    if (!ok) flags[0] = 1;
+    tc_commit2_mc_warp(done, 3);
   } else if (warp == 1) {
     if (lane == 0) {
-      if (even) {
-        int it = 0, j = 0, ci = 0, slot = 0;
-        for (int u = cid; u < n_units && !flags[0]; u += nclusters, ++j) {
-          const int acc = j & 1;
-          if (!mbar_wait_cl(&tempty[acc], ((uint32_t)(j >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ACCUM)) {
-            flags[0] = 1;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(acc * C::MAX_BN);
-          for (int i = 0; i < a.blocks; ++i, ++it) {
-            const int s = it % C::STAGES;
-            const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
-            if ((i & 3) == 0) {
-              slot = ci & 1;
-              if (!mbar_wait_cl(&sf_full[slot], (uint32_t)(ci >> 1) & 1u, status, P5_ERR_WAIT_FULL)) {
-                flags[0] = 1;
-                break;
-              }
-              ++ci;
-            }
-            if (!mbar_wait(&full[s], ph, status, P5_ERR_WAIT_FULL) || !mbar_wait(&pair[s], ph, status, P5_ERR_WAIT_FULL)) {
+      const uint32_t pair0 = map_peer(smem_u32(pair), 0);
+      int it = 0, slot = -1;
+      uint32_t sf_ph = 1;
+      for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+        for (int i = 0; i < a.blocks; ++i, ++it) {
+          const int s = it % C::STAGES;
+          if ((i & 3) == 0) {  // a chunk's first stage is passed on once its scale words are in place too
+            if (++slot == slots) slot = 0;
+            if (slot == 0) sf_ph ^= 1u;
+            if (!mbar_wait(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL)) {
               flags[0] = 1;
               break;
             }
             tc_fence_after();
-            const uint32_t xa = smem_u32(ring + s * C::STAGE), wa = xa + C::A_BYTES;
-            const uint32_t sf = tmem + (uint32_t)(C::SF_COL + slot * C::SF_PITCH);
-            const uint32_t idesc = fp8_idesc(256, a.bn, i & 3);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma2_mxf8(d, sw128_kmajor_desc(xa + kk * 32), sw128_kmajor_desc(wa + kk * 32), idesc, sf, sf + 4,
-                           (i > 0 || kk > 0) ? 1u : 0u);
-            tc_commit2_mc(&empty[s], 3);
-            if ((i & 3) == 3 || i == a.blocks - 1) tc_commit2_mc(&sf_empty[slot], 3);
+            tc_fence_before();
           }
-          if (flags[0]) break;
-          tc_commit2_mc(&tfull[acc], 3);
-        }
-        tc_commit2_mc(done, 3);
-      } else {
-        const uint32_t pair0 = map_peer(smem_u32(pair), 0);
-        int it = 0;
-        for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
-          for (int i = 0; i < a.blocks; ++i, ++it) {
-            const int s = it % C::STAGES;
-            if (!mbar_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
-              flags[0] = 1;
-              break;
-            }
-            mbar_arrive_cluster_relaxed(pair0 + (uint32_t)s * 8u);
+          if (!mbar_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
+            flags[0] = 1;
+            break;
           }
+          mbar_arrive_cluster_relaxed(pair0 + (uint32_t)s * 8u);
         }
       }
     }
     __syncwarp();
   } else if (warp >= 12) {
-    // ---- scale words of this CTA's 128 tokens and of all bn features
-    const uint32_t t_sf = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SF_COL;
-    const uint32_t full0 = map_peer(smem_u32(sf_full), 0);
+    // ---- scale words of this CTA's 128 tokens and of all bn (<= 256) features.  Every quarter of the lanes needs all of
+    // them, but a gather of 4 bytes a row takes a pass of the shared-memory pipe for each row (loaded by each warp for
+    // itself it slowed the whole kernel by a third), so the four warps load 96 of the 384 rows each, 16 blocks at a
+    // time and that far ahead, and share them through shared memory.
+    const int sw = warp - 12;
+    const uint32_t t_sf = tmem + ((uint32_t)(sw * 32) << 16) + (uint32_t)(2 * a.bn);
     const int chunks = (a.blocks + 3) >> 2;
-    int ci = 0;
-    for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+    const bool vec_x = a.ld_xs % 16 == 0 && ((uintptr_t)a.xs & 15) == 0, vec_w = a.ld_ws % 16 == 0 && ((uintptr_t)a.ws & 15) == 0;
+    int u = cid, k = 0, xrow = 0, wrow = 0;  // the next piece of 16 blocks: tile u, chunks k .. k + 3
+    auto enter = [&]() {
       int tt, tf;
       decode(u, tt, tf);
-      const int xrow = tt * 256 + (int)rank * 128, wrow = tf * a.bn;
-      for (int k = 0; k < chunks; ++k, ++ci) {
-        const int slot = ci & 1;
-        uint32_t xv[4], wv[8];
+      xrow = tt * 256 + (int)rank * 128;
+      wrow = tf * a.bn;
+    };
+    uint4 next[3];
+    auto load = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xv[j] = fp8_scale_word(a.xs, a.ld_xs, xrow + 32 * j + lane, a.T, k, a.blocks);
+      for (int j = 0; j < 3; ++j) {
+        const int r = (3 * sw + j) * 32 + lane;
+        next[j] = r < 128 ? fp8_scale_quad(a.xs, a.ld_xs, xrow + r, a.T, k, a.blocks, vec_x)
+                          : fp8_scale_quad(a.ws, a.ld_ws, wrow + r - 128, a.F, k, a.blocks, vec_w);
+      }
+    };
+    if (u < n_units) {
+      enter();
+      load();
+    }
+    bool ok = true;
+    int slot = -1;
+    uint32_t sf_ph = 1;
+    for (int piece = 0; u < n_units && ok; ++piece) {
+      uint4* buf = sf_rows + (piece & 1) * 384;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) wv[j] = fp8_scale_word(a.ws, a.ld_ws, wrow + 32 * j + lane, a.F, k, a.blocks);
-        const bool ok = !flags[0] && mbar_wait_cl(&sf_empty[slot], ((uint32_t)(ci >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_EMPTY);
-        if (__any_sync(0xffffffffu, !ok)) {
-          flags[0] = 1;
-          break;
-        }
+      for (int j = 0; j < 3; ++j) buf[(3 * sw + j) * 32 + lane] = next[j];
+      // a buffer is written again two pieces later, after this wait for the piece between: every warp has read it by then
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rows_full[piece & 1]);
+      ok = mbar_wait_warp(&rows_full[piece & 1], (uint32_t)(piece >> 1) & 1u, status, P5_ERR_WAIT_FULL);
+      const int here = min(4, chunks - k);
+      k += 4;
+      if (k >= chunks) {
+        k = 0;
+        u += nclusters;
+        if (u < n_units) enter();
+      }
+      for (int c = 0; c < here && ok; ++c) {
+        if (++slot == slots) slot = 0;
+        if (slot == 0) sf_ph ^= 1u;
+        uint32_t v[12];
+#pragma unroll
+        for (int j = 0; j < 12; ++j) v[j] = reinterpret_cast<const uint32_t*>(buf + 32 * j + lane)[c];
+        if (c == 0 && u < n_units) load();
+        ok = !flags[0] && mbar_wait(&sf_empty[slot], sf_ph ^ 1u, status, P5_ERR_WAIT_EMPTY);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t ta = t_sf + (uint32_t)(slot * C::SF_PITCH);
-        tmem_st4(ta, xv[0], xv[1], xv[2], xv[3]);
-        tmem_st4(ta + 4u, wv[0], wv[1], wv[2], wv[3]);
-        tmem_st4(ta + 8u, wv[4], wv[5], wv[6], wv[7]);
+        tmem_st4(ta, v[0], v[1], v[2], v[3]);
+        tmem_st4(ta + 4u, v[4], v[5], v[6], v[7]);
+        tmem_st4(ta + 8u, v[8], v[9], v[10], v[11]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (even)
-            mbar_arrive(&sf_full[slot]);
-          else
-            mbar_arrive_cluster(full0 + (uint32_t)slot * 8u);
-        }
+        if (lane == 0) mbar_arrive(&sf_full[slot]);
       }
     }
+    if (!ok) flags[0] = 1;
   } else if (warp >= 4) {
     // ---- epilogue: this CTA's 128 tokens, each half of the warps one half of the features
     const int sub = warp & 3, half = (warp - 4) >> 2;
@@ -544,7 +617,7 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
       const bool ok = !flags[0] && mbar_wait(&tfull[acc], (uint32_t)(j >> 1) & 1u, status, P5_ERR_WAIT_ACCUM);
       if (!ok) flags[0] = 1;
       tc_fence_after();
-      const uint32_t t_acc = tmem + lane_addr + (uint32_t)(acc * C::MAX_BN);
+      const uint32_t t_acc = tmem + lane_addr + (uint32_t)(acc * a.bn);
       const int t = tt * 256 + (int)rank * 128 + sub * 32 + lane, fb = tf * a.bn;
 #pragma unroll 1
       for (int c = c_begin; c < c_end; c += 40) {
