@@ -115,48 +115,56 @@ __device__ __forceinline__ void fp8_drain(uint64_t* full, int stages, int issued
 
 enum Fp8Epi : int { FP8_STORE = 0, FP8_GELU = 1, FP8_RESID = 2, FP8_GATED = 3, FP8_GEGLU = 4, FP8_F32 = 5 };
 
+// The epilogue's arithmetic on eight consecutive features f.. of token t, in fp32 (F % 8 == 0, f < F): v becomes the result,
+// its first four elements for GeGLU.
+template <int EPI>
+__device__ __forceinline__ void fp8_math8(const Fp8Args& a, float (&v)[8], int t, int f) {
+  if (a.bias) {
+    float b[8];
+    unpack8(*reinterpret_cast<const uint4*>(a.bias + f), b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+  }
+  if (EPI == FP8_GEGLU) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = gelu_tanh(v[2 * i]) * v[2 * i + 1];
+  }
+  if (EPI == FP8_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu_tanh(v[i]);
+  }
+  if (EPI == FP8_GATED) {
+    float g[8];
+    unpack8(*reinterpret_cast<const uint4*>(a.gate + f), g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= g[i];
+  }
+  if (EPI == FP8_RESID || EPI == FP8_GATED) {
+    float r[8];
+    unpack8(*reinterpret_cast<const uint4*>(a.res + (long)t * a.F + f), r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+}
+
 // Epilogue of eight consecutive features f.. of token t (t < T; f + 8 may pass F), fp32 throughout and rounded once.
 // 16-byte accesses where the rows allow them: F % 8 == 0 (f is a multiple of 8, the bases are 16-byte aligned).
 template <int EPI>
 __device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], int t, int f) {
   if (f >= a.F) return;
   if (a.F % 8 == 0) {
-    if (a.bias) {
-      float b[8];
-      unpack8(*reinterpret_cast<const uint4*>(a.bias + f), b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += b[i];
-    }
+    fp8_math8<EPI>(a, v, t, f);
     const long at = (long)t * a.F + f;
     if (EPI == FP8_F32) {
       float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
       d[0] = make_float4(v[0], v[1], v[2], v[3]);
       d[1] = make_float4(v[4], v[5], v[6], v[7]);
-      return;
+    } else if (EPI == FP8_GEGLU) {
+      *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + at / 2) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + at) =
+          make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
     }
-    if (EPI == FP8_GEGLU) {
-      *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + at / 2) = make_uint2(
-          pack_bf2(gelu_tanh(v[0]) * v[1], gelu_tanh(v[2]) * v[3]), pack_bf2(gelu_tanh(v[4]) * v[5], gelu_tanh(v[6]) * v[7]));
-      return;
-    }
-    if (EPI == FP8_GELU) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = gelu_tanh(v[i]);
-    }
-    if (EPI == FP8_GATED) {
-      float g[8];
-      unpack8(*reinterpret_cast<const uint4*>(a.gate + f), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= g[i];
-    }
-    if (EPI == FP8_RESID || EPI == FP8_GATED) {
-      float r[8];
-      unpack8(*reinterpret_cast<const uint4*>(a.res + at), r);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += r[i];
-    }
-    *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + at) =
-        make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
     return;
   }
 #pragma unroll
@@ -373,13 +381,14 @@ __global__ void __launch_bounds__(256, 1)
 // and its epilogue could not run under the next tile's products.
 //   warp 0 TMA, warp 1 MMA (odd CTA: relay), warp 2 TMEM, warps 4-11 epilogue, warps 12-15 scales
 struct Fp8PairCfg {
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = 120 * 128, STAGE = A_BYTES + 16384;
-  static constexpr int STAGES = 6;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = 120 * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 5;
   static constexpr int MAX_BN = 240, SF_PITCH = 12, MAX_SLOTS = 8;
   // chunks of scale words that fit in tensor memory beside two accumulators of bn columns (2 at 240, 5 at 224, 8 from 208 down)
   __host__ __device__ static constexpr int slots(int bn) { return (512 - 2 * bn) / SF_PITCH < MAX_SLOTS ? (512 - 2 * bn) / SF_PITCH : MAX_SLOTS; }
   static constexpr int SF_BYTES = 2 * 384 * 16;  // scales of 16 blocks of every row, two buffers
-  static constexpr int SMEM = 1024 + STAGES * STAGE + SF_BYTES + 512;
+  static constexpr int OUT_PITCH = 144, OUT_WARP = 32 * OUT_PITCH;  // staged output: 32 rows of 128 bytes, conflict-free pitch
+  static constexpr int SMEM = 1024 + STAGES * STAGE + SF_BYTES + 8 * OUT_WARP + 512;
   static constexpr int THREADS = 512;
 };
 
@@ -391,7 +400,8 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* ring = smem_raw + (((raw + 1023) & ~1023u) - raw);
   uint4* sf_rows = reinterpret_cast<uint4*>(ring + C::STAGES * C::STAGE);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::STAGES * C::STAGE + C::SF_BYTES);  // own TMA landed
+  uint8_t* out_rows = ring + C::STAGES * C::STAGE + C::SF_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_rows + 8 * C::OUT_WARP);  // own TMA landed
   uint64_t* empty = full + C::STAGES;        // pair MMAs done with the stage (multicast commit)
   uint64_t* pair = empty + C::STAGES;        // even CTA: the odd CTA's stage landed (relay)
   uint64_t* tfull = pair + C::STAGES;        // [2] accumulator complete (multicast commit)
@@ -607,35 +617,81 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
     const int sub = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_addr = (uint32_t)(sub * 32) << 16;
     const uint32_t tempty0 = map_peer(smem_u32(tempty), 0);
-    // halves in multiples of 8 columns
-    const int c_begin = half ? (a.bn / 16) * 8 : 0, c_end = half ? a.bn : (a.bn / 16) * 8;
+    // the halves meet at a multiple of 16 columns, so that output rows start on 32-byte sectors
+    const int middle = (a.bn / 2 + 15) / 16 * 16;
+    const int c_begin = half ? middle : 0, c_end = half ? a.bn : middle;
+    // Rows of 128 output bytes are staged in shared memory and written by whole rows: a thread owns one token, so its own
+    // 16-byte stores lie a row apart and reach L2 as half sectors (7744 x 32768 x 2048 GeGLU 474 us, no stores 340).
+    constexpr int ES = EPI == FP8_F32 ? 4 : 2, PER = EPI == FP8_GEGLU ? 2 : 1;  // output bytes; columns an output value
+    constexpr int PASS = 128 / ES * PER;                                       // columns of 128 output bytes
+    const bool staged = (a.F / PER) % (16 / ES) == 0 && a.F % 8 == 0;
+    uint8_t* stage = out_rows + (warp - 4) * C::OUT_WARP;
+    const long out_pitch = (long)(a.F / PER) * ES;
     int j = 0;
     for (int u = cid; u < n_units; u += nclusters, ++j) {
       int tt, tf;
       decode(u, tt, tf);
       const int acc = j & 1;
-      const bool ok = !flags[0] && mbar_wait(&tfull[acc], (uint32_t)(j >> 1) & 1u, status, P5_ERR_WAIT_ACCUM);
+      const bool ok = !flags[0] && mbar_wait_warp(&tfull[acc], (uint32_t)(j >> 1) & 1u, status, P5_ERR_WAIT_ACCUM);
       if (!ok) flags[0] = 1;
       tc_fence_after();
       const uint32_t t_acc = tmem + lane_addr + (uint32_t)(acc * a.bn);
-      const int t = tt * 256 + (int)rank * 128 + sub * 32 + lane, fb = tf * a.bn;
+      const int t_warp = tt * 256 + (int)rank * 128 + sub * 32, fb = tf * a.bn;
+      const int t = t_warp + lane;
 #pragma unroll 1
-      for (int c = c_begin; c < c_end; c += 40) {
-        uint32_t r[5][8];
-        __syncwarp();
+      for (int c = c_begin; ok && c < c_end; c += PASS) {
+        const int width = min(PASS, c_end - c);  // a multiple of 16
 #pragma unroll
-        for (int q = 0; q < 5; ++q)
-          if (c + 8 * q < c_end) tmem_ld8(t_acc + (uint32_t)(c + 8 * q), r[q]);
-        tmem_wait_ld();
-        if (ok && t < a.T) {
+        for (int q = 0; q < PASS; q += 32) {
+          if (q >= width) break;
+          uint32_t r[32];
+          if (q + 32 <= width) {
+            tmem_ld32(t_acc + (uint32_t)(c + q), r);
+          } else {
+            uint32_t r16[16];
+            tmem_ld16(t_acc + (uint32_t)(c + q), r16);
 #pragma unroll
-          for (int q = 0; q < 5; ++q) {
-            if (c + 8 * q >= c_end) continue;
+            for (int i = 0; i < 16; ++i) r[i] = r16[i], r[16 + i] = 0u;
+          }
+          tmem_wait_ld();
+#pragma unroll
+          for (int p = 0; p < 32; p += 8) {
+            if (q + p >= width) break;
+            const int f = fb + c + q + p;
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[q][i]);
-            fp8_epilogue8<EPI>(a, v, t, fb + c + 8 * q);
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[p + i]);
+            if (!staged) {
+              if (t < a.T) fp8_epilogue8<EPI>(a, v, t, f);
+              continue;
+            }
+            if (f >= a.F || t >= a.T) continue;
+            fp8_math8<EPI>(a, v, t, f);
+            uint8_t* d = stage + lane * C::OUT_PITCH + (q + p) / PER * ES;
+            if (EPI == FP8_F32) {
+              reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<float4*>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else if (EPI == FP8_GEGLU) {
+              *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+            } else {
+              *reinterpret_cast<uint4*>(d) =
+                  make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+            }
           }
+        }
+        if (staged) {
+          __syncwarp();
+          const int bytes = min(width, a.F - fb - c) / PER * ES;  // of a row, a multiple of 16 (none where fb + c >= F)
+          const int piece = (lane & 7) * 16;
+          uint8_t* dst = static_cast<uint8_t*>(a.out) + (long)(fb + c) / PER * ES + piece;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = 4 * i + (lane >> 3);
+            if (piece < bytes && t_warp + row < a.T)
+              *reinterpret_cast<uint4*>(dst + (long)(t_warp + row) * out_pitch) =
+                  *reinterpret_cast<const uint4*>(stage + row * C::OUT_PITCH + piece);
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();
