@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/pi05.h"
 #include "fp8.cuh"
@@ -36,55 +37,49 @@ int launched(const char* what, char* err, size_t err_len) {
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // ------------------------------------------------------------------ quantisation
-// A half warp takes one block of 128 values, 8 a lane.  Memory-bound: each lane loads ITEMS blocks' pieces before it
-// works on the first.
+// A half warp takes a block of 128 values, 8 a lane, and ITEMS consecutive blocks; memory-bound, so all loads are issued
+// before the first block is worked on, and the work on a block is kept to about 6 instructions a value (maxima on bit
+// patterns, one cross-lane reduction).
 template <typename X, bool VEC, int ITEMS>
-__global__ void fp8_quantize_kernel(const X* x, long ldx, int cols, uint32_t blocks, uint32_t items, uint8_t* q, long ldq,
-                                    uint8_t* scales, long lds) {
+__global__ void __launch_bounds__(256)
+    fp8_quantize_kernel(const X* x, long ldx, int cols, uint32_t blocks, uint32_t items, uint8_t* q, long ldq, uint8_t* scales,
+                        long lds) {
   const int lane = threadIdx.x & 15;
   const uint32_t first = (blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4)) * ITEMS;
-  float f[ITEMS][8];
+  const uint32_t row0 = first / blocks, blk0 = first - row0 * blocks;
+  Fp8Raw<X> raw[ITEMS];
+  uint32_t row = row0, blk = blk0;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const uint32_t it = first + k;
-    const uint32_t row = it / blocks;
-    const int c0 = (int)(it % blocks) * FP8_BLOCK + 8 * lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[k][i] = 0.f;
-    if (it < items && c0 < cols) {
+    const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
+    raw[k].clear();
+    if (first + k < items && c0 < cols) {
       const X* src = x + (long)row * ldx + c0;
-      if (VEC) {
-        if (sizeof(X) == 2) {
-          unpack8(*reinterpret_cast<const uint4*>(src), f[k]);
-        } else {
-          const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-          f[k][0] = a.x, f[k][1] = a.y, f[k][2] = a.z, f[k][3] = a.w;
-          f[k][4] = b.x, f[k][5] = b.y, f[k][6] = b.z, f[k][7] = b.w;
-        }
+      if (VEC)
+        raw[k].load(src);
+      else
+        raw[k].load_some(src, min(8, cols - c0));
+    }
+    if (++blk == blocks) blk = 0, ++row;
+  }
+  row = row0, blk = blk0;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    int byte;
+    const uint2 code = fp8_encode8<16>(raw[k], byte);
+    if (first + k < items) {
+      const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
+      uint8_t* dst = q + (long)row * ldq + c0;
+      if (c0 + 8 <= cols) {
+        *reinterpret_cast<uint2*>(dst) = code;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c0 + i < cols) f[k][i] = (float)src[i];
+          if (c0 + i < cols) dst[i] = (uint8_t)((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
       }
+      if (lane == 0) scales[(long)row * lds + blk] = (uint8_t)byte;
     }
-  }
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const uint32_t it = first + k;
-    int byte;
-    const uint2 code = fp8_encode8<16>(f[k], byte);
-    if (it >= items) continue;
-    const uint32_t row = it / blocks, blk = it % blocks;
-    const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
-    uint8_t* dst = q + (long)row * ldq + c0;
-    if (c0 + 8 <= cols) {
-      *reinterpret_cast<uint2*>(dst) = code;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < cols) dst[i] = (uint8_t)((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
-    }
-    if (lane == 0) scales[(long)row * lds + blk] = (uint8_t)byte;
+    if (++blk == blocks) blk = 0, ++row;
   }
 }
 
@@ -106,58 +101,78 @@ __device__ __forceinline__ bool kv_span(const KvRows& a, int b, int& slot, long&
   return slot >= 0 && slot < a.n_slots;
 }
 
-// One thread an 8-value piece of a head row, HD / 8 neighbouring lanes a row; grid (pieces, batch, K | V).
-// Where two samples of a call name the same slot and position the later sample's row is kept.
-template <int HD, bool WRITE>
-__global__ void kv8_rows_kernel(const KvRows a) {
+// One thread an 8-value piece of a head row, HD / 8 neighbouring lanes a row, ITEMS rows a thread with their loads issued
+// together; grid (rows, batch, K | V).  Where two samples of a call name the same slot and position the later sample's
+// row is kept.
+template <int HD, bool WRITE, int ITEMS>
+__global__ void __launch_bounds__(256) kv8_rows_kernel(const KvRows a) {
   constexpr int LANES = HD / 8;
   const int b = blockIdx.y;
   int slot, n;
   long p0;
-  bool ok = kv_span(a, b, slot, p0, n);
-  __shared__ int later;
-  if (WRITE) {
-    if (threadIdx.x == 0) later = 0;
-    __syncthreads();
-    if (a.slots)
-      for (int o = b + 1 + threadIdx.x; o < a.batch; o += blockDim.x)
-        if (a.slots[o] == slot) later = 1;
-    __syncthreads();
+  const bool mine = kv_span(a, b, slot, p0, n);
+  bool later = false;  // a later sample names this slot: rows are compared one by one
+  if (WRITE && a.slots) {
+    for (int o = b + 1 + threadIdx.x; o < a.batch; o += blockDim.x) later |= a.slots[o] == slot;
+    later = __syncthreads_or(later);
   }
-  const long i = (long)blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;  // head row of the sample
-  const int piece = threadIdx.x % LANES;
-  const long t = i / a.kv_heads;
-  const int h = (int)(i % a.kv_heads);
-  const long pos = p0 + t;
-  ok = ok && t < n && pos >= 0 && pos < a.capacity;
-  if (WRITE && ok && later) {
-    for (int o = b + 1; o < a.batch; ++o) {
-      int so, no;
-      long po;
-      if (kv_span(a, o, so, po, no) && so == slot && pos >= po && pos < po + no) ok = false;
+  if (!mine) return;
+  const int per = blockDim.x / LANES, piece = threadIdx.x % LANES;
+  const long first = (long)blockIdx.x * per * ITEMS + threadIdx.x / LANES;  // head row of the sample
+  const bf16* src = blockIdx.z ? a.v : a.k;
+  bf16* dst = blockIdx.z ? a.vo : a.ko;
+  uint8_t* codes = (blockIdx.z ? a.v8 : a.k8) + 8 * piece;
+  uint8_t* bytes = blockIdx.z ? a.vs : a.ks;
+  long head[ITEMS], at[ITEMS];
+  bool ok[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t i = (uint32_t)(first + k * per), t = i / (uint32_t)a.kv_heads, h = i - t * (uint32_t)a.kv_heads;  // head_rows < 2^31
+    const long pos = p0 + t;
+    ok[k] = t < (uint32_t)n && pos >= 0 && pos < a.capacity;
+    if (WRITE && later && ok[k]) {
+      for (int o = b + 1; o < a.batch; ++o) {
+        int so, no;
+        long po;
+        if (kv_span(a, o, so, po, no) && so == slot && pos >= po && pos < po + no) ok[k] = false;
+      }
     }
+    head[k] = ((long)slot * a.capacity + pos) * a.kv_heads + h;
+    at[k] = (long)b * a.b_stride + (long)t * a.t_stride + (long)h * HD + 8 * piece;
   }
-  const long head = ((long)slot * a.capacity + pos) * a.kv_heads + h;
-  const long at = (long)b * a.b_stride + t * a.t_stride + (long)h * HD + 8 * piece;
-  uint8_t* codes = (blockIdx.z ? a.v8 : a.k8);
-  uint8_t* bytes = (blockIdx.z ? a.vs : a.ks);
   if (WRITE) {
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (ok) unpack8(*reinterpret_cast<const uint4*>((blockIdx.z ? a.v : a.k) + at), f);
-    int byte;
-    const uint2 code = fp8_encode8<LANES>(f, byte);
-    if (ok) {
-      *reinterpret_cast<uint2*>(codes + head * HD + 8 * piece) = code;
-      if (piece == 0) bytes[head] = (uint8_t)byte;
+    Fp8Raw<bf16> raw[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      raw[k].clear();
+      if (ok[k]) raw[k].load(src + at[k]);
     }
-  } else if (ok) {
-    const uint2 code = *reinterpret_cast<const uint2*>(codes + head * HD + 8 * piece);
-    const float s = fp8_scale_value(bytes[head]);
-    const float2 x0 = fp8_to_f2((uint16_t)code.x), x1 = fp8_to_f2((uint16_t)(code.x >> 16));
-    const float2 x2 = fp8_to_f2((uint16_t)code.y), x3 = fp8_to_f2((uint16_t)(code.y >> 16));
-    *reinterpret_cast<uint4*>((blockIdx.z ? a.vo : a.ko) + at) =
-        make_uint4(pack_bf2(x0.x * s, x0.y * s), pack_bf2(x1.x * s, x1.y * s), pack_bf2(x2.x * s, x2.y * s),
-                   pack_bf2(x3.x * s, x3.y * s));
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      int byte;
+      const uint2 code = fp8_encode8<LANES>(raw[k], byte);
+      if (ok[k]) {
+        *reinterpret_cast<uint2*>(codes + head[k] * HD) = code;
+        if (piece == 0) bytes[head[k]] = (uint8_t)byte;
+      }
+    }
+  } else {
+    uint2 code[ITEMS];
+    int byte[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      code[k] = ok[k] ? *reinterpret_cast<const uint2*>(codes + head[k] * HD) : make_uint2(0u, 0u);
+      byte[k] = ok[k] ? bytes[head[k]] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      if (!ok[k]) continue;
+      const float s = fp8_scale_value(byte[k]);
+      const float2 x0 = fp8_to_f2((uint16_t)code[k].x), x1 = fp8_to_f2((uint16_t)(code[k].x >> 16));
+      const float2 x2 = fp8_to_f2((uint16_t)code[k].y), x3 = fp8_to_f2((uint16_t)(code[k].y >> 16));
+      *reinterpret_cast<uint4*>(dst + at[k]) = make_uint4(pack_bf2(x0.x * s, x0.y * s), pack_bf2(x1.x * s, x1.y * s),
+                                                          pack_bf2(x2.x * s, x2.y * s), pack_bf2(x3.x * s, x3.y * s));
+    }
   }
 }
 
@@ -177,17 +192,26 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
   if (!a.slots && a.batch > a.n_slots)
     return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
   const long head_rows = (long)a.T * a.kv_heads;
+  // 4 rows a thread, one where the call has too few for that to fill the machine
   const int threads = 256, per = threads / (head_dim / 8);
-  const long gx = (head_rows + per - 1) / per;
-  if (gx > 0x7fffffffL) return fail(err, err_len, PI05_ERR_ARG, "%s: too many rows", what);
+  const bool few = head_rows * a.batch < 148L * 8 * per;
+  const long gx = (head_rows + per * (few ? 1 : 4) - 1) / (per * (few ? 1 : 4));
+  if (head_rows > 0x7fffffffL) return fail(err, err_len, PI05_ERR_ARG, "%s: T * kv_heads must be below 2^31", what);
   const dim3 grid((unsigned)gx, a.batch, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    if (few)
+      kv8_rows_kernel<HD, WRITE, 1><<<grid, threads, 0, st>>>(a);
+    else
+      kv8_rows_kernel<HD, WRITE, 4><<<grid, threads, 0, st>>>(a);
+  };
   if (head_dim == 64)
-    kv8_rows_kernel<64, WRITE><<<grid, threads, 0, st>>>(a);
+    go(std::integral_constant<int, 64>());
   else if (head_dim == 128)
-    kv8_rows_kernel<128, WRITE><<<grid, threads, 0, st>>>(a);
+    go(std::integral_constant<int, 128>());
   else
-    kv8_rows_kernel<256, WRITE><<<grid, threads, 0, st>>>(a);
+    go(std::integral_constant<int, 256>());
   return launched(what, err, err_len);
 }
 
@@ -266,24 +290,26 @@ struct LinearPlan {
   int bn, splits;
 };
 
-// Picks the kernel and its tile by an estimate of SM clocks: waves of tiles x K blocks x clocks of a block.  A block
-// costs what its operand bytes take into one SM's shared memory (about 45 B a clock) and a tile its fill and
-// epilogue.
+// Picks the kernel and its tile by an estimate of its time in microseconds, fitted to measurements of 27 shapes (tokens
+// 1 to 7744, features 1024 to 32768, K 1024 to 16384; each plan forced in turn).  A K block costs an SM what its operand
+// bytes take to arrive; a cluster's exchange grows with its CTAs.  E.g. 50 x 8192 x 1024: 32-token tiles 6.4, 64 8.2, pair
+// kernel 12.5; 968 x 2560 x 2048: pair 11.8 (160 features), 12.9 (240), 64-token tiles 18.3; 50 x 1024 x 4096: one
+// CTA a tile 13.2, clusters of four 7.4; 7744 x 2048 x 16384: pair 204 (240), 262 (128), 128-token tiles 413.
 LinearPlan linear_plan(int T, int F, int blocks, int sms) {
   LinearPlan best = {0, 0, 1};
   double best_cost = 1e300;
   for (int bn = 240; bn >= 128; bn -= 16) {
     const double units = (double)((T + 255) / 256) * ((F + bn - 1) / bn);
-    const double waves = ceil(units / (sms / 2));
-    const double cost = 5000 + waves * (blocks * 2.3 * bn + 300);
+    const double cost = 5.5 + ceil(units / (sms / 2)) * (blocks * (0.26 + 0.0005 * bn) + 0.3);
     if (cost < best_cost) best_cost = cost, best = {0, bn, 1};
   }
   for (int bn = 32; bn <= 128; bn *= 2) {
     if (bn > 32 && T <= bn / 2) break;
     const double tiles = (double)((F + 127) / 128) * ((T + bn - 1) / bn);
+    const double block = bn == 32 ? 0.36 : (bn == 64 ? 0.47 : 0.42);
     for (int s = 1; s <= 8 && s <= blocks; s *= 2) {
-      const double waves = ceil(tiles * s / sms);
-      const double cost = waves * (3500 + ((blocks + s - 1) / s) * (364 + 2.84 * bn) + (s > 1 ? 1500 : 0));
+      const double on_an_sm = ceil(tiles * s / sms);
+      const double cost = 3.7 + on_an_sm * ((blocks + s - 1) / s * block + (s > 1 ? 0.3 + 0.4 * s : 0));
       if (cost < best_cost) best_cost = cost, best = {bn, bn, s};
     }
   }

@@ -50,26 +50,69 @@ __device__ __forceinline__ float2 fp8_to_f2(uint16_t c2) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// Exponent byte of the block that LANES consecutive lanes hold 8 values of each (0 where a lane has none), and
-// the lane's 8 codes.  Every lane of the warp calls it.
-template <int LANES>
-__device__ __forceinline__ uint2 fp8_encode8(const float (&f)[8], int& byte) {
-  float m = 0.f;
+// Eight values as they lie in memory.  Magnitudes are compared as bit patterns (of one sign they order like the values,
+// infinities and NaNs above all finite ones).
+template <typename X>
+struct Fp8Raw;
+template <>
+struct Fp8Raw<bf16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  __device__ __forceinline__ void load(const bf16* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  }
+  __device__ __forceinline__ void load_some(const bf16* p, int n) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));  // fmaxf drops a NaN: counted below
-  bool bad = false;
+    for (int i = 0; i < 8; ++i)
+      if (i < n) w[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
+  }
+  __device__ __forceinline__ uint32_t top() const {  // as an fp32 bit pattern
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+};
+template <>
+struct Fp8Raw<float> {
+  uint32_t w[8];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= !(fabsf(f[i]) <= 3.4028234e38f);
-  if (bad) m = INFINITY;
+    for (int i = 0; i < 8; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const float* p) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  }
+  __device__ __forceinline__ void load_some(const float* p, int n) {
 #pragma unroll
-  for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (m == INFINITY) {
+    for (int i = 0; i < 8; ++i)
+      if (i < n) w[i] = __float_as_uint(p[i]);
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
+};
+
+// The codes of a lane's eight values and the exponent byte of the block that LANES consecutive lanes hold.
+// Every lane of the warp calls it.
+template <int LANES, typename X>
+__device__ __forceinline__ uint2 fp8_encode8(const Fp8Raw<X>& x, int& byte) {
+  const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+  const uint32_t m = __reduce_max_sync(mask, x.top());
+  if (m >= 0x7f800000u) {  // an infinity or a NaN
     byte = 255;
     return make_uint2(0u, 0u);
   }
-  byte = fp8_scale_byte(m);
+  byte = fp8_scale_byte(__uint_as_float(m));
   const float r = fp8_scale_inverse(byte);
-  return make_uint2(fp8_pack4(f[0] * r, f[1] * r, f[2] * r, f[3] * r), fp8_pack4(f[4] * r, f[5] * r, f[6] * r, f[7] * r));
+  return make_uint2(fp8_pack4(x.at(0) * r, x.at(1) * r, x.at(2) * r, x.at(3) * r),
+                    fp8_pack4(x.at(4) * r, x.at(5) * r, x.at(6) * r, x.at(7) * r));
 }
 
 }  // namespace p5

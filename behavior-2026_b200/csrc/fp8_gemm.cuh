@@ -147,12 +147,33 @@ __device__ __forceinline__ void fp8_math8(const Fp8Args& a, float (&v)[8], int t
   }
 }
 
+// The same for rows that are not a multiple of 16 bytes: element by element, features past F left alone.
+template <int EPI>
+__device__ __forceinline__ void fp8_math8_any(const Fp8Args& a, float (&v)[8], int t, int f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (f + i >= a.F) break;
+    if (a.bias) v[i] += bf(a.bias[f + i]);
+    if (EPI == FP8_GELU) v[i] = gelu_tanh(v[i]);
+    if (EPI == FP8_GATED) v[i] *= bf(a.gate[f + i]);
+    if (EPI == FP8_RESID || EPI == FP8_GATED) v[i] += bf(a.res[(long)t * a.F + f + i]);
+  }
+  if (EPI == FP8_GEGLU) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = gelu_tanh(v[2 * i]) * v[2 * i + 1];
+  }
+}
+// 16-byte accesses: rows of out, res start on 16-byte boundaries (the bases do)
+template <int EPI>
+__device__ __forceinline__ bool fp8_rows_aligned(const Fp8Args& a) {
+  return a.F % (EPI == FP8_GEGLU ? 16 : 8) == 0;
+}
+
 // Epilogue of eight consecutive features f.. of token t (t < T; f + 8 may pass F), fp32 throughout and rounded once.
-// 16-byte accesses where the rows allow them: F % 8 == 0 (f is a multiple of 8, the bases are 16-byte aligned).
 template <int EPI>
 __device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], int t, int f) {
   if (f >= a.F) return;
-  if (a.F % 8 == 0) {
+  if (fp8_rows_aligned<EPI>(a)) {
     fp8_math8<EPI>(a, v, t, f);
     const long at = (long)t * a.F + f;
     if (EPI == FP8_F32) {
@@ -167,21 +188,17 @@ __device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], i
     }
     return;
   }
+  fp8_math8_any<EPI>(a, v, t, f);
+  constexpr int PER = EPI == FP8_GEGLU ? 2 : 1;
+  const int n = (min(8, a.F - f)) / PER;
+  const long at = ((long)t * a.F + f) / PER;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-#pragma unroll
-    for (int j = i; j < i + 2; ++j) {
-      if (f + j >= a.F) continue;
-      if (a.bias) v[j] += bf(a.bias[f + j]);
-      const long at = (long)t * a.F + f + j;
-      if (EPI == FP8_F32) static_cast<float*>(a.out)[at] = v[j];
-      if (EPI == FP8_GELU) v[j] = gelu_tanh(v[j]);
-      if (EPI == FP8_GATED) v[j] *= bf(a.gate[f + j]);
-      if (EPI == FP8_RESID || EPI == FP8_GATED) v[j] += bf(a.res[at]);
-      if (EPI != FP8_F32 && EPI != FP8_GEGLU) static_cast<bf16*>(a.out)[at] = tobf(v[j]);
-    }
-    if (EPI == FP8_GEGLU && f + i + 1 < a.F)
-      static_cast<bf16*>(a.out)[((long)t * a.F + f + i) / 2] = tobf(gelu_tanh(v[i]) * v[i + 1]);
+  for (int i = 0; i < 8 / PER; ++i) {
+    if (i >= n) break;
+    if (EPI == FP8_F32)
+      static_cast<float*>(a.out)[at + i] = v[i];
+    else
+      static_cast<bf16*>(a.out)[at + i] = tobf(v[i]);
   }
 }
 
@@ -194,16 +211,17 @@ __device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], i
 template <int BN>
 struct Fp8FewCfg {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN >= 128 ? 5 : (BN >= 64 ? 7 : 8);
+  static constexpr int STAGES = BN >= 128 ? 5 : (BN >= 64 ? 3 : 4);
+  static constexpr int PER_SM = BN >= 128 ? 1 : 2;  // two CTAs share an SM: one's fill and epilogue run under the other's loads
   static constexpr int TILE = BN * 128 * 4;  // fp32 partial tile [token][feature]
   static constexpr int SF_SLOTS = 4, SF_COL = BN, SF_PITCH = 8;  // scale words: 4 columns of A, BN / 32 of B
   static constexpr uint32_t TMEM_COLS = BN >= 128 ? 256 : (BN >= 64 ? 128 : 64);
   static constexpr int SMEM = 1024 + STAGES * STAGE + TILE + 512;
-  static_assert(TILE <= STAGES * STAGE && SF_COL + SF_SLOTS * SF_PITCH <= (int)TMEM_COLS && SMEM <= 232448, "");
+  static_assert(TILE <= STAGES * STAGE && SF_COL + SF_SLOTS * SF_PITCH <= (int)TMEM_COLS && SMEM * PER_SM <= 232448 - 1024, "");
 };
 
 template <int BN, int EPI>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(256, Fp8FewCfg<BN>::PER_SM)
     fp8_few_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Fp8Args a) {
   using C = Fp8FewCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -624,7 +642,7 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
     // 16-byte stores lie a row apart and reach L2 as half sectors (7744 x 32768 x 2048 GeGLU 474 us, no stores 340).
     constexpr int ES = EPI == FP8_F32 ? 4 : 2, PER = EPI == FP8_GEGLU ? 2 : 1;  // output bytes; columns an output value
     constexpr int PASS = 128 / ES * PER;                                       // columns of 128 output bytes
-    const bool staged = (a.F / PER) % (16 / ES) == 0 && a.F % 8 == 0;
+    const bool rows16 = fp8_rows_aligned<EPI>(a);
     uint8_t* stage = out_rows + (warp - 4) * C::OUT_WARP;
     const long out_pitch = (long)(a.F / PER) * ES;
     int j = 0;
@@ -661,12 +679,11 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[p + i]);
-            if (!staged) {
-              if (t < a.T) fp8_epilogue8<EPI>(a, v, t, f);
-              continue;
-            }
             if (f >= a.F || t >= a.T) continue;
-            fp8_math8<EPI>(a, v, t, f);
+            if (rows16)
+              fp8_math8<EPI>(a, v, t, f);
+            else
+              fp8_math8_any<EPI>(a, v, t, f);
             uint8_t* d = stage + lane * C::OUT_PITCH + (q + p) / PER * ES;
             if (EPI == FP8_F32) {
               reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -679,20 +696,30 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
             }
           }
         }
-        if (staged) {
-          __syncwarp();
-          const int bytes = min(width, a.F - fb - c) / PER * ES;  // of a row, a multiple of 16 (none where fb + c >= F)
+        __syncwarp();
+        const int bytes = min(width, a.F - fb - c) / PER * ES;  // of a row (none where fb + c >= F)
+        uint8_t* dst = static_cast<uint8_t*>(a.out) + (long)(fb + c) / PER * ES;
+        if (rows16) {
           const int piece = (lane & 7) * 16;
-          uint8_t* dst = static_cast<uint8_t*>(a.out) + (long)(fb + c) / PER * ES + piece;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int row = 4 * i + (lane >> 3);
             if (piece < bytes && t_warp + row < a.T)
-              *reinterpret_cast<uint4*>(dst + (long)(t_warp + row) * out_pitch) =
+              *reinterpret_cast<uint4*>(dst + (long)(t_warp + row) * out_pitch + piece) =
                   *reinterpret_cast<const uint4*>(stage + row * C::OUT_PITCH + piece);
           }
-          __syncwarp();
+        } else {
+          for (int row = 0; row < 32 && t_warp + row < a.T; ++row)
+            for (int e = lane * ES; e < bytes; e += 32 * ES) {
+              uint8_t* d = dst + (long)(t_warp + row) * out_pitch + e;
+              const uint8_t* sp = stage + row * C::OUT_PITCH + e;
+              if (ES == 4)
+                *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(sp);
+              else
+                *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(sp);
+            }
         }
+        __syncwarp();
       }
       tc_fence_before();
       __syncwarp();

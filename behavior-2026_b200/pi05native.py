@@ -10,7 +10,6 @@ There is no fallback: if libpi05.so is missing or fails to load, importing this 
 """
 import ctypes
 import os
-import threading
 
 import numpy as np
 
@@ -781,218 +780,17 @@ def linear_static_status(stream=None):
         raise Pi05Error(rc, err.value.decode())
 
 
-# -- 8-bit operators (pi05_fp8_*, pi05_kv8_*) on torch CUDA tensors, on torch's current stream of the tensors' device
-
-_FP8 = threading.local()
-
-
-def _fp8_call(fn, dev, *args):
-    """One call with `dev` current, on its current torch stream; raises Pi05Error with the library's message."""
-    import torch
-
-    err = getattr(_FP8, "err", None)
-    if err is None:
-        err = _FP8.err = ctypes.create_string_buffer(512)
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, stream, err, 512)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, stream, err, 512)
-    if rc != OK:
-        raise Pi05Error(rc, err.value.decode())
+# -- 8-bit operators (pi05_fp8_*, pi05_kv8_*) on torch CUDA tensors: pi05fp8.py, loaded on first use because it needs torch
+_FP8_NAMES = ("fp8_quantize", "fp8_linear", "fp8_status", "kv8_write", "kv8_read", "kv8_attention")
 
 
-def _fp8_need(ok, what):
-    if not ok:
-        raise Pi05Error(ERR_ARG, what)
+def __getattr__(name):
+    if name in _FP8_NAMES:
+        import pi05fp8
 
-
-def _fp8_same(dev, *tensors):
-    for t in tensors:
-        _fp8_need(t is None or t.device == dev, f"tensors on {dev} and {t.device if t is not None else None}")
-
-
-def _fp8_addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def fp8_quantize(x, out=None):
-    """pi05_fp8_quantize: x [rows][cols] bf16 or fp32 (rows may be strided) -> (q, scales): q float8_e4m3fn [rows][cols]
-    with rows a multiple of 16 bytes apart, scales uint8 [rows][ceil(cols / 128)] with rows a multiple of 4 bytes apart;
-    x ~ q * 2^(scales - 127) block by block.  `out` = (q, scales) of an earlier call to write into."""
-    import torch
-
-    _fp8_need(x.is_cuda and x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float32),
-              "fp8_quantize: x must be a CUDA tensor [rows][cols], bf16 or fp32")
-    rows, cols = x.shape
-    _fp8_need(rows > 0 and cols > 0 and (x.stride(1) == 1 or cols == 1), "fp8_quantize: x is empty or its rows are not contiguous")
-    blocks = (cols + 127) // 128
-    if out is None:
-        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=x.device)[:, :cols]
-        s = torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=x.device)[:, :blocks]
-    else:
-        q, s = out
-        _fp8_same(x.device, q, s)
-        _fp8_need(q.dtype == torch.float8_e4m3fn and s.dtype == torch.uint8 and q.shape == (rows, cols)
-                  and s.shape == (rows, blocks) and (q.stride(1) == 1 or cols == 1) and (s.stride(1) == 1 or blocks == 1),
-                  "fp8_quantize: out must be (float8_e4m3fn [rows][cols], uint8 [rows][ceil(cols / 128)])")
-    ldx, ldq, lds = (_fp8_pitch(t) for t in (x, q, s))
-    _fp8_call(lib.pi05_fp8_quantize, x.device, rows, cols, x.data_ptr(), int(x.dtype == torch.float32), ldx, q.data_ptr(), ldq,
-              s.data_ptr(), lds)
-    return q, s
-
-
-def _fp8_pitch(t):
-    """elements between rows; of a single row any pitch will do, so one that every check takes"""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
-
-
-def fp8_linear(x, x_scales, w, w_scales, epi="store", bias=None, res=None, gate=None, out=None):
-    """pi05_fp8_linear: epilogue(x . w^T) of two quantised operands (fp8_quantize's outputs: x [T][K], w [F][K]); epi
-    "store", "gelu", "resid", "gated", "geglu" (w rows interleaved gate/up) or "f32"; bias, gate [F], res [T][F] bf16.
-    Returns bf16 [T][F] ([T][F/2] for geglu, fp32 for f32); `out` may be given, and may be res."""
-    import torch
-
-    e4m3, u8, bf = torch.float8_e4m3fn, torch.uint8, torch.bfloat16
-    _fp8_need(x.is_cuda and x.dtype == e4m3 and w.dtype == e4m3 and x_scales.dtype == u8 and w_scales.dtype == u8,
-              "fp8_linear: x, w must be CUDA float8_e4m3fn tensors, their scales uint8")
-    _fp8_need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.numel() > 0 and w.numel() > 0,
-              "fp8_linear: x [T][K] and w [F][K] must agree in K and not be empty")
-    T, K = x.shape
-    F = w.shape[0]
-    blocks = (K + 127) // 128
-    _fp8_need(x_scales.shape == (T, blocks) and w_scales.shape == (F, blocks),
-              "fp8_linear: scales must be [rows][ceil(K / 128)]")
-    for t in (x, w, x_scales, w_scales):
-        _fp8_need(t.stride(1) == 1 or t.shape[1] == 1, "fp8_linear: rows of the operands and scales must be contiguous")
-    _fp8_need(epi in Engine.EPI, f"fp8_linear: unknown epilogue {epi!r}")
-    _fp8_need(epi != "geglu" or F % 2 == 0, "fp8_linear: geglu needs an even F")
-    for t, shape, what in ((bias, (F,), "bias [F]"), (gate, (F,), "gate [F]"), (res, (T, F), "res [T][F]")):
-        _fp8_need(t is None or (t.dtype == bf and t.shape == shape and t.is_contiguous()),
-                  f"fp8_linear: {what} must be contiguous bf16")
-    shape, dtype = (T, F // 2 if epi == "geglu" else F), torch.float32 if epi == "f32" else bf
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
-    _fp8_need(out.dtype == dtype and out.shape == shape and out.is_contiguous(),
-              f"fp8_linear: out must be contiguous {dtype} {list(shape)}")
-    _fp8_same(x.device, x_scales, w, w_scales, bias, res, gate, out)
-    _fp8_call(lib.pi05_fp8_linear, x.device, T, F, K, x.data_ptr(), _fp8_pitch(x), x_scales.data_ptr(), _fp8_pitch(x_scales),
-              w.data_ptr(), _fp8_pitch(w), w_scales.data_ptr(), _fp8_pitch(w_scales), _fp8_addr(bias), _fp8_addr(res),
-              _fp8_addr(gate), Engine.EPI[epi], out.data_ptr())
-    return out
-
-
-def fp8_status(device=None):
-    """pi05_fp8_status: waits for the current torch stream of `device`; raises Pi05Error(ERR_DEVICE) if a device-side wait of
-    an 8-bit operator there has given up since the last call."""
-    import torch
-
-    _fp8_call(lib.pi05_fp8_status, torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device))
-
-
-def _kv8_cache(what, dev, k8, k_scales, v8, v_scales, slots, batch):
-    import torch
-
-    _fp8_need(k8.dim() == 4 and k8.shape == v8.shape and k_scales.shape == v_scales.shape == k8.shape[:3],
-              f"{what}: codes must be [slots][capacity][kv_heads][head_dim], scales [slots][capacity][kv_heads]")
-    _fp8_need(k8.dtype == v8.dtype == torch.float8_e4m3fn and k_scales.dtype == v_scales.dtype == torch.uint8,
-              f"{what}: codes must be float8_e4m3fn, scales uint8")
-    _fp8_need(k8.is_contiguous() and v8.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous(),
-              f"{what}: the cache must be contiguous")
-    _fp8_same(dev, k8, k_scales, v8, v_scales)
-    _kv8_index(what, dev, batch, slots=slots)
-
-
-def _kv8_index(what, dev, batch, **tensors):
-    import torch
-
-    for name, t in tensors.items():
-        _fp8_need(t is None or (t.dtype == torch.int32 and t.shape == (batch,) and t.is_contiguous() and t.device == dev),
-                  f"{what}: {name} must be a contiguous int32 tensor [batch] on {dev}")
-
-
-def _kv8_rows(what, k, v, k8):
-    import torch
-
-    _fp8_need(k.is_cuda and k.dtype == v.dtype == torch.bfloat16 and k.dim() == 4 and k.shape == v.shape and k.numel() > 0
-              and k.shape[2:] == k8.shape[2:] and k.device == v.device,
-              f"{what}: k, v must be CUDA bf16 tensors [batch][T][kv_heads][head_dim] of the cache's heads")
-    h, d = k.shape[2:]
-    for t in (k, v):
-        _fp8_need(t.stride(3) == 1 and (h == 1 or t.stride(2) == d) and t.stride() == k.stride(),
-                  f"{what}: the heads of k, v must be contiguous and both strided alike")
-    return _kv8_strides(k)
-
-
-def _kv8_strides(t):
-    """(sample, token) strides of [batch][T][heads][head_dim]; along an axis of length 1 any stride will do"""
-    token = t.stride(1) if t.shape[1] > 1 else t.shape[2] * t.shape[3]
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * token), token
-
-
-def kv8_write(k, v, k8, k_scales, v8, v_scales, start=None, count=None, slots=None):
-    """pi05_kv8_write: quantises k, v (bf16 [batch][T][kv_heads][head_dim]) into the cache (k8, v8 float8_e4m3fn
-    [slots][capacity][kv_heads][head_dim], scales uint8 [slots][capacity][kv_heads]): sample b's rows t < count[b] go to
-    positions start[b] + t of slot slots[b].  start, count, slots: int32 CUDA tensors [batch] or None."""
-    sb, st = _kv8_rows("kv8_write", k, v, k8)
-    batch, T, h, d = k.shape
-    _kv8_cache("kv8_write", k.device, k8, k_scales, v8, v_scales, slots, batch)
-    _kv8_index("kv8_write", k.device, batch, start=start, count=count)
-    _fp8_call(lib.pi05_kv8_write, k.device, batch, T, h, d, k.data_ptr(), v.data_ptr(), sb, st, k8.shape[0], k8.shape[1],
-              k8.data_ptr(), k_scales.data_ptr(), v8.data_ptr(), v_scales.data_ptr(), _fp8_addr(start), _fp8_addr(count),
-              _fp8_addr(slots))
-
-
-def kv8_read(k8, k_scales, v8, v_scales, start=None, T=None, count=None, slots=None, out=None):
-    """pi05_kv8_read: positions start[b] + t, t < count[b] <= T, of slot slots[b] back as bf16 (k, v) [batch][T][kv_heads]
-    [head_dim].  The batch is that of start, count or slots (else every slot), T defaults to the capacity.  Rows that are not
-    read keep what `out` = (k, v) held (0 in new tensors)."""
-    import torch
-
-    n = next((t.shape[0] for t in (start, count, slots) if t is not None), k8.shape[0])
-    T = k8.shape[1] if T is None else T
-    if out is None:
-        shape = (n, T) + tuple(k8.shape[2:])
-        out = tuple(torch.zeros(shape, dtype=torch.bfloat16, device=k8.device) for _ in range(2))
-    k, v = out
-    sb, st = _kv8_rows("kv8_read", k, v, k8)
-    _fp8_need(k.shape[:2] == (n, T), "kv8_read: out must be [batch][T][kv_heads][head_dim]")
-    _kv8_cache("kv8_read", k.device, k8, k_scales, v8, v_scales, slots, n)
-    _kv8_index("kv8_read", k.device, n, start=start, count=count)
-    _fp8_call(lib.pi05_kv8_read, k.device, n, T, k8.shape[2], k8.shape[3], k.data_ptr(), v.data_ptr(), sb, st, k8.shape[0],
-              k8.shape[1], k8.data_ptr(), k_scales.data_ptr(), v8.data_ptr(), v_scales.data_ptr(), _fp8_addr(start),
-              _fp8_addr(count), _fp8_addr(slots))
-    return k, v
-
-
-def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False, scale=None, out=None):
-    """pi05_kv8_attention: attention of q (bf16 [batch][T][heads][head_dim], samples and tokens may be strided) over the
-    first lens[b] positions of slot slots[b]; causal: token t sees lens[b] - T + t + 1 of them.  scale defaults to
-    head_dim^-0.5.  Returns bf16 [batch][T][heads][head_dim]."""
-    import torch
-
-    _fp8_need(q.is_cuda and q.dtype == torch.bfloat16 and q.dim() == 4 and q.numel() > 0 and k8.dim() == 4
-              and q.shape[3] == k8.shape[3] and q.shape[2] % k8.shape[2] == 0,
-              "kv8_attention: q must be a CUDA bf16 tensor [batch][T][heads][head_dim], heads a multiple of the cache's")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    batch, T, heads, d = q.shape
-    for t in (q, out):
-        _fp8_need(t.dtype == torch.bfloat16 and t.shape == q.shape and t.stride(3) == 1 and (heads == 1 or t.stride(2) == d),
-                  "kv8_attention: q and out must be bf16 of one shape with contiguous heads")
-    _kv8_cache("kv8_attention", q.device, k8, k_scales, v8, v_scales, slots, batch)
-    _kv8_index("kv8_attention", q.device, batch, lens=lens)
-    _fp8_need(lens is not None, "kv8_attention: lens is required")
-    _fp8_same(q.device, out)
-    kvh, cap = k8.shape[2], k8.shape[1]
-    need = lib.pi05_kv8_attention_workspace(batch, T, heads, kvh, d, cap)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    (qb, qt), (ob, ot) = _kv8_strides(q), _kv8_strides(out)
-    _fp8_call(lib.pi05_kv8_attention, q.device, batch, T, heads, kvh, d, q.data_ptr(), qb, qt, k8.shape[0], cap, k8.data_ptr(),
-              k_scales.data_ptr(), v8.data_ptr(), v_scales.data_ptr(), lens.data_ptr(), _fp8_addr(slots), int(causal),
-              d**-0.5 if scale is None else scale, out.data_ptr(), ob, ot, _fp8_addr(ws), max(need, 0))
-    return out
+        globals().update((n, getattr(pi05fp8, n)) for n in _FP8_NAMES)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def bf16_bits_to_f32(bits):
