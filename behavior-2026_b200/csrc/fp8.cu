@@ -15,6 +15,7 @@
 #include "fp8.cuh"
 #include "fp8_gemm.cuh"
 #include "kv8_attention.cuh"
+#include "kv8_attention_tc.cuh"
 
 using namespace p5;
 
@@ -234,11 +235,13 @@ bool tmap(CUtensorMap* m, const void* base, long rows, int K, long ld, int box_r
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool set_smem(const void* f, int bytes) {
+  return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+
 template <int EPI>
 bool linear_attributes() {
-  auto set = [](const void* f, int bytes) {
-    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-  };
+  auto set = set_smem;
   return set((const void*)fp8_few_kernel<32, EPI>, Fp8FewCfg<32>::SMEM) &&
          set((const void*)fp8_few_kernel<64, EPI>, Fp8FewCfg<64>::SMEM) &&
          set((const void*)fp8_few_kernel<128, EPI>, Fp8FewCfg<128>::SMEM) &&
@@ -262,7 +265,12 @@ int setup(char* err, size_t err_len, int* sms) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2 || !linear_attributes<FP8_STORE>() ||
         !linear_attributes<FP8_GELU>() || !linear_attributes<FP8_RESID>() || !linear_attributes<FP8_GATED>() ||
-        !linear_attributes<FP8_GEGLU>() || !linear_attributes<FP8_F32>())
+        !linear_attributes<FP8_GEGLU>() || !linear_attributes<FP8_F32>() ||
+        !set_smem((const void*)kv8_attn_tc_kernel<128>, Kv8TcCfg<128>::SMEM) ||
+        !set_smem((const void*)kv8_attn_tc_kernel<256>, Kv8TcCfg<256>::SMEM) ||
+        !set_smem((const void*)kv8_attn_rows_kernel<64>, Kv8RowsCfg<64>::SMEM) ||
+        !set_smem((const void*)kv8_attn_rows_kernel<128>, Kv8RowsCfg<128>::SMEM) ||
+        !set_smem((const void*)kv8_attn_rows_kernel<256>, Kv8RowsCfg<256>::SMEM))
       return fail(err, err_len, PI05_ERR_CUDA, "preparing the 8-bit kernels failed: %s", cudaGetErrorString(cudaGetLastError()));
     g_sms[dev] = n;
   }
@@ -368,17 +376,72 @@ int num_sms() {
   return n;
 }
 
-int attn_splits(int batch, int T, int heads, int kv_heads, int capacity) {
-  const long tiles = (long)batch * kv_heads * (((long)T * (heads / kv_heads) + 7) / 8);
-  const int max_useful = std::max(1, capacity / 256);
-  return (int)std::max<long>(1, std::min<long>({(long)max_useful, 2L * num_sms() / tiles, 64L}));
+struct AttentionPlan {
+  bool tc;              // kv8_attn_tc_kernel (128 rows a CTA) or kv8_attn_rows_kernel (8)
+  int splits, cluster;  // key splits, CTAs of a cluster (splits is a multiple)
+};
+
+// By sizes that the host knows (the lengths are on the device): key splits fill the machine once where the cache allows a
+// CTA at least 128 keys; of the rows kernel in clusters of up to 8, so that up to 8 splits need no second kernel.
+AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
+  const long rows = (long)T * (heads / kv_heads), pairs = (long)batch * kv_heads;
+  const bool tc = head_dim >= 128 && rows > 32;
+  if (tc) {
+    const long tiles = pairs * ((rows + 127) / 128);
+    const long splits = std::max<long>(1, std::min<long>(((long)capacity + 127) / 128, num_sms() / tiles));
+    return {true, (int)splits, 1};
+  }
+  const long tiles = pairs * ((rows + 7) / 8);
+  const long places = (long)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
+  long splits = std::max<long>(1, std::min<long>({((long)capacity + 127) / 128, places / tiles, 256L}));
+  int cluster = 1;
+  while (cluster < 8 && 2 * cluster <= splits) cluster *= 2;
+  return {false, (int)(splits / cluster * cluster), cluster};
+}
+
+// [slots][capacity][kv_heads][head_dim] codes in boxes of 64 positions x 128 bytes of one head
+bool cache_map(CUtensorMap* m, const void* base, const Kv8Args& a, int head_dim) {
+  const cuuint64_t head = head_dim, pos = head * a.kv_heads;
+  cuuint64_t dims[4] = {head, (cuuint64_t)a.kv_heads, (cuuint64_t)a.capacity, (cuuint64_t)a.n_slots};
+  cuuint64_t strides[3] = {head, pos, pos * a.capacity};
+  cuuint32_t box[4] = {128, 1, 64, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int HD>
-int attention(const Kv8Args& a, int batch, cudaStream_t st, char* err, size_t err_len) {
-  const dim3 grid((a.T * a.G + 7) / 8, batch * a.kv_heads, a.splits);
-  kv8_attn_rows_kernel<HD, 1, 4><<<grid, 128, 0, st>>>(a);
-  if (a.splits > 1) {
+int attention_tc(const Kv8Args& a, int batch, cudaStream_t st, char* err, size_t err_len) {
+  CUtensorMap tk, tv;
+  if (!cache_map(&tk, a.k, a, HD) || !cache_map(&tv, a.v, a, HD))
+    return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: tensor map rejected the cache");
+  const dim3 grid((unsigned)(((long)a.T * a.G + 127) / 128), batch * a.kv_heads, a.splits);
+  kv8_attn_tc_kernel<HD><<<grid, Kv8TcCfg<HD>::THREADS, Kv8TcCfg<HD>::SMEM, st>>>(tk, tv, a);
+  if (a.groups > 1) {
+    const long rows = (long)batch * a.T * a.heads;
+    kv8_attn_combine_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, batch);
+  }
+  return launched("pi05_kv8_attention", err, err_len);
+}
+
+template <int HD>
+int attention(const Kv8Args& a, int batch, int cluster, cudaStream_t st, char* err, size_t err_len) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.T * a.G + 7) / 8, batch * a.kv_heads, a.splits);
+  cfg.blockDim = dim3(32 * Kv8RowsCfg<HD>::W);
+  cfg.dynamicSmemBytes = Kv8RowsCfg<HD>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = cluster;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  void* params[] = {const_cast<Kv8Args*>(&a)};
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, (const void*)kv8_attn_rows_kernel<HD>, params);
+  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_kv8_attention: %s", cudaGetErrorString(e));
+  if (a.groups > 1) {
     const long rows = (long)batch * a.T * a.heads;
     kv8_attn_combine_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, batch);
   }
@@ -500,8 +563,9 @@ extern "C" PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int h
   if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || capacity < 1 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return PI05_ERR_ARG;
-  const int64_t splits = attn_splits(batch, T, heads, kv_heads, capacity);
-  return splits == 1 ? 0 : splits * batch * T * heads * ((int64_t)head_dim * 4 + 8);
+  const AttentionPlan p = attention_plan(batch, T, heads, kv_heads, head_dim, capacity);
+  const int64_t groups = p.splits / p.cluster;
+  return groups == 1 ? 0 : groups * batch * T * heads * ((int64_t)head_dim * 4 + 8);
 }
 
 extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_heads, int head_dim, const void* q,
@@ -524,6 +588,8 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
                 "pi05_kv8_attention: q, out and the caches must be 16-byte aligned device pointers, tokens of q and out "
                 "at least heads * head_dim elements and a multiple of 8 apart, samples of out not overlapping");
   if (!slots && batch > n_slots) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: batch exceeds the cache's slots");
+  if ((int64_t)kv_heads * head_dim * capacity >= (1LL << 40))
+    return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: a slot of the cache must be smaller than 2^40 bytes");
   if (!(scale == scale) || scale - scale != 0.f) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: scale must be finite");
   Kv8Args a = {};
   a.q = static_cast<const bf16*>(q);
@@ -546,16 +612,23 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
   a.kv_heads = kv_heads;
   a.G = heads / kv_heads;
   a.causal = causal != 0;
-  a.splits = attn_splits(batch, T, heads, kv_heads, capacity);
+  const AttentionPlan plan = attention_plan(batch, T, heads, kv_heads, head_dim, capacity);
+  a.splits = plan.splits;
+  a.groups = plan.splits / plan.cluster;
   const int64_t need = pi05_kv8_attention_workspace(batch, T, heads, kv_heads, head_dim, capacity);
   if (need > 0) {
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
       return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
     a.ws_o = static_cast<float*>(workspace);
-    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + (int64_t)a.splits * batch * T * heads * head_dim);
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + (int64_t)a.groups * batch * T * heads * head_dim);
   }
+  int sms = 0;
+  const int rc = setup(err, err_len, &sms);
+  if (rc != PI05_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 64) return attention<64>(a, batch, st, err, err_len);
-  if (head_dim == 128) return attention<128>(a, batch, st, err, err_len);
-  return attention<256>(a, batch, st, err, err_len);
+  if (plan.tc)
+    return head_dim == 128 ? attention_tc<128>(a, batch, st, err, err_len) : attention_tc<256>(a, batch, st, err, err_len);
+  if (head_dim == 64) return attention<64>(a, batch, plan.cluster, st, err, err_len);
+  if (head_dim == 128) return attention<128>(a, batch, plan.cluster, st, err, err_len);
+  return attention<256>(a, batch, plan.cluster, st, err, err_len);
 }

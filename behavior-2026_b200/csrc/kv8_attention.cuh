@@ -2,18 +2,22 @@
 //
 //   out[b][t][h][:] = sum_j p_j V_j,  p = softmax_j(scale * q . K_j),  j < lens[b] (causal: j < lens[b] - T + t + 1)
 //
-// The query heads of a K/V head and the T tokens of a sample are folded into rows r = t * G + g.  A CTA owns
-// 8 * NT rows of one (sample, K/V head) and one key split; its warps walk 16-key steps, each warp the steps
-// w, w + W, ... of the split with a running maximum and sum of its own, merged through shared memory at the end.
+// The query heads of a K/V head and the T tokens of a sample are folded into rows r = t * G + g.  A CTA owns 8 of the
+// rows of one (sample, K/V head) and one key split; its warps walk steps of 32 keys, each warp the steps w, w + W, ... of the
+// split with a running maximum and sum of its own, merged through shared memory at the end, then over the cluster's
+// CTAs (the neighbouring splits) through distributed shared memory, then, where there are more splits than a cluster
+// holds, by kv8_attn_combine_kernel.
+//
+// One new token reads the whole cache once for a handful of products, so what counts is bytes in flight: each warp
+// keeps a ring of its own of STAGES steps (cp.async, no barrier between warps), 48 to 192 KB an SM.
 //
 // Everything is computed transposed, keys and head dims on the 16-row side of mma.m16n8k16 and query rows on
 // the 8-column side, because one token of 8 heads has 8 rows, not 16:
 //   S^T[16 keys][8 rows] = K Q^T      O^T[16 dims][8 rows] += V^T P^T
 // The order of the reduction index and of the output rows of an MMA is free, so each thread takes the operands
-// that it can load in 16-byte pieces: lane (g, c) = (lane / 4, lane % 4) holds head dims 64 i + 16 c .. + 15 of
-// keys g and g + 8, and head dims 128 i + 16 g .. + 15 of keys 2c, 2c + 1, 2c + 8, 2c + 9.  K and V go from
-// global memory to registers, are widened to fp16 there (exact) and never touch shared memory.  P^T goes
-// from the accumulator layout to the operand layout by movmatrix.
+// that it can read in 16-byte pieces: lane (g, c) = (lane / 4, lane % 4) holds head dims 64 i + 16 c .. + 15 of
+// keys g and g + 8, and head dims 128 i + 16 g .. + 15 of keys 2c, 2c + 1, 2c + 8, 2c + 9, widened to fp16 in
+// registers (exact).  P^T goes from the accumulator layout to the operand layout by movmatrix.
 //
 // fp16 operands: a query row is scaled by a power of two so that its largest element is near 2^15 (elements
 // down to 2^-29 of it keep all 8 bits of a bf16); P carries the V row's scale relative to a running exponent
@@ -35,9 +39,9 @@ struct Kv8Args {
   long o_b, o_t;
   float scale_log2;  // scale * log2(e)
   int n_slots, capacity, T, heads, kv_heads, G, causal;
-  int splits;
-  float* ws_o;   // [splits][batch][heads * T][head_dim], O in units of the split's 2^m
-  float2* ws_ml; // [splits][batch][heads * T] (m, l)
+  int splits, groups;  // key splits, and clusters of them: splits = groups * CTAs of a cluster
+  float* ws_o;         // [groups][batch][heads * T][head_dim], O in units of the group's 2^m
+  float2* ws_ml;       // [groups][batch][heads * T] (m, l)
 };
 
 __device__ __forceinline__ uint32_t movmatrix_b16(uint32_t v) {
@@ -51,326 +55,389 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
 // 2^n for any integer n (0 below 2^-127, 2^127 above)
 __device__ __forceinline__ float exp2_int(int n) {
   return n < -127 ? 0.f : __uint_as_float(n == -127 ? 0x400000u : (uint32_t)(min(n, 127) + 127) << 23);
 }
 
-template <int HD, int NT, int W>
-__global__ void __launch_bounds__(32 * W)
+template <int HD>
+struct Kv8RowsCfg {
+  static constexpr int W = 4, KEYS = 32, STAGES = 3;
+  static constexpr int HALF = KEYS * HD, STAGE = 2 * HALF;  // bytes of a step: K rows, V rows
+  static constexpr int SMEM = W * STAGES * STAGE;
+  static constexpr int PER_SM = HD == 256 ? 1 : (HD == 128 ? 2 : 4);
+  static_assert(8 * HD * 4 <= STAGES * STAGE, "a warp's O tile is staged in its ring");
+};
+
+// byte offset of 16-byte piece p of key row `key` of a stage.  Pieces are swizzled so that the eight lanes of a
+// 16-byte (V of HD 64: sixteen of an 8-byte) access hit different banks: K pieces 4 i + c of keys g, g + 1, V pieces g, g + 1 of
+// keys 2 c.
+template <int HD>
+__device__ __forceinline__ int kv8_k_at(int key, int p) {
+  return HD == 64 ? key * 64 + p * 16 : key * HD + ((p ^ ((key & 1) << 2)) << 4);
+}
+template <int HD>
+__device__ __forceinline__ int kv8_v_at(int key, int p) {
+  return HD == 64 ? (key >> 1) * 128 + (((key & 1) ^ ((key >> 1) & 1)) << 6) + ((p ^ (((key >> 2) & 1) << 1)) << 4)
+                  : key * HD + ((p ^ (key & 6)) << 4);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM)
     kv8_attn_rows_kernel(const Kv8Args a) {
-  constexpr int KI = HD / 64;                      // 16-byte K pieces of a key per lane
-  constexpr int VI = HD >= 128 ? HD / 128 : 1;     // 16-byte V pieces of a key per lane (HD 64: 8 bytes)
-  constexpr int VB = HD >= 128 ? 16 : 8;           // bytes of a V piece
-  constexpr int MT = HD / 16;                      // 16-dim tiles of O^T
-  constexpr int R = 8 * NT;
-  __shared__ float sm_o[R][HD + 4];
-  __shared__ float sm_m[W][R], sm_l[W][R];
+  using C = Kv8RowsCfg<HD>;
+  constexpr int W = C::W, KI = HD / 64, VI = HD >= 128 ? HD / 128 : 1;
+  constexpr int VB = HD >= 128 ? 16 : 8;  // bytes of a lane's V piece
+  constexpr int MT = HD / 16;             // 16-dim tiles of O^T
+  constexpr int PIECES = HD / 16;         // 16-byte pieces of a key row
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sm_m[W][8], sm_l[W][8];
   __shared__ int sm_e[W];
+  __shared__ float cta_m[8], cta_l[8];
+  __shared__ int cta_e;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-  const int rows = a.T * a.G, row0 = blockIdx.x * R;
+  const int rows = a.T * a.G, row0 = blockIdx.x * 8;
   const int split = blockIdx.z;
   const int slot = a.slots ? a.slots[b] : b;
   const int len = (slot < 0 || slot >= a.n_slots) ? 0 : max(0, min(a.lens[b], a.capacity));
   // keys that any of the CTA's rows sees
-  const int t_last = min(row0 + R, rows) - 1;
+  const int t_last = min(row0 + 8, rows) - 1;
   const int top = a.causal ? max(0, min(len, len - a.T + t_last / a.G + 1)) : len;
-  // the split's steps of 16 keys
-  const int steps = (top + 15) >> 4;
+  // the split's steps
+  const int steps = (top + C::KEYS - 1) / C::KEYS;
   const int per = (steps + a.splits - 1) / a.splits;
   const int s_begin = min(split * per, steps), s_end = min(s_begin + per, steps);
 
-  // ---- Q^T operand: row g of each 8-row tile, scaled to fp16
-  uint32_t qf[NT][KI][8];
-  float rf[NT][2];  // this thread's accumulator columns: rows 2c, 2c + 1 of each tile
-  int lim[NT][2];
+  const long key_pitch = (long)a.kv_heads * HD;
+  const long cache0 = (long)slot * a.capacity * a.kv_heads + kvh;  // in heads
+  const uint8_t* kp = a.k + cache0 * HD;
+  const uint8_t* vp = a.v + cache0 * HD;
+  const uint8_t* ksp = a.ks + cache0;
+  const uint8_t* vsp = a.vs + cache0;
+  uint8_t* ring = smem + warp * C::STAGES * C::STAGE;
+
+  // One step's K and V rows into a stage (keys from `top` on become zeros), and this lane's scale bytes: K and V of
+  // key `lane`.  255 where there is no key: no exponent of its own, and its p is 0.
+  int kq[C::STAGES], vq[C::STAGES];
+  auto fetch = [&](int step, int st) {
+    if (step < s_end) {
+      const int key0 = step * C::KEYS;
+      uint8_t* dst = ring + st * C::STAGE;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = row0 + 8 * n + g;
+      for (int i = 0; i < PIECES; ++i) {
+        const int q = i * 32 + lane, key = q / PIECES, p = q % PIECES;
+        const bool in = key0 + key < top;
+        const long off = in ? (long)(key0 + key) * key_pitch + 16 * p : 0;
+        cp_async16(dst + kv8_k_at<HD>(key, p), kp + off, in);
+        cp_async16(dst + C::HALF + kv8_v_at<HD>(key, p), vp + off, in);
+      }
+      const bool in = key0 + lane < top;
+      kq[st] = in ? (int)ksp[(long)(key0 + lane) * a.kv_heads] : 255;
+      vq[st] = in ? (int)vsp[(long)(key0 + lane) * a.kv_heads] : 255;
+    }
+    cp_async_commit();
+  };
+  int step = s_begin + warp;
+#pragma unroll
+  for (int i = 0; i < C::STAGES - 1; ++i) fetch(step + i * W, i);
+
+  // ---- Q^T operand: row g, scaled to fp16
+  uint32_t qf[KI][8];
+  float rf[2];  // this thread's accumulator columns: rows 2c, 2c + 1
+  int lim[2];
+  {
+    const int r = row0 + g;
     const bool in = r < rows;
     const int t = in ? r / a.G : 0, h = kvh * a.G + (in ? r % a.G : 0);
     const bf16* src = a.q + (long)b * a.q_b + (long)t * a.q_t + (long)h * HD;
-    uint32_t raw[KI][8];
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint4 u = in ? *reinterpret_cast<const uint4*>(src + 64 * i + 16 * c + 8 * j) : make_uint4(0, 0, 0, 0);
-        raw[i][4 * j] = u.x, raw[i][4 * j + 1] = u.y, raw[i][4 * j + 2] = u.z, raw[i][4 * j + 3] = u.w;
+        qf[i][4 * j] = u.x, qf[i][4 * j + 1] = u.y, qf[i][4 * j + 2] = u.z, qf[i][4 * j + 3] = u.w;
       }
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 f = unpack_bf2(raw[i][j]);
+        const float2 f = unpack_bf2(qf[i][j]);
         m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
       }
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // e: |q| < 2^(e + 1); rows are scaled by 2^(14 - e) (kept within the float range)
+    // |q| < 2^(e + 1); the row is scaled by 2^(14 - e) (kept within the float range)
     const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -112), 127);
     const float up = exp2_int(14 - e);
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 f = unpack_bf2(raw[i][j]);
+        const float2 f = unpack_bf2(qf[i][j]);
         const __half2 hh = __floats2half2_rn(f.x * up, f.y * up);
-        qf[n][i][j] = *reinterpret_cast<const uint32_t*>(&hh);
+        qf[i][j] = *reinterpret_cast<const uint32_t*>(&hh);
       }
     const float down = a.scale_log2 * exp2_int(e - 14);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      rf[n][j] = __shfl_sync(0xffffffffu, down, (2 * c + j) * 4);
-      const int rr = row0 + 8 * n + 2 * c + j;
-      lim[n][j] = rr >= rows ? 0 : (a.causal ? min(len, len - a.T + rr / a.G + 1) : len);
+      rf[j] = __shfl_sync(0xffffffffu, down, (2 * c + j) * 4);
+      const int rr = row0 + 2 * c + j;
+      lim[j] = rr >= rows ? 0 : (a.causal ? min(len, len - a.T + rr / a.G + 1) : len);
     }
   }
 
-  float o[NT][MT][4];
-  float m_run[NT][2], l_run[NT][2];
+  float o[MT][4];
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   int eb = -1000;  // exponent of the V scales that O is in units of
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_run[n][0] = m_run[n][1] = -INFINITY;
-    l_run[n][0] = l_run[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-  }
+  for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  const long key_pitch = (long)a.kv_heads * HD;
-  const long cache0 = ((long)slot * a.capacity * a.kv_heads + kvh);  // in heads
-  const uint8_t* kp = a.k + cache0 * HD;
-  const uint8_t* vp = a.v + cache0 * HD;
-  const uint8_t* ksp = a.ks + cache0;
-  const uint8_t* vsp = a.vs + cache0;
-
-  uint4 kr[2][KI], vr[4][VI];
-  int kb[2], vb[2];
-  auto load_k = [&](int step) {
+  for (; step < s_end;) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int key = step * 16 + g + 8 * j;
-      const bool in = key < top;
-      kb[j] = in ? (int)ksp[(long)key * a.kv_heads] : 127;
-      vb[j] = in ? (int)vsp[(long)key * a.kv_heads] : 255;  // no exponent of its own; p is 0
+    for (int st = 0; st < C::STAGES; ++st) {
+      if (step >= s_end) break;
+      cp_async_wait<C::STAGES - 2>();
+      __syncwarp();
+      // the stage of the step before last is free: every lane has read it
+      fetch(step + (C::STAGES - 1) * W, (st + C::STAGES - 1) % C::STAGES);
+      const uint8_t* sk = ring + st * C::STAGE;
+      const uint8_t* sv = sk + C::HALF;
+      // ---- S^T = K Q^T, two chains a 16-key tile
+      float s[2][4], s2[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
       for (int i = 0; i < KI; ++i)
-        kr[j][i] = in ? ldg_stream(kp + key * key_pitch + 64 * i + 16 * c) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  auto load_v = [&](int step) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = step * 16 + 2 * c + (j & 1) + 8 * (j >> 1);
-      const bool in = key < top;
+        for (int n = 0; n < 2; ++n) {
+          const uint4 u0 = *reinterpret_cast<const uint4*>(sk + kv8_k_at<HD>(16 * n + g, 4 * i + c));
+          const uint4 u1 = *reinterpret_cast<const uint4*>(sk + kv8_k_at<HD>(16 * n + g + 8, 4 * i + c));
+          const uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        if (VB == 16) {
-          vr[j][i] = in ? ldg_stream(vp + key * key_pitch + 128 * i + 16 * g) : make_uint4(0, 0, 0, 0);
-        } else {
-          const uint2 u = in ? *reinterpret_cast<const uint2*>(vp + key * key_pitch + 8 * g) : make_uint2(0, 0);
-          vr[j][i] = make_uint4(u.x, u.y, 0, 0);
+          for (int p = 0; p < 4; ++p) {
+            const uint32_t af[4] = {fp8_to_h2((uint16_t)w0[p]), fp8_to_h2((uint16_t)w1[p]), fp8_to_h2((uint16_t)(w0[p] >> 16)),
+                                    fp8_to_h2((uint16_t)(w1[p] >> 16))};
+            mma_f16_16816(p & 1 ? s2[n] : s[n], af, qf[i][2 * p], qf[i][2 * p + 1]);
+          }
         }
-      }
-    }
-  };
-
-  int step = s_begin + warp;
-  if (step < s_end) {
-    load_k(step);
-    load_v(step);
-  }
-  for (; step < s_end; step += W) {
-    // ---- S^T = K Q^T
-    float s[NT][4];
+      // ---- logits in base 2; a cached NaN row (scale byte 255) makes the rows that see it NaN
+      const int key0 = step * C::KEYS + g;
+      int ev[2][2];
+      bool grow = false;
+      int em = -1000;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const uint32_t w0[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w};
-      const uint32_t w1[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
+        for (int q = 0; q < 2; ++q) {
+          const int kb = __shfl_sync(0xffffffffu, kq[st], 16 * n + 8 * q + g), vb = __shfl_sync(0xffffffffu, vq[st], 16 * n + 8 * q + g);
+          const float kf = (kb == 255 || vb == 255) ? NAN : fp8_scale_value(kb);
+          ev[n][q] = vb == 255 ? -1000 : vb - 127;
+          em = max(em, ev[n][q]);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const uint32_t af[4] = {fp8_to_h2((uint16_t)w0[p]), fp8_to_h2((uint16_t)w1[p]), fp8_to_h2((uint16_t)(w0[p] >> 16)),
-                                fp8_to_h2((uint16_t)(w1[p] >> 16))};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], af, qf[n][i][2 * p], qf[n][i][2 * p + 1]);
-      }
-    }
-    const int kb0 = kb[0], kb1 = kb[1], vb0 = vb[0], vb1 = vb[1];
-    const int key0 = step * 16 + g;
-    if (step + W < s_end) load_k(step + W);
-
-    // ---- logits in base 2; a cached NaN row (scale byte 255) makes the rows that see it NaN
-    const float kf0 = (kb0 == 255 || vb0 == 255) ? NAN : fp8_scale_value(kb0);
-    const float kf1 = (kb1 == 255 || vb1 == 255) ? NAN : fp8_scale_value(kb1);
-    bool grow = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+          for (int j = 0; j < 2; ++j) {
+            const float x = (s[n][2 * q + j] + s2[n][2 * q + j]) * rf[j] * kf;
+            s[n][2 * q + j] = key0 + 16 * n + 8 * q < lim[j] ? x : -INFINITY;
+          }
+        }
+      float mt[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float x0 = s[n][j] * rf[n][j] * kf0, x1 = s[n][2 + j] * rf[n][j] * kf1;
-        s[n][j] = key0 < lim[n][j] ? x0 : -INFINITY;
-        s[n][2 + j] = key0 + 8 < lim[n][j] ? x1 : -INFINITY;
-        grow |= fmaxf(s[n][j], s[n][2 + j]) > m_run[n][j] + 8.f;
+        mt[j] = fmaxf(fmaxf(s[0][j], s[0][2 + j]), fmaxf(s[1][j], s[1][2 + j]));
+        grow |= mt[j] > m_run[j] + 8.f;
       }
-    const int ev0 = vb0 == 255 ? -1000 : vb0 - 127, ev1 = vb1 == 255 ? -1000 : vb1 - 127;
-    grow |= max(ev0, ev1) > eb + 7;
-    if (__any_sync(0xffffffffu, grow)) {
-      int em = max(ev0, ev1);
+      grow |= em > eb + 7;
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) em = max(em, __shfl_xor_sync(0xffffffffu, em, d));
-      em = max(em, eb);
-      const float ealpha = exp2_int(eb - em);  // eb = -1000 at first: 0, O is 0 anyway
-      eb = em;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int d = 4; d < 32; d <<= 1) em = max(em, __shfl_xor_sync(0xffffffffu, em, d));
+        em = max(em, eb);
+        const float ealpha = exp2_int(eb - em);  // 0 at first, when O is 0 anyway
+        eb = em;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float m = fmaxf(s[n][j], s[n][2 + j]);
+          float m = mt[j];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-          m = fmaxf(m, m_run[n][j]);
-          const float alpha = m_run[n][j] == -INFINITY ? 0.f : ex2_approx(m_run[n][j] - m);
-          m_run[n][j] = m;
-          l_run[n][j] *= alpha;
+          m = fmaxf(m, m_run[j]);
+          const float alpha = m_run[j] == -INFINITY ? 0.f : ex2_approx(m_run[j] - m);
+          m_run[j] = m;
+          l_run[j] *= alpha;
           const float al = alpha * ealpha;
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            o[n][i][j] *= al;
-            o[n][i][2 + j] *= al;
+            o[i][j] *= al;
+            o[i][2 + j] *= al;
           }
         }
-    }
-    // ---- P^T, each key's V scale folded in
-    const float vf0 = exp2_int(ev0 - eb), vf1 = exp2_int(ev1 - eb);
-    uint32_t pf[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float p[4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float mm = m_run[n][j] == -INFINITY ? 0.f : m_run[n][j];
-        p[j] = ex2_approx(s[n][j] - mm);
-        p[2 + j] = ex2_approx(s[n][2 + j] - mm);
-        l_run[n][j] += p[j] + p[2 + j];
       }
-      const __half2 h0 = __floats2half2_rn(p[0] * vf0, p[1] * vf0), h1 = __floats2half2_rn(p[2] * vf1, p[3] * vf1);
-      pf[n][0] = movmatrix_b16(*reinterpret_cast<const uint32_t*>(&h0));
-      pf[n][1] = movmatrix_b16(*reinterpret_cast<const uint32_t*>(&h1));
-    }
-    // ---- O^T += V^T P^T: tile (i, j) holds dims 16 g + 2 j and + 1 of the 128-dim part i
+      // ---- P^T, each key's V scale folded in
+      uint32_t pf[2][2];
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const uint32_t w[4][4] = {{vr[0][i].x, vr[0][i].y, vr[0][i].z, vr[0][i].w},
-                                {vr[1][i].x, vr[1][i].y, vr[1][i].z, vr[1][i].w},
-                                {vr[2][i].x, vr[2][i].y, vr[2][i].z, vr[2][i].w},
-                                {vr[3][i].x, vr[3][i].y, vr[3][i].z, vr[3][i].w}};
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int q = 0; q < VB / 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
+          const float vf = exp2_int(ev[n][q] - eb);
+          float p[2];
 #pragma unroll
-        for (int hlf = 0; hlf < 2; ++hlf) {
-          // bytes (2 hlf, 2 hlf + 1) of the word of two keys, interleaved by key
-          const uint32_t lo = __byte_perm(w[0][q], w[1][q], hlf ? 0x7362 : 0x5140);
-          const uint32_t hi = __byte_perm(w[2][q], w[3][q], hlf ? 0x7362 : 0x5140);
-          const uint32_t af[4] = {fp8_to_h2((uint16_t)lo), fp8_to_h2((uint16_t)(lo >> 16)), fp8_to_h2((uint16_t)hi),
-                                  fp8_to_h2((uint16_t)(hi >> 16))};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][i * (VB / 2) + 2 * q + hlf], af, pf[n][0], pf[n][1]);
+          for (int j = 0; j < 2; ++j) {
+            p[j] = ex2_approx(s[n][2 * q + j] - (m_run[j] == -INFINITY ? 0.f : m_run[j]));
+            l_run[j] += p[j];
+          }
+          const __half2 h = __floats2half2_rn(p[0] * vf, p[1] * vf);
+          pf[n][q] = movmatrix_b16(*reinterpret_cast<const uint32_t*>(&h));
         }
-      }
+      // ---- O^T += V^T P^T: tile (i, j) holds dims 16 g + 2 j and + 1 of the 128-dim part i
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int key = 16 * n + 2 * c + (k & 1) + 8 * (k >> 1);
+            if (VB == 16) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sv + kv8_v_at<HD>(key, 8 * i + g));
+              w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(sv + kv8_v_at<HD>(key, g >> 1) + (g & 1) * 8);
+              w[k][0] = u.x, w[k][1] = u.y;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < VB / 4; ++q)
+#pragma unroll
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              // bytes (2 hlf, 2 hlf + 1) of the word of two keys, interleaved by key
+              const uint32_t lo = __byte_perm(w[0][q], w[1][q], hlf ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(w[2][q], w[3][q], hlf ? 0x7362 : 0x5140);
+              const uint32_t af[4] = {fp8_to_h2((uint16_t)lo), fp8_to_h2((uint16_t)(lo >> 16)), fp8_to_h2((uint16_t)hi),
+                                      fp8_to_h2((uint16_t)(hi >> 16))};
+              mma_f16_16816(o[i * (VB / 2) + 2 * q + hlf], af, pf[n][0], pf[n][1]);
+            }
+        }
+      step += W;
     }
-    if (step + W < s_end) load_v(step + W);
   }
+  cp_async_wait<0>();
 
-  // ---- merge the warps: row maxima and exponents first, then O in warp order (reruns give the same bits)
+  // ---- merge the warps: maxima and exponents first, then O in warp order (reruns give the same bits)
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l_run[n][j] += __shfl_xor_sync(0xffffffffu, l_run[n][j], d);
+    for (int d = 4; d < 32; d <<= 1) l_run[j] += __shfl_xor_sync(0xffffffffu, l_run[j], d);
   if (g == 0) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sm_m[warp][8 * n + 2 * c + j] = m_run[n][j];
-        sm_l[warp][8 * n + 2 * c + j] = l_run[n][j];
-      }
+    for (int j = 0; j < 2; ++j) {
+      sm_m[warp][2 * c + j] = m_run[j];
+      sm_l[warp][2 * c + j] = l_run[j];
+    }
   }
   if (lane == 0) sm_e[warp] = eb;
   __syncthreads();
   int e_all = -1000;
 #pragma unroll
   for (int w = 0; w < W; ++w) e_all = max(e_all, sm_e[w]);
-  float fac[NT][2];
+  float* tile = reinterpret_cast<float*>(smem);  // [W][8][HD], each warp's in its own ring
+  constexpr int TILE = C::STAGES * C::STAGE / 4;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int j = 0; j < 2; ++j) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float m = -INFINITY;
+    for (int w = 0; w < W; ++w) m = fmaxf(m, sm_m[w][2 * c + j]);
+    const float f = m_run[j] == -INFINITY ? 0.f : ex2_approx(m_run[j] - m) * exp2_int(eb - e_all);
+    float* dst = tile + warp * TILE + (2 * c + j) * HD;
 #pragma unroll
-      for (int w = 0; w < W; ++w) m = fmaxf(m, sm_m[w][8 * n + 2 * c + j]);
-      fac[n][j] = m_run[n][j] == -INFINITY ? 0.f : ex2_approx(m_run[n][j] - m) * exp2_int(eb - e_all);
-    }
-#pragma unroll 1
-  for (int w = 0; w < W; ++w) {
-    if (warp == w) {
+    for (int i = 0; i < VI; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float* dst = sm_o[8 * n + 2 * c + j];
-#pragma unroll
-          for (int i = 0; i < VI; ++i)
-#pragma unroll
-            for (int q = 0; q < VB; ++q) {
-              const float x = o[n][i * (VB / 2) + q / 2][(q & 1) * 2 + j] * fac[n][j];
-              float* d = dst + 128 * i + VB * g + q;
-              *d = w == 0 ? x : *d + x;
-            }
-        }
-    }
-    __syncthreads();
+      for (int q = 0; q < VB; q += 4) {
+        const int k = i * (VB / 2) + q / 2;
+        *reinterpret_cast<float4*>(dst + 128 * i + VB * g + q) =
+            make_float4(o[k][j] * f, o[k][2 + j] * f, o[k + 1][j] * f, o[k + 1][2 + j] * f);
+      }
   }
-  const float unit = exp2_int(e_all);
-  const int out_rows = a.T * a.heads;
-  for (int r = warp; r < R; r += W) {
-    const int row = row0 + r;
-    if (row >= rows) continue;
+  if (threadIdx.x < 8) {
+    const int r = threadIdx.x;
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) m = fmaxf(m, sm_m[w][r]);
 #pragma unroll
     for (int w = 0; w < W; ++w) l += sm_m[w][r] == -INFINITY ? sm_l[w][r] : sm_l[w][r] * ex2_approx(sm_m[w][r] - m);  // 0 or NaN
+    cta_m[r] = m;
+    cta_l[r] = l;
+  }
+  if (threadIdx.x == 0) cta_e = e_all;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * HD; i += 32 * W) {  // 8 rows of HD in float4s, summed into the first warp's tile
+    float4 x = reinterpret_cast<const float4*>(tile)[i];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float4 y = reinterpret_cast<const float4*>(tile + w * TILE)[i];
+      x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    }
+    reinterpret_cast<float4*>(tile)[i] = x;
+  }
+
+  // ---- merge the cluster's CTAs: CTA p finishes rows p, p + size, ... , in rank order
+  const int size = a.splits / a.groups, rank = split % size, group = split / size;
+  if (size > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  const int out_rows = a.T * a.heads;
+  for (int r = rank + size * warp; r < 8; r += size * W) {
+    const int row = row0 + r;
+    if (row >= rows) continue;
+    float m = -INFINITY, l = 0.f, x[HD / 32];
+    int e = -1000;
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) x[k] = 0.f;
+    for (int p = 0; p < size; ++p) {
+      m = fmaxf(m, size > 1 ? ld_peer_f32(map_peer(smem_u32(&cta_m[r]), p)) : cta_m[r]);
+      e = max(e, size > 1 ? __float_as_int(ld_peer_f32(map_peer(smem_u32(&cta_e), p))) : cta_e);
+    }
+    for (int p = 0; p < size; ++p) {
+      const float mp = size > 1 ? ld_peer_f32(map_peer(smem_u32(&cta_m[r]), p)) : cta_m[r];
+      const float lp = size > 1 ? ld_peer_f32(map_peer(smem_u32(&cta_l[r]), p)) : cta_l[r];
+      const int ep = size > 1 ? __float_as_int(ld_peer_f32(map_peer(smem_u32(&cta_e), p))) : cta_e;
+      const float f = mp == -INFINITY ? 0.f : ex2_approx(mp - m);
+      l += mp == -INFINITY ? lp : lp * f;
+      const float fe = f * exp2_int(ep - e);
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k) {
+        const float* q = tile + r * HD + 64 * k + 2 * lane;
+        const uint32_t at = size > 1 ? map_peer(smem_u32(q), p) : 0u;
+        x[2 * k] += fe * (size > 1 ? ld_peer_f32(at) : q[0]);
+        x[2 * k + 1] += fe * (size > 1 ? ld_peer_f32(at + 4) : q[1]);
+      }
+    }
+    const float unit = exp2_int(e);
     const int t = row / a.G, h = kvh * a.G + row % a.G;
-    if (a.splits == 1) {
+    if (a.groups == 1) {
       // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
       const float inv = l == 0.f ? 0.f : unit / l;
       bf16* dst = a.out + (long)b * a.o_b + (long)t * a.o_t + (long)h * HD;
-      for (int d = 2 * lane; d < HD; d += 64)
-        *reinterpret_cast<uint32_t*>(dst + d) = pack_bf2(sm_o[r][d] * inv, sm_o[r][d + 1] * inv);
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k)
+        *reinterpret_cast<uint32_t*>(dst + 64 * k + 2 * lane) = pack_bf2(x[2 * k] * inv, x[2 * k + 1] * inv);
     } else {
-      const long i = ((long)split * (gridDim.y / a.kv_heads) + b) * out_rows + (long)h * a.T + t;
-      for (int d = lane; d < HD; d += 32) a.ws_o[i * HD + d] = sm_o[r][d] * unit;
+      const long i = ((long)group * (gridDim.y / a.kv_heads) + b) * out_rows + (long)h * a.T + t;
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k)
+        *reinterpret_cast<float2*>(a.ws_o + i * HD + 64 * k + 2 * lane) = make_float2(x[2 * k] * unit, x[2 * k + 1] * unit);
       if (lane == 0) a.ws_ml[i] = make_float2(m, l);
     }
   }
+  if (size > 1) {
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while a peer reads its shared memory
+  }
 }
 
-// Joins the key splits of a row: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, splits in order.
+// Joins the groups of key splits of a row: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, in order.
 // One warp a row.
 template <int HD>
 __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
@@ -379,11 +446,11 @@ __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
   const long i = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (i >= rows) return;
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.ws_ml[s * rows + i].x);
+  for (int s = 0; s < a.groups; ++s) m = fmaxf(m, a.ws_ml[s * rows + i].x);
   float l = 0.f, acc[HD / 32];
 #pragma unroll
   for (int k = 0; k < HD / 32; ++k) acc[k] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = 0; s < a.groups; ++s) {
     const float2 ml = a.ws_ml[s * rows + i];
     if (ml.x == -INFINITY && ml.y == 0.f) continue;
     const float f = ex2_approx(ml.x - m);

@@ -1,0 +1,536 @@
+// kv8_attention_tc.cuh — attention over the 8-bit K/V cache for many query rows, on the 5th-generation tensor cores
+// (head_dim 128 and 256; the mathematics and the arguments are kv8_attention.cuh's).
+//
+// A CTA owns 128 folded query rows (r = t * G + g) of one (sample, K/V head) and one key split, and walks its keys in
+// tiles of 64:
+//   S = Q K^T     kind::f8f6f4, the K codes straight from the cache by TMA.  Q keeps 8 bits as two e4m3 operands, Q ~ 2^e (hi + lo)
+//                 with lo = e4m3(q - hi): off by at most 2^-10 where the row's largest element is 256 or more, and the two
+//                 products at twice the fp16 rate cost what one fp16 product would, without widening K.  Q lives in tensor
+//                 memory (HD / 2 columns), so a product reads only K from shared memory.
+//   softmax       thread = row = TMEM lane, two warpgroups with half of a tile's columns each; logits are scaled by the row's
+//                 and the key's powers of two here.  Both take the row maximum over all 64 columns, so they agree on it
+//                 without an exchange.
+//   O += P V      kind::f16, P in fp16 with the V row's scale folded in (11 bits, as in kv8_attention.cuh), V widened to
+//                 fp16 by four converter warps (exact; keys that no row sees become zeros, whatever the cache holds there).
+//                 An e4m3 P would need three operands to keep the small weights of a long cache.
+// The running maximum moves only when a tile exceeds it by 2^8 and the V exponent eb only when a scale exceeds it by 2^7;
+// both rescale O through tcgen05.ld/st.  eb is the same for all rows and kept by the warp that loads the scales.
+//   warp 0 TMA, warp 1 MMA issue, warp 2 TMEM, warp 3 scales, warps 4-11 softmax, warps 12-15 V
+#pragma once
+#include "fp8_gemm.cuh"
+#include "kv8_attention.cuh"
+
+namespace p5 {
+
+template <int HD>
+struct Kv8TcCfg {
+  static constexpr int ROWS = 128, KT = 64;
+  static constexpr int ATOMS = HD / 128;           // 128-byte blocks of a key row
+  static constexpr int TILE8 = KT * HD;            // codes of a K or V tile
+  static constexpr int TILE16 = KT * HD * 2;       // a widened V tile
+  static constexpr int P_BYTES = ROWS * KT * 2;    // 16 KB
+  static constexpr int NK = HD == 256 ? 3 : 4;     // K and V code rings
+  static constexpr int NSC = 4;                    // scale slots
+  static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8, P_OFF = W_OFF + 2 * TILE16;
+  static constexpr int SC_OFF = P_OFF + 2 * P_BYTES;
+  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64], vf[64], rescale factor of O
+  static constexpr int BAR_OFF = SC_OFF + NSC * SC_SLOT;
+  static constexpr int SMEM = 1024 + BAR_OFF + 512;
+  static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O
+  static constexpr int OUT_PITCH = HD * 2 + 16;
+  static constexpr int THREADS = 512;
+  static_assert(O_COL + HD <= 512 && ROWS * OUT_PITCH <= P_OFF && SMEM <= 232448, "");
+};
+
+// D (+)= A[tmem] B[smem]^T, kind::f8f6f4 (e4m3 x e4m3), issued by the elected lane of a whole warp
+__device__ __forceinline__ void tc_mma_f8_ta(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(512, 1)
+    kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Kv8Args a) {
+  using C = Kv8TcCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [NK] codes landed
+  uint64_t* k_empty = k_full + C::NK;                                // [NK] S product done
+  uint64_t* v_full = k_empty + C::NK;                                // [NK]
+  uint64_t* v_empty = v_full + C::NK;                                // [NK] widened (4 warps)
+  uint64_t* w_full = v_empty + C::NK;                                // [2] widened V in place (4 warps)
+  uint64_t* w_empty = w_full + 2;                                    // [2] P V product done
+  uint64_t* sc_full = w_empty + 2;                                   // [NSC] scales in place
+  uint64_t* sc_empty = sc_full + C::NSC;                             // [NSC] read by the 8 softmax warps
+  uint64_t* s_full = sc_empty + C::NSC;                              // [2]
+  uint64_t* s_empty = s_full + 2;                                    // [2] (8 warps)
+  uint64_t* p_full = s_empty + 2;                                    // [2] (8 warps)
+  uint64_t* p_empty = p_full + 2;                                    // [2] P V product done
+  uint64_t* q_full = p_empty + 2;                                    // Q in tensor memory (8 warps)
+  uint64_t* o_full = q_full + 1;                                     // every MMA complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort, [1] eb at the end
+  float* exch = reinterpret_cast<float*>(smem + C::P_OFF);  // [2][128] between the warpgroups (before the first, after the last P)
+  int* status = &g_fp8_status;
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+  const int rows = a.T * a.G;
+  // the last rows first: under a causal mask they have the most keys
+  const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * C::ROWS;
+  const int split = blockIdx.z;
+  const int slot = a.slots ? a.slots[b] : b;
+  const int len = (slot < 0 || slot >= a.n_slots) ? 0 : max(0, min(a.lens[b], a.capacity));
+  const int t_last = (min(row0 + C::ROWS, rows) - 1) / a.G;
+  const int top = a.causal ? max(0, min(len, len - a.T + t_last + 1)) : len;  // keys that any of the rows sees
+  const int tiles = (top + C::KT - 1) / C::KT;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int j0 = min(split * per, tiles), n = min(j0 + per, tiles) - j0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 4);
+    }
+    for (int i = 0; i < C::NSC; ++i) {
+      mbar_init(&sc_full[i], 1);
+      mbar_init(&sc_empty[i], 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&w_full[i], 4);
+      mbar_init(&w_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 8);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&p_empty[i], 1);
+    }
+    mbar_init(q_full, 8);
+    mbar_init(o_full, 1);
+    flags[0] = 0;
+    flags[1] = -1000;
+    fence_barrier_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < n && !flags[0]; ++i) {
+        const int s = i % C::NK;
+        const uint32_t ph = (uint32_t)(i / C::NK) & 1u;
+        const int key0 = (j0 + i) * C::KT;
+        if (!mbar_wait(&k_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+          flags[0] = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&k_full[s], C::TILE8);
+        for (int c = 0; c < C::ATOMS; ++c)
+          tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * 128, &tk, &k_full[s], c * 128, kvh, key0, slot);
+        if (!mbar_wait(&v_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+          flags[0] = 1;
+          mbar_wait(&k_full[s], ph, status, P5_ERR_WAIT_ATTN);
+          break;
+        }
+        mbar_arrive_expect_tx(&v_full[s], C::TILE8);
+        for (int c = 0; c < C::ATOMS; ++c)
+          tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * 128, &tv, &v_full[s], c * 128, kvh, key0, slot);
+        issued = i + 1;
+      }
+      fp8_drain(k_full, C::NK, issued, flags, status);
+      fp8_drain(v_full, C::NK, issued, flags, status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::KT >> 3) << 17) | (8u << 24);
+    constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // fp16, B MN-major
+    const uint32_t base = smem_u32(smem);
+    bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
+    for (int i = 0; i <= n && ok; ++i) {
+      if (i < n) {
+        const int s = i % C::NK, sb = i & 1;
+        ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+             mbar_wait_warp(&s_empty[sb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ka = base + C::K_OFF + s * C::TILE8;
+        const uint32_t d = tmem + (uint32_t)(C::S_COL + sb * C::KT);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int kk = 0; kk < HD / 32; ++kk)
+            tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
+                         sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
+        tc_commit_warp(&k_empty[s]);
+        tc_commit_warp(&s_full[sb]);
+      }
+      if (i >= 1) {
+        const int j = i - 1, pb = j & 1;
+        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+        ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t pa = base + C::P_OFF + pb * C::P_BYTES, va = base + C::W_OFF + pb * C::TILE16;
+#pragma unroll
+        for (int kk = 0; kk < C::KT / 16; ++kk)
+          tc_mma_f16_warp(tmem + C::O_COL, sw128_kmajor_desc(pa + kk * 32), sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o,
+                          (j | kk) ? 1u : 0u);
+        tc_commit_warp(&w_empty[pb]);
+        tc_commit_warp(&p_empty[pb]);
+      }
+    }
+    if (!ok) flags[0] = 1;
+    tc_commit_warp(o_full);
+  } else if (warp == 3) {
+    // ---- scales: two keys a lane, loaded a tile ahead
+    const long c0 = (long)slot * a.capacity * a.kv_heads + kvh;
+    int kb[2], vb[2];
+    auto load = [&](int i) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int key = (j0 + i) * C::KT + 2 * lane + q;
+        const bool in = i < n && key < top;
+        kb[q] = in ? (int)a.ks[c0 + (long)key * a.kv_heads] : 127;
+        vb[q] = in ? (int)a.vs[c0 + (long)key * a.kv_heads] : -1;  // no key
+      }
+    };
+    int eb = -1000;
+    load(0);
+    for (int i = 0; i < n; ++i) {
+      const int s = i % C::NSC;
+      float kf[2], vf[2];
+      int ev[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
+        ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
+      }
+      load(i + 1);
+      const int em = __reduce_max_sync(0xffffffffu, max(ev[0], ev[1]));
+      float rescale = 1.f;
+      if (em > eb + 7) {
+        if (i > 0) rescale = exp2_int(eb - em);  // 0 where there was no exponent yet: O is 0
+        eb = em;
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) vf[q] = exp2_int(ev[q] - eb);
+      bool ok = !flags[0] && mbar_wait(&sc_empty[s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+      if (!__all_sync(0xffffffffu, ok)) {
+        flags[0] = 1;
+        break;
+      }
+      float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
+      *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
+      *reinterpret_cast<float2*>(sc + C::KT + 2 * lane) = make_float2(vf[0], vf[1]);
+      if (lane == 0) {
+        sc[2 * C::KT] = rescale;
+        flags[1] = eb;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc_full[s]);
+    }
+  } else if (warp >= 12) {
+    // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
+    // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
+    const int cw = warp - 12;
+    for (int i = 0; i < n; ++i) {
+      const int s = i % C::NK, wb = i & 1;
+      const bool ok = !flags[0] && mbar_wait(&v_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                      mbar_wait(&w_empty[wb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+      if (!__all_sync(0xffffffffu, ok)) {
+        flags[0] = 1;
+        break;
+      }
+      const int valid = top - (j0 + i) * C::KT;  // rows from here on become zeros
+      const uint8_t* src = smem + C::V_OFF + s * C::TILE8;
+      uint8_t* dst = smem + C::W_OFF + wb * C::TILE16;
+#pragma unroll
+      for (int k = 0; k < C::KT * HD / 16 / 128; ++k) {
+        const int id = k * 128 + cw * 32 + lane;  // [row pair][4 pieces of a group][2 rows] ...
+        const int j4 = id & 3, hi = (id >> 2) & 1, rest = id >> 3;
+        const int group = rest % (HD / 64), pair = rest / (HD / 64);  // 64-dim box, pair of rows of an 8-row group
+        const int row = (pair >> 2) * 8 + ((pair & 3) ^ (hi ? 5 : 0));
+        const int piece = group * 4 + j4;  // 16-byte piece of the key's codes
+        uint4 u = *reinterpret_cast<const uint4*>(src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+        if (row >= valid) u = make_uint4(0, 0, 0, 0);
+        uint8_t* d = dst + group * (C::KT * 128) + row * 128;
+        *reinterpret_cast<uint4*>(d + (((2 * j4) ^ (row & 7)) << 4)) =
+            make_uint4(fp8_to_h2((uint16_t)u.x), fp8_to_h2((uint16_t)(u.x >> 16)), fp8_to_h2((uint16_t)u.y), fp8_to_h2((uint16_t)(u.y >> 16)));
+        *reinterpret_cast<uint4*>(d + (((2 * j4 + 1) ^ (row & 7)) << 4)) =
+            make_uint4(fp8_to_h2((uint16_t)u.z), fp8_to_h2((uint16_t)(u.z >> 16)), fp8_to_h2((uint16_t)u.w), fp8_to_h2((uint16_t)(u.w >> 16)));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&v_empty[s]);
+        mbar_arrive(&w_full[wb]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- softmax: thread = row = TMEM lane; warpgroup g exponentiates columns [32 g, 32 g + 32) of a tile and owns
+    // half of the head dims of Q and O
+    const int g = (warp - 4) >> 2, sub = warp & 3;
+    const int r = sub * 32 + lane, row = row0 + r;
+    const bool in = row < rows;
+    const int t = in ? row / a.G : 0, h = kvh * a.G + (in ? row % a.G : 0);
+    const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
+    float rf;
+    {
+      const bf16* src = a.q + (long)b * a.q_b + (long)t * a.q_t + (long)h * HD + g * (HD / 2);
+      uint32_t mb = 0;  // the largest magnitude as a bf16 pattern
+#pragma unroll 4
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint4 u = in ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+        const uint32_t v = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+        mb = max(mb, max(v >> 16, v & 0xffffu));
+      }
+      exch[g * 128 + r] = __uint_as_float(mb << 16);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      mb = max(__float_as_uint(exch[r]), __float_as_uint(exch[128 + r]));
+      const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN
+      const int byte = bad ? 127 : fp8_scale_byte(__uint_as_float(mb));
+      const float up = bad ? 0.f : fp8_scale_inverse(byte);
+      rf = bad ? NAN : fp8_scale_value(byte) * a.scale_log2;
+      constexpr int NC = HD / 8;  // columns of this half: four codes each
+#pragma unroll 1
+      for (int i = 0; i < NC; i += 16) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          const uint4 u = in && !bad ? reinterpret_cast<const uint4*>(src)[(i + k) / 2] : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f0 = unpack_bf2(w[2 * e]), f1 = unpack_bf2(w[2 * e + 1]);
+            const float x0 = f0.x * up, x1 = f0.y * up, x2 = f1.x * up, x3 = f1.y * up;
+            hi[k + e] = fp8_pack4(x0, x1, x2, x3);
+            const float2 h0 = fp8_to_f2((uint16_t)hi[k + e]), h1 = fp8_to_f2((uint16_t)(hi[k + e] >> 16));
+            lo[k + e] = fp8_pack4(x0 - h0.x, x1 - h0.y, x2 - h1.x, x3 - h1.y);
+          }
+        }
+        __syncwarp();
+        tmem_st16(t_lane + (uint32_t)(C::Q_COL + g * NC + i), hi);
+        tmem_st16(t_lane + (uint32_t)(C::Q_COL + HD / 4 + g * NC + i), lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // exch lies where P goes
+    }
+    const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
+    const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
+    uint8_t* prow = smem + C::P_OFF + r * 128;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool alive = true;
+    for (int j = 0; j < n; ++j) {
+      const int sb = j & 1, ss = j % C::NSC;
+      const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+      bool ok = !flags[0] && mbar_wait(&sc_full[ss], (uint32_t)(j / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                mbar_wait(&s_full[sb], ph, status, P5_ERR_WAIT_ATTN);
+      if (!__all_sync(0xffffffffu, ok)) {
+        flags[0] = 1;
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      const float* sc = reinterpret_cast<const float*>(smem + C::SC_OFF + ss * C::SC_SLOT);
+      // own columns in own[], the other warpgroup's only for the maximum
+      uint32_t own[32], oth[32];
+      tmem_ld32(t_lane + (uint32_t)(C::S_COL + sb * C::KT + 32 * g), own);
+      tmem_ld32(t_lane + (uint32_t)(C::S_COL + sb * C::KT + 32 * (g ^ 1)), oth);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[sb]);
+      const int valid = lim - (j0 + j) * C::KT;  // columns of the tile that this row sees (may be <= 0)
+      float mt = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 k0 = *reinterpret_cast<const float4*>(sc + 32 * g + c), k1 = *reinterpret_cast<const float4*>(sc + 32 * (g ^ 1) + c);
+        const float kf0[4] = {k0.x, k0.y, k0.z, k0.w}, kf1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          own[c + e] = __float_as_uint(__uint_as_float(own[c + e]) * kf0[e]);
+          oth[c + e] = __float_as_uint(__uint_as_float(oth[c + e]) * kf1[e]);
+        }
+      }
+      if (valid < C::KT) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (32 * g + c >= valid) own[c] = __float_as_uint(-INFINITY);
+          if (32 * (g ^ 1) + c >= valid) oth[c] = __float_as_uint(-INFINITY);
+        }
+      }
+      {
+        float mx[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(own[k]), __uint_as_float(oth[k]));
+#pragma unroll
+        for (int c = 4; c < 32; c += 4)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], __uint_as_float(own[c + k]), __uint_as_float(oth[c + k]));
+        mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      }
+      // in base 2: rf carries the row's power of two, the softmax scale (of either sign) and log2 e
+      if (rf < 0.f) {
+        float mn = INFINITY;  // the largest logit is the smallest product
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (32 * g + c < valid) mn = fminf(mn, __uint_as_float(own[c]));
+          if (32 * (g ^ 1) + c < valid) mn = fminf(mn, __uint_as_float(oth[c]));
+        }
+        mt = mn == INFINITY ? -INFINITY : mn * rf;
+      } else {
+        mt = mt == -INFINITY ? mt : mt * rf;
+      }
+      const float rescale = sc[2 * C::KT];
+      bool need = rescale != 1.f;
+      float alpha = rescale;
+      if (j == 0) {
+        m_run = mt;
+      } else if (mt > m_run + 8.f) {
+        need = true;
+        const float al = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mt);
+        m_run = mt;
+        l_run *= al;
+        alpha *= al;
+      }
+      const float msc = m_run == -INFINITY ? 0.f : m_run;
+      uint32_t pk[16];
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 v4 = *reinterpret_cast<const float4*>(sc + C::KT + 32 * g + c);
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __uint_as_float(own[c + e]);
+          p[e] = 32 * g + c + e < valid ? ex2_approx(fmaf(x, rf, -msc)) : 0.f;
+          ls[e] += p[e];
+        }
+        const __half2 h0 = __floats2half2_rn(p[0] * v4.x, p[1] * v4.y), h1 = __floats2half2_rn(p[2] * v4.z, p[3] * v4.w);
+        pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+        pk[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+      }
+      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc_empty[ss]);
+      // P buffer sb was last read by the P V product of tile j - 2
+      ok = mbar_wait(&p_empty[sb], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
+      uint8_t* pdst = prow + sb * C::P_BYTES;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(pdst + (((4 * g + c) ^ (r & 7)) << 4)) =
+            make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+      fence_proxy_async_smem();
+      if (j > 0 && __any_sync(0xffffffffu, need)) {
+        // wait for the P V product of tile j - 1, then rescale this warp's part of O
+        ok = ok && mbar_wait(&p_empty[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
+        if (__all_sync(0xffffffffu, ok)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD / 2; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + (uint32_t)c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(t_o + (uint32_t)c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      if (!__all_sync(0xffffffffu, ok)) {
+        flags[0] = 1;
+        alive = false;
+        break;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[sb]);
+    }
+
+    // ---- O / l, or the split's partial
+    const bool done = mbar_wait(o_full, 0, status, P5_ERR_WAIT_ATTN);
+    tc_fence_after();
+    const bool good = __all_sync(0xffffffffu, done && alive) && !flags[0];
+    exch[g * 128 + r] = l_run;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float l = exch[r] + exch[128 + r];
+    const float unit = exp2_int(n > 0 ? (int)flags[1] : 0);
+    // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
+    const float f = a.groups == 1 ? (l == 0.f ? 0.f : unit / l) : unit;
+    const long part = ((long)split * (gridDim.y / a.kv_heads) + b) * ((long)a.T * a.heads);
+#pragma unroll 1
+    for (int c = 0; c < HD / 2; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld32(t_o + (uint32_t)c, o);
+      tmem_wait_ld();
+      if (n == 0) {  // no MMA wrote this accumulator
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = 0u;
+      }
+      if (a.groups == 1) {
+        uint4* dst = reinterpret_cast<uint4*>(smem + r * C::OUT_PITCH + (g * (HD / 2) + c) * 2);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          dst[q] = make_uint4(pack_bf2(__uint_as_float(o[8 * q]) * f, __uint_as_float(o[8 * q + 1]) * f),
+                              pack_bf2(__uint_as_float(o[8 * q + 2]) * f, __uint_as_float(o[8 * q + 3]) * f),
+                              pack_bf2(__uint_as_float(o[8 * q + 4]) * f, __uint_as_float(o[8 * q + 5]) * f),
+                              pack_bf2(__uint_as_float(o[8 * q + 6]) * f, __uint_as_float(o[8 * q + 7]) * f));
+      } else if (in && good) {
+        float4* dst = reinterpret_cast<float4*>(a.ws_o + (part + (long)h * a.T + t) * HD + g * (HD / 2) + c);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          dst[q] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f, __uint_as_float(o[4 * q + 2]) * f,
+                               __uint_as_float(o[4 * q + 3]) * f);
+      }
+    }
+    if (a.groups > 1) {
+      if (in && good && g == 0) a.ws_ml[part + (long)h * a.T + t] = make_float2(m_run, l);
+    } else {
+      // staged above (K and V buffers are idle: every MMA is done), written by whole rows
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (good)
+        for (int k = warp - 4; k < C::ROWS && row0 + k < rows; k += 8) {
+          const int tt = (row0 + k) / a.G, hh = kvh * a.G + (row0 + k) % a.G;
+          if (lane < HD / 8)
+            reinterpret_cast<uint4*>(a.out + (long)b * a.o_b + (long)tt * a.o_t + (long)hh * HD)[lane] =
+                *reinterpret_cast<const uint4*>(smem + k * C::OUT_PITCH + lane * 16);
+        }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace p5
