@@ -34,12 +34,13 @@ struct Kv8TcCfg {
   static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8, P_OFF = W_OFF + 2 * TILE16;
   static constexpr int SC_OFF = P_OFF + 2 * P_BYTES;
   static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64], vf[64], rescale factor of O
-  static constexpr int BAR_OFF = SC_OFF + NSC * SC_SLOT;
+  static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [2][128] floats between the two softmax warpgroups
+  static constexpr int BAR_OFF = X_OFF + 2 * ROWS * 4;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
   static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O
   static constexpr int OUT_PITCH = HD * 2 + 16;
   static constexpr int THREADS = 512;
-  static_assert(O_COL + HD <= 512 && ROWS * OUT_PITCH <= P_OFF && SMEM <= 232448, "");
+  static_assert(O_COL + HD <= 512 && ROWS * OUT_PITCH <= P_OFF && W_OFF + ROWS * OUT_PITCH <= SC_OFF && SMEM <= 232448, "");
 };
 
 // D (+)= A[tmem] B[smem]^T, kind::f8f6f4 (e4m3 x e4m3), issued by the elected lane of a whole warp
@@ -60,6 +61,25 @@ __device__ __forceinline__ void tc_mma_f16_warp(uint32_t d, uint64_t a, uint64_t
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// two fp32 operations in one instruction (sm_100 packed arithmetic)
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
 }
 
 template <int HD>
@@ -85,7 +105,7 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* o_full = q_full + 1;                                     // every MMA complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort, [1] eb at the end
-  float* exch = reinterpret_cast<float*>(smem + C::P_OFF);  // [2][128] between the warpgroups (before the first, after the last P)
+  float* exch = reinterpret_cast<float*>(smem + C::X_OFF);
   int* status = &g_fp8_status;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -258,6 +278,7 @@ __global__ void __launch_bounds__(512, 1)
     // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
     // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
     const int cw = warp - 12;
+    if (!mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN)) flags[0] = 1;  // Q is staged where widened V goes
     for (int i = 0; i < n; ++i) {
       const int s = i % C::NK, wb = i & 1;
       const bool ok = !flags[0] && mbar_wait(&v_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
@@ -301,11 +322,24 @@ __global__ void __launch_bounds__(512, 1)
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
     float rf;
     {
-      const bf16* src = a.q + (long)b * a.q_b + (long)t * a.q_t + (long)h * HD + g * (HD / 2);
+      // the 128 query rows into shared memory (one round trip, whole rows a warp), then each thread its half row
+      uint8_t* sq = smem + C::W_OFF;
+      const long q_row = (long)b * a.q_b + (long)t * a.q_t + (long)h * HD;
+      constexpr int PER = HD / 8;  // 16-byte pieces of a row
+#pragma unroll 8
+      for (int k = 0; k < 16 * PER / 32; ++k) {
+        const int id = k * 32 + lane, rr = g * 16 + id / PER, p = id % PER;  // row of this warp's 32
+        const long src = __shfl_sync(0xffffffffu, q_row, rr);
+        cp_async16(sq + (sub * 32 + rr) * C::OUT_PITCH + p * 16, a.q + src + p * 8, row0 + sub * 32 + rr < rows);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const uint4* src = reinterpret_cast<const uint4*>(sq + r * C::OUT_PITCH + g * HD);
       uint32_t mb = 0;  // the largest magnitude as a bf16 pattern
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        const uint4 u = in ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+        const uint4 u = src[i];
         const uint32_t v = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
         mb = max(mb, max(v >> 16, v & 0xffffu));
       }
@@ -314,15 +348,18 @@ __global__ void __launch_bounds__(512, 1)
       mb = max(__float_as_uint(exch[r]), __float_as_uint(exch[128 + r]));
       const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN
       const int byte = bad ? 127 : fp8_scale_byte(__uint_as_float(mb));
-      const float up = bad ? 0.f : fp8_scale_inverse(byte);
-      rf = bad ? NAN : fp8_scale_value(byte) * a.scale_log2;
+      // rf > 0, so that a masked logit of -inf stays one: the sign of the softmax scale goes into Q, and a scale of 0 makes
+      // Q zero
+      const float sign = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
+      const float up = bad ? 0.f : sign * fp8_scale_inverse(byte);
+      rf = bad ? NAN : (sign == 0.f ? 1.f : fp8_scale_value(byte) * fabsf(a.scale_log2));
       constexpr int NC = HD / 8;  // columns of this half: four codes each
 #pragma unroll 1
       for (int i = 0; i < NC; i += 16) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
-          const uint4 u = in && !bad ? reinterpret_cast<const uint4*>(src)[(i + k) / 2] : make_uint4(0, 0, 0, 0);
+          const uint4 u = src[(i + k) / 2];
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -341,7 +378,6 @@ __global__ void __launch_bounds__(512, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // exch lies where P goes
     }
     const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
     const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
@@ -369,16 +405,16 @@ __global__ void __launch_bounds__(512, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_empty[sb]);
       const int valid = lim - (j0 + j) * C::KT;  // columns of the tile that this row sees (may be <= 0)
-      float mt = -INFINITY;
+      // each column by its key's power of two
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 k0 = *reinterpret_cast<const float4*>(sc + 32 * g + c), k1 = *reinterpret_cast<const float4*>(sc + 32 * (g ^ 1) + c);
-        const float kf0[4] = {k0.x, k0.y, k0.z, k0.w}, kf1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          own[c + e] = __float_as_uint(__uint_as_float(own[c + e]) * kf0[e]);
-          oth[c + e] = __float_as_uint(__uint_as_float(oth[c + e]) * kf1[e]);
-        }
+        const float2 a0 = mul2(make_float2(__uint_as_float(own[c]), __uint_as_float(own[c + 1])), make_float2(k0.x, k0.y));
+        const float2 a1 = mul2(make_float2(__uint_as_float(own[c + 2]), __uint_as_float(own[c + 3])), make_float2(k0.z, k0.w));
+        const float2 b0 = mul2(make_float2(__uint_as_float(oth[c]), __uint_as_float(oth[c + 1])), make_float2(k1.x, k1.y));
+        const float2 b1 = mul2(make_float2(__uint_as_float(oth[c + 2]), __uint_as_float(oth[c + 3])), make_float2(k1.z, k1.w));
+        own[c] = __float_as_uint(a0.x), own[c + 1] = __float_as_uint(a0.y), own[c + 2] = __float_as_uint(a1.x), own[c + 3] = __float_as_uint(a1.y);
+        oth[c] = __float_as_uint(b0.x), oth[c + 1] = __float_as_uint(b0.y), oth[c + 2] = __float_as_uint(b1.x), oth[c + 3] = __float_as_uint(b1.y);
       }
       if (valid < C::KT) {
 #pragma unroll
@@ -387,28 +423,15 @@ __global__ void __launch_bounds__(512, 1)
           if (32 * (g ^ 1) + c >= valid) oth[c] = __float_as_uint(-INFINITY);
         }
       }
-      {
-        float mx[4];
+      float mx[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(own[k]), __uint_as_float(oth[k]));
+      for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(own[k]), __uint_as_float(oth[k]));
 #pragma unroll
-        for (int c = 4; c < 32; c += 4)
+      for (int c = 4; c < 32; c += 4)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], __uint_as_float(own[c + k]), __uint_as_float(oth[c + k]));
-        mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      }
-      // in base 2: rf carries the row's power of two, the softmax scale (of either sign) and log2 e
-      if (rf < 0.f) {
-        float mn = INFINITY;  // the largest logit is the smallest product
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (32 * g + c < valid) mn = fminf(mn, __uint_as_float(own[c]));
-          if (32 * (g ^ 1) + c < valid) mn = fminf(mn, __uint_as_float(oth[c]));
-        }
-        mt = mn == INFINITY ? -INFINITY : mn * rf;
-      } else {
-        mt = mt == -INFINITY ? mt : mt * rf;
-      }
+        for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], __uint_as_float(own[c + k]), __uint_as_float(oth[c + k]));
+      // in base 2: rf carries the row's power of two, the softmax scale and log2 e
+      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rf;
       const float rescale = sc[2 * C::KT];
       bool need = rescale != 1.f;
       float alpha = rescale;
@@ -423,22 +446,22 @@ __global__ void __launch_bounds__(512, 1)
       }
       const float msc = m_run == -INFINITY ? 0.f : m_run;
       uint32_t pk[16];
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const float2 rf2 = make_float2(rf, rf), nm2 = make_float2(-msc, -msc);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 v4 = *reinterpret_cast<const float4*>(sc + C::KT + 32 * g + c);
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __uint_as_float(own[c + e]);
-          p[e] = 32 * g + c + e < valid ? ex2_approx(fmaf(x, rf, -msc)) : 0.f;
-          ls[e] += p[e];
-        }
-        const __half2 h0 = __floats2half2_rn(p[0] * v4.x, p[1] * v4.y), h1 = __floats2half2_rn(p[2] * v4.z, p[3] * v4.w);
+        const float2 x0 = fma2(make_float2(__uint_as_float(own[c]), __uint_as_float(own[c + 1])), rf2, nm2);
+        const float2 x1 = fma2(make_float2(__uint_as_float(own[c + 2]), __uint_as_float(own[c + 3])), rf2, nm2);
+        const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
+        ls[0] = add2(ls[0], p0);
+        ls[1] = add2(ls[1], p1);
+        const float2 w0 = mul2(p0, make_float2(v4.x, v4.y)), w1 = mul2(p1, make_float2(v4.z, v4.w));
+        const __half2 h0 = __floats2half2_rn(w0.x, w0.y), h1 = __floats2half2_rn(w1.x, w1.y);
         pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
         pk[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
       }
-      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      l_run += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc_empty[ss]);
       // P buffer sb was last read by the P V product of tile j - 2
@@ -516,15 +539,17 @@ __global__ void __launch_bounds__(512, 1)
     if (a.groups > 1) {
       if (in && good && g == 0) a.ws_ml[part + (long)h * a.T + t] = make_float2(m_run, l);
     } else {
-      // staged above (K and V buffers are idle: every MMA is done), written by whole rows
+      // staged above (K and V buffers are idle: every MMA is done), written by whole rows: each warp 16 of its lanes' rows
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (good)
-        for (int k = warp - 4; k < C::ROWS && row0 + k < rows; k += 8) {
-          const int tt = (row0 + k) / a.G, hh = kvh * a.G + (row0 + k) % a.G;
-          if (lane < HD / 8)
-            reinterpret_cast<uint4*>(a.out + (long)b * a.o_b + (long)tt * a.o_t + (long)hh * HD)[lane] =
-                *reinterpret_cast<const uint4*>(smem + k * C::OUT_PITCH + lane * 16);
-        }
+      const long o_row = (long)b * a.o_b + (long)t * a.o_t + (long)h * HD;
+      constexpr int PER = HD / 8;
+#pragma unroll 8
+      for (int k = 0; k < 16 * PER / 32; ++k) {
+        const int id = k * 32 + lane, rr = g * 16 + id / PER, p = id % PER;
+        const long dst = __shfl_sync(0xffffffffu, o_row, rr);
+        if (good && row0 + sub * 32 + rr < rows)
+          *reinterpret_cast<uint4*>(a.out + dst + p * 8) = *reinterpret_cast<const uint4*>(smem + (sub * 32 + rr) * C::OUT_PITCH + p * 16);
+      }
     }
   }
   tc_fence_before();
