@@ -7,9 +7,10 @@
 //                 with lo = e4m3(q - hi): off by at most 2^-10 where the row's largest element is 256 or more, and the two
 //                 products at twice the fp16 rate cost what one fp16 product would, without widening K.  Q lives in tensor
 //                 memory (HD / 2 columns), so a product reads only K from shared memory.
-//   softmax       thread = row = TMEM lane, two warpgroups with half of a tile's columns each; logits are scaled by the row's
-//                 and the key's powers of two here.  Both take the row maximum over all 64 columns, so they agree on it
-//                 without an exchange.
+//   softmax       thread = row = TMEM lane; two warpgroups take turns, one the even tiles and one the odd, so a tile's long
+//                 chain (load, scale, maximum, exponentials, store) runs beside the next one's.  They share the running maximum
+//                 of a row through shared memory: a tile's warp waits for its turn, raises the maximum if it must, and passes
+//                 the turn on before its exponentials.  Each keeps its own sum.
 //   O += P V      kind::f16, P in fp16 with the V row's scale folded in (11 bits, as in kv8_attention.cuh), V widened to
 //                 fp16 by four converter warps (exact; keys that no row sees become zeros, whatever the cache holds there).
 //                 An e4m3 P would need three operands to keep the small weights of a long cache.
@@ -34,8 +35,8 @@ struct Kv8TcCfg {
   static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8, P_OFF = W_OFF + 2 * TILE16;
   static constexpr int SC_OFF = P_OFF + 2 * P_BYTES;
   static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64], vf[64], rescale factor of O
-  static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [2][128] floats between the two softmax warpgroups
-  static constexpr int BAR_OFF = X_OFF + 2 * ROWS * 4;
+  static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
+  static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
   static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O
   static constexpr int OUT_PITCH = HD * 2 + 16;
@@ -63,6 +64,16 @@ __device__ __forceinline__ void tc_mma_f16_warp(uint32_t d, uint64_t a, uint64_t
       : "memory");
 }
 
+// The block's 512 x 128 registers, split: 64 a thread for warps 0-3, 184 for the softmax, 80 for the V warps (512 x 128 =
+// 128 x 64 + 256 x 184 + 128 x 80).  Each warpgroup sets its own share once, the shrinking ones first in time or not.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 // two fp32 operations in one instruction (sm_100 packed arithmetic)
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   uint64_t d;
@@ -96,12 +107,13 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* w_full = v_empty + C::NK;                                // [2] widened V in place (4 warps)
   uint64_t* w_empty = w_full + 2;                                    // [2] P V product done
   uint64_t* sc_full = w_empty + 2;                                   // [NSC] scales in place
-  uint64_t* sc_empty = sc_full + C::NSC;                             // [NSC] read by the 8 softmax warps
-  uint64_t* s_full = sc_empty + C::NSC;                              // [2]
-  uint64_t* s_empty = s_full + 2;                                    // [2] (8 warps)
-  uint64_t* p_full = s_empty + 2;                                    // [2] (8 warps)
+  uint64_t* sc_empty = sc_full + C::NSC;                             // [NSC] read by the tile's 4 softmax warps
+  uint64_t* s_full = sc_empty + C::NSC;                              // [2] of the even and the odd tiles
+  uint64_t* s_empty = s_full + 2;                                    // [2] (4 warps)
+  uint64_t* p_full = s_empty + 2;                                    // [2] (4 warps)
   uint64_t* p_empty = p_full + 2;                                    // [2] P V product done
-  uint64_t* q_full = p_empty + 2;                                    // Q in tensor memory (8 warps)
+  uint64_t* turn = p_empty + 2;                                      // [2][4] the other warpgroup's warp has passed the turn
+  uint64_t* q_full = turn + 8;                                       // Q in tensor memory (8 warps)
   uint64_t* o_full = q_full + 1;                                     // every MMA complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort, [1] eb at the end
@@ -131,16 +143,17 @@ __global__ void __launch_bounds__(512, 1)
     }
     for (int i = 0; i < C::NSC; ++i) {
       mbar_init(&sc_full[i], 1);
-      mbar_init(&sc_empty[i], 8);
+      mbar_init(&sc_empty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&w_full[i], 4);
       mbar_init(&w_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 8);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], 4);
       mbar_init(&p_empty[i], 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     mbar_init(q_full, 8);
     mbar_init(o_full, 1);
     flags[0] = 0;
@@ -158,6 +171,8 @@ __global__ void __launch_bounds__(512, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
+  if (warp < 4) {
+  regs_dec<64>();
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
@@ -191,7 +206,8 @@ __global__ void __launch_bounds__(512, 1)
     constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // fp16, B MN-major
     const uint32_t base = smem_u32(smem);
     bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
-    for (int i = 0; i <= n && ok; ++i) {
+    // S runs two tiles ahead of P V: its buffer is free as soon as the softmax has read it, long before P is there
+    for (int i = 0; i < n + 2 && ok; ++i) {
       if (i < n) {
         const int s = i % C::NK, sb = i & 1;
         ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
@@ -209,8 +225,8 @@ __global__ void __launch_bounds__(512, 1)
         tc_commit_warp(&k_empty[s]);
         tc_commit_warp(&s_full[sb]);
       }
-      if (i >= 1) {
-        const int j = i - 1, pb = j & 1;
+      if (i >= 2) {
+        const int j = i - 2, pb = j & 1;
         const uint32_t ph = (uint32_t)(j >> 1) & 1u;
         ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
         if (!ok) break;
@@ -274,7 +290,9 @@ __global__ void __launch_bounds__(512, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc_full[s]);
     }
+  }
   } else if (warp >= 12) {
+    regs_dec<80>();
     // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
     // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
     const int cw = warp - 12;
@@ -312,9 +330,10 @@ __global__ void __launch_bounds__(512, 1)
         mbar_arrive(&w_full[wb]);
       }
     }
-  } else if (warp >= 4) {
-    // ---- softmax: thread = row = TMEM lane; warpgroup g exponentiates columns [32 g, 32 g + 32) of a tile and owns
-    // half of the head dims of Q and O
+  } else {
+    regs_inc<184>();
+    // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
+    // Q and O at the start and the end
     const int g = (warp - 4) >> 2, sub = warp & 3;
     const int r = sub * 32 + lane, row = row0 + r;
     const bool in = row < rows;
@@ -380,15 +399,15 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(q_full);
     }
     const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
-    const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
-    uint8_t* prow = smem + C::P_OFF + r * 128;
+    uint8_t* prow = smem + C::P_OFF + g * C::P_BYTES + r * 128;
+    float* m_ref = exch + 4 * C::ROWS + r;  // the row's running maximum
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true;
-    for (int j = 0; j < n; ++j) {
-      const int sb = j & 1, ss = j % C::NSC;
+    for (int j = g; j < n; j += 2) {
+      const int ss = j % C::NSC;
       const uint32_t ph = (uint32_t)(j >> 1) & 1u;
       bool ok = !flags[0] && mbar_wait(&sc_full[ss], (uint32_t)(j / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
-                mbar_wait(&s_full[sb], ph, status, P5_ERR_WAIT_ATTN);
+                mbar_wait(&s_full[g], ph, status, P5_ERR_WAIT_ATTN);
       if (!__all_sync(0xffffffffu, ok)) {
         flags[0] = 1;
         alive = false;
@@ -396,63 +415,68 @@ __global__ void __launch_bounds__(512, 1)
       }
       tc_fence_after();
       const float* sc = reinterpret_cast<const float*>(smem + C::SC_OFF + ss * C::SC_SLOT);
-      // own columns in own[], the other warpgroup's only for the maximum
-      uint32_t own[32], oth[32];
-      tmem_ld32(t_lane + (uint32_t)(C::S_COL + sb * C::KT + 32 * g), own);
-      tmem_ld32(t_lane + (uint32_t)(C::S_COL + sb * C::KT + 32 * (g ^ 1)), oth);
-      tmem_wait_ld();
+      float x[C::KT];
+      {
+        uint32_t lo[32], hi[32];
+        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g * C::KT), lo);
+        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g * C::KT + 32), hi);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(lo[c]), x[32 + c] = __uint_as_float(hi[c]);
+      }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[sb]);
+      if (lane == 0) mbar_arrive(&s_empty[g]);
       const int valid = lim - (j0 + j) * C::KT;  // columns of the tile that this row sees (may be <= 0)
       // each column by its key's power of two
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 k0 = *reinterpret_cast<const float4*>(sc + 32 * g + c), k1 = *reinterpret_cast<const float4*>(sc + 32 * (g ^ 1) + c);
-        const float2 a0 = mul2(make_float2(__uint_as_float(own[c]), __uint_as_float(own[c + 1])), make_float2(k0.x, k0.y));
-        const float2 a1 = mul2(make_float2(__uint_as_float(own[c + 2]), __uint_as_float(own[c + 3])), make_float2(k0.z, k0.w));
-        const float2 b0 = mul2(make_float2(__uint_as_float(oth[c]), __uint_as_float(oth[c + 1])), make_float2(k1.x, k1.y));
-        const float2 b1 = mul2(make_float2(__uint_as_float(oth[c + 2]), __uint_as_float(oth[c + 3])), make_float2(k1.z, k1.w));
-        own[c] = __float_as_uint(a0.x), own[c + 1] = __float_as_uint(a0.y), own[c + 2] = __float_as_uint(a1.x), own[c + 3] = __float_as_uint(a1.y);
-        oth[c] = __float_as_uint(b0.x), oth[c + 1] = __float_as_uint(b0.y), oth[c + 2] = __float_as_uint(b1.x), oth[c + 3] = __float_as_uint(b1.y);
+      for (int c = 0; c < C::KT; c += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(sc + c);
+        const float2 a0 = mul2(make_float2(x[c], x[c + 1]), make_float2(k.x, k.y));
+        const float2 a1 = mul2(make_float2(x[c + 2], x[c + 3]), make_float2(k.z, k.w));
+        x[c] = a0.x, x[c + 1] = a0.y, x[c + 2] = a1.x, x[c + 3] = a1.y;
       }
       if (valid < C::KT) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (32 * g + c >= valid) own[c] = __float_as_uint(-INFINITY);
-          if (32 * (g ^ 1) + c >= valid) oth[c] = __float_as_uint(-INFINITY);
-        }
+        for (int c = 0; c < C::KT; ++c)
+          if (c >= valid) x[c] = -INFINITY;
       }
-      float mx[4];
+      float mx[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(own[k]), __uint_as_float(oth[k]));
+      for (int k = 0; k < 8; ++k) mx[k] = fmaxf(x[k], x[8 + k]);
 #pragma unroll
-      for (int c = 4; c < 32; c += 4)
+      for (int c = 16; c < C::KT; c += 16)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], __uint_as_float(own[c + k]), __uint_as_float(oth[c + k]));
+        for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], x[c + k], x[c + 8 + k]);
       // in base 2: rf carries the row's power of two, the softmax scale and log2 e
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rf;
+      const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
       const float rescale = sc[2 * C::KT];
       bool need = rescale != 1.f;
-      float alpha = rescale;
-      if (j == 0) {
-        m_run = mt;
-      } else if (mt > m_run + 8.f) {
-        need = true;
-        const float al = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mt);
-        m_run = mt;
-        l_run *= al;
-        alpha *= al;
+      float alpha = rescale, m = mt;
+      if (j > 0) {  // the turn: the maximum after tile j - 1
+        ok = mbar_wait(&turn[4 * g + sub], (uint32_t)((j >> 1) - 1 + g) & 1u, status, P5_ERR_WAIT_ATTN);
+        const float before = *m_ref;
+        m = before;
+        if (mt > before + 8.f) {
+          need = true;
+          m = mt;
+          alpha *= before == -INFINITY ? 0.f : ex2_approx(before - mt);
+        }
       }
-      const float msc = m_run == -INFINITY ? 0.f : m_run;
-      uint32_t pk[16];
+      *m_ref = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&turn[4 * (g ^ 1) + sub]);
+      l_run *= m_run == m ? 1.f : (m_run == -INFINITY ? 0.f : ex2_approx(m_run - m));
+      m_run = m;
+      const float msc = m == -INFINITY ? 0.f : m;
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       const float2 rf2 = make_float2(rf, rf), nm2 = make_float2(-msc, -msc);
+      uint32_t pk[C::KT / 2];
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 v4 = *reinterpret_cast<const float4*>(sc + C::KT + 32 * g + c);
-        const float2 x0 = fma2(make_float2(__uint_as_float(own[c]), __uint_as_float(own[c + 1])), rf2, nm2);
-        const float2 x1 = fma2(make_float2(__uint_as_float(own[c + 2]), __uint_as_float(own[c + 3])), rf2, nm2);
+      for (int c = 0; c < C::KT; c += 4) {
+        const float4 v4 = *reinterpret_cast<const float4*>(sc + C::KT + c);
+        const float2 x0 = fma2(make_float2(x[c], x[c + 1]), rf2, nm2);
+        const float2 x1 = fma2(make_float2(x[c + 2], x[c + 3]), rf2, nm2);
         const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
         ls[0] = add2(ls[0], p0);
         ls[1] = add2(ls[1], p1);
@@ -464,27 +488,25 @@ __global__ void __launch_bounds__(512, 1)
       l_run += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc_empty[ss]);
-      // P buffer sb was last read by the P V product of tile j - 2
-      ok = mbar_wait(&p_empty[sb], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
-      uint8_t* pdst = prow + sb * C::P_BYTES;
+      // P buffer g was last read by the P V product of tile j - 2
+      ok = ok && mbar_wait(&p_empty[g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4*>(pdst + (((4 * g + c) ^ (r & 7)) << 4)) =
-            make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
       fence_proxy_async_smem();
       if (j > 0 && __any_sync(0xffffffffu, need)) {
-        // wait for the P V product of tile j - 1, then rescale this warp's part of O
-        ok = ok && mbar_wait(&p_empty[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
+        // wait for the P V product of tile j - 1, then rescale this warp's rows of O
+        ok = ok && mbar_wait(&p_empty[g ^ 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD / 2; c += 32) {
+          for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
-            tmem_ld32(t_o + (uint32_t)c, o);
+            tmem_ld32(t_lane + (uint32_t)(C::O_COL + c), o);
             tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(t_o + (uint32_t)c, o);
+            tmem_st32(t_lane + (uint32_t)(C::O_COL + c), o);
           }
           tmem_wait_st();
         }
@@ -496,16 +518,21 @@ __global__ void __launch_bounds__(512, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[sb]);
+      if (lane == 0) mbar_arrive(&p_full[g]);
     }
+    const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
 
     // ---- O / l, or the split's partial
     const bool done = mbar_wait(o_full, 0, status, P5_ERR_WAIT_ATTN);
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, done && alive) && !flags[0];
+    // the later tile's maximum is the larger; O is in units of it
     exch[g * 128 + r] = l_run;
+    exch[(2 + g) * 128 + r] = m_run;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float l = exch[r] + exch[128 + r];
+    const float m0 = exch[256 + r], m1 = exch[384 + r];
+    m_run = fmaxf(m0, m1);
+    const float l = (m0 == m_run ? 1.f : ex2_approx(m0 - m_run)) * exch[r] + (m1 == m_run ? 1.f : ex2_approx(m1 - m_run)) * exch[128 + r];
     const float unit = exp2_int(n > 0 ? (int)flags[1] : 0);
     // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
     const float f = a.groups == 1 ? (l == 0.f ? 0.f : unit / l) : unit;
