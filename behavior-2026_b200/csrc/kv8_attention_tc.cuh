@@ -93,6 +93,10 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return *reinterpret_cast<float2*>(&d);
 }
 
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  return fma2(b, make_float2(-1.f, -1.f), a);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(512, 1)
     kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Kv8Args a) {
@@ -126,6 +130,27 @@ __global__ void __launch_bounds__(512, 1)
   // the last rows first: under a causal mask they have the most keys
   const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * C::ROWS;
   const int split = blockIdx.z;
+  // the 128 query rows into shared memory, before anything that waits for slots and lengths: each softmax warp loads
+  // 16 whole rows, of the 32 that its lanes (thread = row) will convert
+  const int g = (warp - 4) >> 2, sub = warp & 3;  // softmax warps: warpgroup, lane quarter
+  const int r = sub * 32 + lane, row = row0 + r;
+  const bool in = row < rows;
+  const int t = in ? row / a.G : 0, h = kvh * a.G + (in ? row - t * a.G : 0);
+  if (warp >= 4 && warp < 12) {
+    const uint32_t sq = smem_u32(smem + C::W_OFF) + (uint32_t)(sub * 32 + g * 16) * C::OUT_PITCH;
+    const bf16* src = a.q + (long)b * a.q_b + (long)t * a.q_t + (long)h * HD;
+    constexpr int PER = HD / 8;  // 16-byte pieces of a row
+#pragma unroll
+    for (int k = 0; k < 16 * PER / 32; ++k) {
+      const int id = k * 32 + lane, rr = id / PER, p = id % PER;
+      const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), g * 16 + rr);
+      const bool there = __shfl_sync(0xffffffffu, (int)in, g * 16 + rr);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sq + rr * C::OUT_PITCH + p * 16),
+                   "l"(from + (there ? (uint64_t)p * 16 : 0)), "r"(there ? 16 : 0)
+                   : "memory");
+    }
+    cp_async_commit();
+  }
   const int slot = a.slots ? a.slots[b] : b;
   const int len = (slot < 0 || slot >= a.n_slots) ? 0 : max(0, min(a.lens[b], a.capacity));
   const int t_last = (min(row0 + C::ROWS, rows) - 1) / a.G;
@@ -334,24 +359,10 @@ __global__ void __launch_bounds__(512, 1)
     regs_inc<184>();
     // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
     // Q and O at the start and the end
-    const int g = (warp - 4) >> 2, sub = warp & 3;
-    const int r = sub * 32 + lane, row = row0 + r;
-    const bool in = row < rows;
-    const int t = in ? row / a.G : 0, h = kvh * a.G + (in ? row % a.G : 0);
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
     float rf;
     {
-      // the 128 query rows into shared memory (one round trip, whole rows a warp), then each thread its half row
-      uint8_t* sq = smem + C::W_OFF;
-      const long q_row = (long)b * a.q_b + (long)t * a.q_t + (long)h * HD;
-      constexpr int PER = HD / 8;  // 16-byte pieces of a row
-#pragma unroll 8
-      for (int k = 0; k < 16 * PER / 32; ++k) {
-        const int id = k * 32 + lane, rr = g * 16 + id / PER, p = id % PER;  // row of this warp's 32
-        const long src = __shfl_sync(0xffffffffu, q_row, rr);
-        cp_async16(sq + (sub * 32 + rr) * C::OUT_PITCH + p * 16, a.q + src + p * 8, row0 + sub * 32 + rr < rows);
-      }
-      cp_async_commit();
+      const uint8_t* sq = smem + C::W_OFF;
       cp_async_wait<0>();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const uint4* src = reinterpret_cast<const uint4*>(sq + r * C::OUT_PITCH + g * HD);
@@ -371,6 +382,7 @@ __global__ void __launch_bounds__(512, 1)
       // Q zero
       const float sign = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
       const float up = bad ? 0.f : sign * fp8_scale_inverse(byte);
+      const float2 up2 = make_float2(up, up);
       rf = bad ? NAN : (sign == 0.f ? 1.f : fp8_scale_value(byte) * fabsf(a.scale_log2));
       constexpr int NC = HD / 8;  // columns of this half: four codes each
 #pragma unroll 1
@@ -382,11 +394,14 @@ __global__ void __launch_bounds__(512, 1)
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float2 f0 = unpack_bf2(w[2 * e]), f1 = unpack_bf2(w[2 * e + 1]);
-            const float x0 = f0.x * up, x1 = f0.y * up, x2 = f1.x * up, x3 = f1.y * up;
-            hi[k + e] = fp8_pack4(x0, x1, x2, x3);
-            const float2 h0 = fp8_to_f2((uint16_t)hi[k + e]), h1 = fp8_to_f2((uint16_t)(hi[k + e] >> 16));
-            lo[k + e] = fp8_pack4(x0 - h0.x, x1 - h0.y, x2 - h1.x, x3 - h1.y);
+            const float2 x0 = mul2(unpack_bf2(w[2 * e]), up2), x1 = mul2(unpack_bf2(w[2 * e + 1]), up2);
+            // x rounded to the 4 bits of a normal code: c - (c - x) with c = (2^20 + 1) x (Dekker's splitting); where the codes are
+            // subnormal the conversion rounds it once more, by at most the 2^-10 that lo is off by anyway
+            const float2 c0 = mul2(x0, make_float2(1048577.f, 1048577.f)), c1 = mul2(x1, make_float2(1048577.f, 1048577.f));
+            const float2 h0 = sub2(c0, sub2(c0, x0)), h1 = sub2(c1, sub2(c1, x1));
+            const float2 l0 = sub2(x0, h0), l1 = sub2(x1, h1);
+            hi[k + e] = fp8_pack4(h0.x, h0.y, h1.x, h1.y);
+            lo[k + e] = fp8_pack4(l0.x, l0.y, l1.x, l1.y);
           }
         }
         __syncwarp();
@@ -566,16 +581,12 @@ __global__ void __launch_bounds__(512, 1)
     if (a.groups > 1) {
       if (in && good && g == 0) a.ws_ml[part + (long)h * a.T + t] = make_float2(m_run, l);
     } else {
-      // staged above (K and V buffers are idle: every MMA is done), written by whole rows: each warp 16 of its lanes' rows
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const long o_row = (long)b * a.o_b + (long)t * a.o_t + (long)h * HD;
-      constexpr int PER = HD / 8;
-#pragma unroll 8
-      for (int k = 0; k < 16 * PER / 32; ++k) {
-        const int id = k * 32 + lane, rr = g * 16 + id / PER, p = id % PER;
-        const long dst = __shfl_sync(0xffffffffu, o_row, rr);
-        if (good && row0 + sub * 32 + rr < rows)
-          *reinterpret_cast<uint4*>(a.out + dst + p * 8) = *reinterpret_cast<const uint4*>(smem + (sub * 32 + rr) * C::OUT_PITCH + p * 16);
+      // staged above (K and V buffers are idle: every MMA is done); each thread sends its half row by one bulk copy
+      fence_proxy_async_smem();
+      if (good && in) {
+        bulk_store_global(a.out + (long)b * a.o_b + (long)t * a.o_t + (long)h * HD + g * (HD / 2),
+                          smem_u32(smem + r * C::OUT_PITCH + g * HD), HD);
+        bulk_store_wait_read();  // the staging must outlive the copy's reads
       }
     }
   }
