@@ -239,6 +239,15 @@ bool set_smem(const void* f, int bytes) {
   return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
 
+// its warpgroups' register shares must fit what the block is launched with, else a share would never be granted
+template <int HD>
+bool attention_attributes() {
+  cudaFuncAttributes f;
+  return set_smem((const void*)kv8_attn_tc_kernel<HD>, Kv8TcCfg<HD>::SMEM) &&
+         cudaFuncGetAttributes(&f, (const void*)kv8_attn_tc_kernel<HD>) == cudaSuccess &&
+         (f.numRegs + 7) / 8 * 8 * Kv8TcCfg<HD>::THREADS >= Kv8TcCfg<HD>::REGS;
+}
+
 template <int EPI>
 bool linear_attributes() {
   auto set = set_smem;
@@ -266,8 +275,7 @@ int setup(char* err, size_t err_len, int* sms) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2 || !linear_attributes<FP8_STORE>() ||
         !linear_attributes<FP8_GELU>() || !linear_attributes<FP8_RESID>() || !linear_attributes<FP8_GATED>() ||
         !linear_attributes<FP8_GEGLU>() || !linear_attributes<FP8_F32>() ||
-        !set_smem((const void*)kv8_attn_tc_kernel<128>, Kv8TcCfg<128>::SMEM) ||
-        !set_smem((const void*)kv8_attn_tc_kernel<256>, Kv8TcCfg<256>::SMEM) ||
+        !attention_attributes<128>() || !attention_attributes<256>() ||
         !set_smem((const void*)kv8_attn_rows_kernel<64>, Kv8RowsCfg<64>::SMEM) ||
         !set_smem((const void*)kv8_attn_rows_kernel<128>, Kv8RowsCfg<128>::SMEM) ||
         !set_smem((const void*)kv8_attn_rows_kernel<256>, Kv8RowsCfg<256>::SMEM))

@@ -38,10 +38,16 @@ struct Kv8TcCfg {
   static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
   static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
-  static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O
+  static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O,
+  // and at HD 128, where there is room, P[2]: it then costs the shared memory, which all of this competes for, nothing
+  static constexpr bool P_TMEM = HD == 128;
+  static constexpr int P_COL = O_COL + HD;
   static constexpr int OUT_PITCH = HD * 2 + 16;
   static constexpr int THREADS = 512;
-  static_assert(O_COL + HD <= 512 && ROWS * OUT_PITCH <= P_OFF && W_OFF + ROWS * OUT_PITCH <= SC_OFF && SMEM <= 232448, "");
+  // registers a thread: warps 0-3, softmax, V; their sum over the block is what 128 a thread at launch make (the host checks)
+  static constexpr int REG_ROLE = 64, REG_SOFT = 184, REG_V = 80;
+  static constexpr int REGS = 128 * REG_ROLE + 256 * REG_SOFT + 128 * REG_V;
+  static_assert(O_COL + HD + (P_TMEM ? KT : 0) <= 512 && REGS <= 65536 && ROWS * OUT_PITCH <= P_OFF && W_OFF + ROWS * OUT_PITCH <= SC_OFF && SMEM <= 232448, "");
 };
 
 // D (+)= A[tmem] B[smem]^T, kind::f8f6f4 (e4m3 x e4m3), issued by the elected lane of a whole warp
@@ -51,6 +57,15 @@ __device__ __forceinline__ void tc_mma_f8_ta(uint32_t d, uint32_t a_tmem, uint64
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_ta_warp(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -64,8 +79,7 @@ __device__ __forceinline__ void tc_mma_f16_warp(uint32_t d, uint64_t a, uint64_t
       : "memory");
 }
 
-// The block's 512 x 128 registers, split: 64 a thread for warps 0-3, 184 for the softmax, 80 for the V warps (512 x 128 =
-// 128 x 64 + 256 x 184 + 128 x 80).  Each warpgroup sets its own share once, the shrinking ones first in time or not.
+// Each warpgroup sets its share of the block's registers once.
 template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(512, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp < 4) {
-  regs_dec<64>();
+  regs_dec<C::REG_ROLE>();
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
@@ -259,8 +273,12 @@ __global__ void __launch_bounds__(512, 1)
         const uint32_t pa = base + C::P_OFF + pb * C::P_BYTES, va = base + C::W_OFF + pb * C::TILE16;
 #pragma unroll
         for (int kk = 0; kk < C::KT / 16; ++kk)
-          tc_mma_f16_warp(tmem + C::O_COL, sw128_kmajor_desc(pa + kk * 32), sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o,
-                          (j | kk) ? 1u : 0u);
+          if (C::P_TMEM)
+            tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
+                               sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
+          else
+            tc_mma_f16_warp(tmem + C::O_COL, sw128_kmajor_desc(pa + kk * 32), sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o,
+                            (j | kk) ? 1u : 0u);
         tc_commit_warp(&w_empty[pb]);
         tc_commit_warp(&p_empty[pb]);
       }
@@ -317,7 +335,7 @@ __global__ void __launch_bounds__(512, 1)
     }
   }
   } else if (warp >= 12) {
-    regs_dec<80>();
+    regs_dec<C::REG_V>();
     // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
     // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
     const int cw = warp - 12;
@@ -356,7 +374,7 @@ __global__ void __launch_bounds__(512, 1)
       }
     }
   } else {
-    regs_inc<184>();
+    regs_inc<C::REG_SOFT>();
     // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
     // Q and O at the start and the end
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
@@ -505,10 +523,17 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(&sc_empty[ss]);
       // P buffer g was last read by the P V product of tile j - 2
       ok = ok && mbar_wait(&p_empty[g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
+      if (C::P_TMEM) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_st32(t_lane + (uint32_t)(C::P_COL + g * (C::KT / 2)), pk);
+        tmem_wait_st();
+      } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-      fence_proxy_async_smem();
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+        fence_proxy_async_smem();
+      }
       if (j > 0 && __any_sync(0xffffffffu, need)) {
         // wait for the P V product of tile j - 1, then rescale this warp's rows of O
         ok = ok && mbar_wait(&p_empty[g ^ 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
