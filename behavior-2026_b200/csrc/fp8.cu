@@ -389,22 +389,32 @@ struct AttentionPlan {
   int splits, cluster;  // key splits, CTAs of a cluster (splits is a multiple)
 };
 
-// By sizes that the host knows (the lengths are on the device): key splits fill the machine once where the cache allows a
-// CTA at least 128 keys; of the rows kernel in clusters of up to 8, so that up to 8 splits need no second kernel.
+// By sizes that the host knows (the lengths are on the device): the kernel and its key splits by an estimate in microseconds of
+// waves x (fixed + steps), fitted to measurements.  E.g. 1018 keys, 8 heads on one of 256: one chunk of 50 tokens
+// 14.2 (rows, 2 splits), 18.2 (tc, 8 splits); 64 chunks 365 (rows), 47.5 (tc); 8 x 5 tokens 14.1 (rows), 16.7 (tc).
 AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
-  const long rows = (long)T * (heads / kv_heads), pairs = (long)batch * kv_heads;
-  const bool tc = head_dim >= 128 && rows > 32;
-  if (tc) {
-    const long tiles = pairs * ((rows + 127) / 128);
-    const long splits = std::max<long>(1, std::min<long>(((long)capacity + 127) / 128, num_sms() / tiles));
-    return {true, (int)splits, 1};
+  const double rows = (double)T * (heads / kv_heads), pairs = (double)batch * kv_heads;
+  AttentionPlan best = {false, 1, 1};
+  double best_cost = 1e300;
+  {  // a step: 32 keys of one of four warps
+    const double tiles = pairs * ceil(rows / 8), steps = ceil(capacity / 128.0);
+    const double places = (double)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
+    const double step = head_dim == 256 ? 1.8 : (head_dim == 128 ? 1.0 : 0.7);
+    for (int s = 1; s <= 256 && (s == 1 || s <= steps); s += s < 8 ? s : 8) {  // 1, 2, 4, 8, 16, 24, ...
+      const double cost = ceil(tiles * s / places) * (6 + ceil(steps / s) * step) + (s > 8 ? 3 : 0);
+      if (cost < best_cost) best_cost = cost, best = {false, s, s < 8 ? s : 8};
+      if (tiles * s > 2 * places) break;
+    }
   }
-  const long tiles = pairs * ((rows + 7) / 8);
-  const long places = (long)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
-  long splits = std::max<long>(1, std::min<long>({((long)capacity + 127) / 128, places / tiles, 256L}));
-  int cluster = 1;
-  while (cluster < 8 && 2 * cluster <= splits) cluster *= 2;
-  return {false, (int)(splits / cluster * cluster), cluster};
+  if (head_dim >= 128) {  // a step: 64 keys
+    const double tiles = pairs * ceil(rows / 128), steps = ceil(capacity / 64.0), step = head_dim == 256 ? 0.9 : 0.65;
+    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= steps); ++s) {
+      const double cost = ceil(tiles * s / num_sms()) * (10 + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
+      if (cost < best_cost) best_cost = cost, best = {true, s, 1};
+      if (tiles * s > 2 * num_sms()) break;
+    }
+  }
+  return best;
 }
 
 // [slots][capacity][kv_heads][head_dim] codes in boxes of 64 positions x 128 bytes of one head

@@ -29,25 +29,25 @@ struct Kv8TcCfg {
   static constexpr int ATOMS = HD / 128;           // 128-byte blocks of a key row
   static constexpr int TILE8 = KT * HD;            // codes of a K or V tile
   static constexpr int TILE16 = KT * HD * 2;       // a widened V tile
-  static constexpr int P_BYTES = ROWS * KT * 2;    // 16 KB
   static constexpr int NK = HD == 256 ? 3 : 4;     // K and V code rings
   static constexpr int NSC = 4;                    // scale slots
-  static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8, P_OFF = W_OFF + 2 * TILE16;
-  static constexpr int SC_OFF = P_OFF + 2 * P_BYTES;
+  static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8;
+  static constexpr int Q_BYTES = ROWS * (HD * 2 + 16);  // query rows on their way in, over the widened V
+  static constexpr int SC_OFF = W_OFF + (2 * TILE16 > Q_BYTES ? 2 * TILE16 : (Q_BYTES + 127) / 128 * 128);
   static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64], vf[64], rescale factor of O
   static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
   static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
-  static constexpr int Q_COL = 0, S_COL = HD / 2, O_COL = HD / 2 + 2 * KT;  // tensor memory: Q hi | lo, S[2], O,
-  // and at HD 128, where there is room, P[2]: it then costs the shared memory, which all of this competes for, nothing
-  static constexpr bool P_TMEM = HD == 128;
-  static constexpr int P_COL = O_COL + HD;
+  // Tensor memory: Q hi | lo, S, P[2], O.  P lies here because all of this competes for the shared memory; at HD 256 that
+  // leaves room for one S buffer only (two, and P in shared memory: 64 chunks 49.7 us).
+  static constexpr int NS = HD == 256 ? 1 : 2;
+  static constexpr int Q_COL = 0, S_COL = HD / 2, P_COL = S_COL + NS * KT, O_COL = P_COL + KT;
   static constexpr int OUT_PITCH = HD * 2 + 16;
   static constexpr int THREADS = 512;
   // registers a thread: warps 0-3, softmax, V; their sum over the block is what 128 a thread at launch make (the host checks)
   static constexpr int REG_ROLE = 64, REG_SOFT = 184, REG_V = 80;
   static constexpr int REGS = 128 * REG_ROLE + 256 * REG_SOFT + 128 * REG_V;
-  static_assert(O_COL + HD + (P_TMEM ? KT : 0) <= 512 && REGS <= 65536 && ROWS * OUT_PITCH <= P_OFF && W_OFF + ROWS * OUT_PITCH <= SC_OFF && SMEM <= 232448, "");
+  static_assert(O_COL + HD <= 512 && REGS <= 65536 && ROWS * OUT_PITCH <= SC_OFF && SMEM <= 232448, "");
 };
 
 // D (+)= A[tmem] B[smem]^T, kind::f8f6f4 (e4m3 x e4m3), issued by the elected lane of a whole warp
@@ -69,16 +69,6 @@ __device__ __forceinline__ void tc_mma_f16_ta_warp(uint32_t d, uint32_t a_tmem, 
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 // Each warpgroup sets its share of the block's registers once.
 template <int N>
 __device__ __forceinline__ void regs_dec() {
@@ -250,11 +240,11 @@ __global__ void __launch_bounds__(512, 1)
       if (i < n) {
         const int s = i % C::NK, sb = i & 1;
         ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
-             mbar_wait_warp(&s_empty[sb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+             (i < C::NS || mbar_wait_warp(&s_empty[(i - C::NS) & 1], (uint32_t)((i - C::NS) >> 1) & 1u, status, P5_ERR_WAIT_ATTN));
         if (!ok) break;
         tc_fence_after();
         const uint32_t ka = base + C::K_OFF + s * C::TILE8;
-        const uint32_t d = tmem + (uint32_t)(C::S_COL + sb * C::KT);
+        const uint32_t d = tmem + (uint32_t)(C::S_COL + sb % C::NS * C::KT);
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -270,15 +260,11 @@ __global__ void __launch_bounds__(512, 1)
         ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t pa = base + C::P_OFF + pb * C::P_BYTES, va = base + C::W_OFF + pb * C::TILE16;
+        const uint32_t va = base + C::W_OFF + pb * C::TILE16;
 #pragma unroll
         for (int kk = 0; kk < C::KT / 16; ++kk)
-          if (C::P_TMEM)
-            tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
-                               sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
-          else
-            tc_mma_f16_warp(tmem + C::O_COL, sw128_kmajor_desc(pa + kk * 32), sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o,
-                            (j | kk) ? 1u : 0u);
+          tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
+                             sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
         tc_commit_warp(&w_empty[pb]);
         tc_commit_warp(&p_empty[pb]);
       }
@@ -432,7 +418,6 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(q_full);
     }
     const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
-    uint8_t* prow = smem + C::P_OFF + g * C::P_BYTES + r * 128;
     float* m_ref = exch + 4 * C::ROWS + r;  // the row's running maximum
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true;
@@ -451,8 +436,8 @@ __global__ void __launch_bounds__(512, 1)
       float x[C::KT];
       {
         uint32_t lo[32], hi[32];
-        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g * C::KT), lo);
-        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g * C::KT + 32), hi);
+        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT), lo);
+        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT + 32), hi);
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(lo[c]), x[32 + c] = __uint_as_float(hi[c]);
@@ -523,17 +508,10 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(&sc_empty[ss]);
       // P buffer g was last read by the P V product of tile j - 2
       ok = ok && mbar_wait(&p_empty[g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
-      if (C::P_TMEM) {
-        __syncwarp();
-        tc_fence_after();
-        tmem_st32(t_lane + (uint32_t)(C::P_COL + g * (C::KT / 2)), pk);
-        tmem_wait_st();
-      } else {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-        fence_proxy_async_smem();
-      }
+      __syncwarp();
+      tc_fence_after();
+      tmem_st32(t_lane + (uint32_t)(C::P_COL + g * (C::KT / 2)), pk);
+      tmem_wait_st();
       if (j > 0 && __any_sync(0xffffffffu, need)) {
         // wait for the P V product of tile j - 1, then rescale this warp's rows of O
         ok = ok && mbar_wait(&p_empty[g ^ 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);

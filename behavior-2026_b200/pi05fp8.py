@@ -60,12 +60,8 @@ def fp8_quantize(x, out=None):
     if out is None:
         # rows of whole 128-byte lines and scale rows of 16 bytes, which fp8_linear loads best
         ldq, lds = blocks * 128 if cols > 64 else 64, (blocks + 15) // 16 * 16
-        q = torch.empty((rows, ldq), dtype=E4M3, device=dev)
-        s = torch.empty((rows, lds), dtype=U8, device=dev)
-        if ldq != cols:
-            q = q[:, :cols]
-        if lds != blocks:
-            s = s[:, :blocks]
+        q = torch.empty_strided((rows, cols), (ldq, 1), dtype=E4M3, device=dev)
+        s = torch.empty_strided((rows, blocks), (lds, 1), dtype=U8, device=dev)
     else:
         q, s = out
         if q.dtype != E4M3 or s.dtype != U8 or q.shape != x.shape or s.shape != (rows, blocks) or q.device != dev or s.device != dev:

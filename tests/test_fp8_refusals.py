@@ -77,11 +77,18 @@ def test_cache_rows_refuse(pn, name, kw):
                                 dict(vs=None), dict(lens=None), dict(out=None), dict(q=A + 8), dict(k8=A + 8), dict(v8=A + 8),
                                 dict(out=A + 8), dict(qb=1020), dict(qt=1020), dict(qt=1016), dict(ot=1016), dict(ob=1020),
                                 dict(ob=512), dict(T=2, ob=1024), dict(batch=5, slots=None), dict(scale=float("inf")),
-                                dict(scale=float("nan")), dict(capacity=4096, ws=None), dict(capacity=4096, ws_bytes=16),
-                                dict(capacity=4096, ws=A + 8)])
+                                dict(scale=float("nan"))])
 def test_attention_refuses(pn, kw):
     rc, msg = call(pn, "pi05_kv8_attention", *attention_args(**kw))
     assert rc == ERR_ARG and msg.startswith("pi05_kv8_attention:")
+
+
+@pytest.mark.parametrize("kw", [dict(ws=None), dict(ws_bytes=16), dict(ws=A + 8)])
+def test_attention_refuses_a_workspace_too_small(pn, kw):
+    kw = dict(batch=1, capacity=1 << 20, **kw)
+    assert pn.lib.pi05_kv8_attention_workspace(1, 1, 8, 2, 128, 1 << 20) > 16  # this shape needs one
+    rc, msg = call(pn, "pi05_kv8_attention", *attention_args(**kw))
+    assert rc == ERR_ARG and "workspace" in msg
 
 
 def test_workspace_of_a_bad_shape_is_an_error(pn):
