@@ -38,28 +38,28 @@ int launched(const char* what, char* err, size_t err_len) {
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // ------------------------------------------------------------------ quantisation
-// A half warp takes a block of 128 values, 8 a lane, and ITEMS consecutive blocks; memory-bound, so all loads are issued
-// before the first block is worked on, and the work on a block is kept to about 6 instructions a value (maxima on bit
-// patterns, one cross-lane reduction).
+// Eight lanes take a block of 128 values, 16 each, and ITEMS consecutive blocks, whose loads are all issued before the first
+// block is worked on.  Measured, 61952 x 2048 bf16: 56 us, 6.75 TB/s of its 381 MB, 1.03 of
+// the copy rate (8 values a lane, maxima by redux.sync over half warps: 70 us at 78 % of the issue slots); fp32 16384 x 4304 52 us, 6.75.
 template <typename X, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(256)
     fp8_quantize_kernel(const X* x, long ldx, int cols, uint32_t blocks, uint32_t items, uint8_t* q, long ldq, uint8_t* scales,
                         long lds) {
-  const int lane = threadIdx.x & 15;
-  const uint32_t first = (blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4)) * ITEMS;
+  const int lane = threadIdx.x & 7;
+  const uint32_t first = (blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3)) * ITEMS;
   const uint32_t row0 = first / blocks, blk0 = first - row0 * blocks;
   Fp8Raw<X> raw[ITEMS];
   uint32_t row = row0, blk = blk0;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
+    const int c0 = (int)blk * FP8_BLOCK + 16 * lane;
     raw[k].clear();
     if (first + k < items && c0 < cols) {
       const X* src = x + (long)row * ldx + c0;
       if (VEC)
         raw[k].load(src);
       else
-        raw[k].load_some(src, min(8, cols - c0));
+        raw[k].load_some(src, min(16, cols - c0));
     }
     if (++blk == blocks) blk = 0, ++row;
   }
@@ -67,16 +67,17 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     int byte;
-    const uint2 code = fp8_encode8<16>(raw[k], byte);
+    const uint4 code = fp8_encode16<8>(raw[k], byte);
     if (first + k < items) {
-      const int c0 = (int)blk * FP8_BLOCK + 8 * lane;
+      const int c0 = (int)blk * FP8_BLOCK + 16 * lane;
       uint8_t* dst = q + (long)row * ldq + c0;
-      if (c0 + 8 <= cols) {
-        *reinterpret_cast<uint2*>(dst) = code;
+      if (c0 + 16 <= cols) {
+        *reinterpret_cast<uint4*>(dst) = code;
       } else {
+        const uint32_t w[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c0 + i < cols) dst[i] = (uint8_t)((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
+        for (int i = 0; i < 16; ++i)
+          if (c0 + i < cols) dst[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
       }
       if (lane == 0) scales[(long)row * lds + blk] = (uint8_t)byte;
     }
@@ -102,13 +103,33 @@ __device__ __forceinline__ bool kv_span(const KvRows& a, int b, int& slot, long&
   return slot >= 0 && slot < a.n_slots;
 }
 
-// One thread an 8-value piece of a head row, HD / 8 neighbouring lanes a row, ITEMS rows a thread with their loads issued
+// One thread a piece of VALS values of a head row, HD / VALS neighbouring lanes a row, ITEMS rows a thread with their loads issued
 // together; grid (rows, batch, K | V).  Where two samples of a call name the same slot and position the later sample's
 // row is kept.
 template <int HD, bool WRITE, int ITEMS>
 __global__ void __launch_bounds__(256) kv8_rows_kernel(const KvRows a) {
-  constexpr int LANES = HD / 8;
+  constexpr int VALS = WRITE ? 16 : 8, LANES = HD / VALS;
   const int b = blockIdx.y;
+  const int per = blockDim.x / LANES, piece = threadIdx.x % LANES;
+  const long first = (long)blockIdx.x * per * ITEMS + threadIdx.x / LANES;  // head row of the sample
+  const bf16* src = blockIdx.z ? a.v : a.k;
+  bf16* dst = blockIdx.z ? a.vo : a.ko;
+  uint8_t* codes = (blockIdx.z ? a.v8 : a.k8) + VALS * piece;
+  uint8_t* bytes = blockIdx.z ? a.vs : a.ks;
+  uint32_t t[ITEMS], h[ITEMS];
+  long at[ITEMS];
+  Fp8Raw<bf16> raw[WRITE ? ITEMS : 1];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const uint32_t i = (uint32_t)(first + k * per);  // head rows of a sample: fewer than 2^31
+    t[k] = i / (uint32_t)a.kv_heads;
+    h[k] = i - t[k] * (uint32_t)a.kv_heads;
+    at[k] = (long)b * a.b_stride + (long)t[k] * a.t_stride + (long)h[k] * HD + VALS * piece;
+    if (WRITE) {  // on their way while the indices are read
+      raw[k].clear();
+      if (t[k] < (uint32_t)a.T) raw[k].load(src + at[k]);
+    }
+  }
   int slot, n;
   long p0;
   const bool mine = kv_span(a, b, slot, p0, n);
@@ -118,19 +139,12 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const KvRows a) {
     later = __syncthreads_or(later);
   }
   if (!mine) return;
-  const int per = blockDim.x / LANES, piece = threadIdx.x % LANES;
-  const long first = (long)blockIdx.x * per * ITEMS + threadIdx.x / LANES;  // head row of the sample
-  const bf16* src = blockIdx.z ? a.v : a.k;
-  bf16* dst = blockIdx.z ? a.vo : a.ko;
-  uint8_t* codes = (blockIdx.z ? a.v8 : a.k8) + 8 * piece;
-  uint8_t* bytes = blockIdx.z ? a.vs : a.ks;
-  long head[ITEMS], at[ITEMS];
+  long head[ITEMS];
   bool ok[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const uint32_t i = (uint32_t)(first + k * per), t = i / (uint32_t)a.kv_heads, h = i - t * (uint32_t)a.kv_heads;  // head_rows < 2^31
-    const long pos = p0 + t;
-    ok[k] = t < (uint32_t)n && pos >= 0 && pos < a.capacity;
+    const long pos = p0 + t[k];
+    ok[k] = t[k] < (uint32_t)n && pos >= 0 && pos < a.capacity;
     if (WRITE && later && ok[k]) {
       for (int o = b + 1; o < a.batch; ++o) {
         int so, no;
@@ -138,22 +152,15 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const KvRows a) {
         if (kv_span(a, o, so, po, no) && so == slot && pos >= po && pos < po + no) ok[k] = false;
       }
     }
-    head[k] = ((long)slot * a.capacity + pos) * a.kv_heads + h;
-    at[k] = (long)b * a.b_stride + (long)t * a.t_stride + (long)h * HD + 8 * piece;
+    head[k] = ((long)slot * a.capacity + pos) * a.kv_heads + h[k];
   }
   if (WRITE) {
-    Fp8Raw<bf16> raw[ITEMS];
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      raw[k].clear();
-      if (ok[k]) raw[k].load(src + at[k]);
-    }
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       int byte;
-      const uint2 code = fp8_encode8<LANES>(raw[k], byte);
+      const uint4 code = fp8_encode16<LANES>(raw[k], byte);
       if (ok[k]) {
-        *reinterpret_cast<uint2*>(codes + head[k] * HD) = code;
+        *reinterpret_cast<uint4*>(codes + head[k] * HD) = code;
         if (piece == 0) bytes[head[k]] = (uint8_t)byte;
       }
     }
@@ -193,10 +200,12 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
   if (!a.slots && a.batch > a.n_slots)
     return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
   const long head_rows = (long)a.T * a.kv_heads;
-  // 4 rows a thread, one where the call has too few for that to fill the machine
-  const int threads = 256, per = threads / (head_dim / 8);
+  // several rows a thread, one where the call has too few for that to fill the machine.  Measured (16 x 4099 x 8 x 128, 404 MB):
+  // writing 68 us with 16 values a thread and 2 rows (8 and 4: 95), reading 62 us with 8 and 4 (16 and 2: 71)
+  constexpr int MANY = WRITE ? 2 : 4;
+  const int threads = 256, per = threads / (head_dim / (WRITE ? 16 : 8));
   const bool few = head_rows * a.batch < 148L * 8 * per;
-  const long gx = (head_rows + per * (few ? 1 : 4) - 1) / (per * (few ? 1 : 4));
+  const long gx = (head_rows + per * (few ? 1 : MANY) - 1) / (per * (few ? 1 : MANY));
   if (head_rows > 0x7fffffffL) return fail(err, err_len, PI05_ERR_ARG, "%s: T * kv_heads must be below 2^31", what);
   const dim3 grid((unsigned)gx, a.batch, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -205,7 +214,7 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
     if (few)
       kv8_rows_kernel<HD, WRITE, 1><<<grid, threads, 0, st>>>(a);
     else
-      kv8_rows_kernel<HD, WRITE, 4><<<grid, threads, 0, st>>>(a);
+      kv8_rows_kernel<HD, WRITE, MANY><<<grid, threads, 0, st>>>(a);
   };
   if (head_dim == 64)
     go(std::integral_constant<int, 64>());
@@ -400,7 +409,7 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
     const double tiles = pairs * ceil(rows / 8), steps = ceil(capacity / 128.0);
     const double places = (double)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
     const double step = head_dim == 256 ? 1.8 : (head_dim == 128 ? 1.0 : 0.7);
-    for (int s = 1; s <= 256 && (s == 1 || s <= steps); s += s < 8 ? s : 8) {  // 1, 2, 4, 8, 16, 24, ...
+    for (int s = 1; s <= 256 && (s == 1 || s <= steps); s *= 2) {
       const double cost = ceil(tiles * s / places) * (6 + ceil(steps / s) * step) + (s > 8 ? 3 : 0);
       if (cost < best_cost) best_cost = cost, best = {false, s, s < 8 ? s : 8};
       if (tiles * s > 2 * places) break;
@@ -408,7 +417,7 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
   }
   if (head_dim >= 128) {  // a step: 64 keys
     const double tiles = pairs * ceil(rows / 128), steps = ceil(capacity / 64.0), step = head_dim == 256 ? 0.9 : 0.65;
-    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= steps); ++s) {
+    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= steps); s += 1 + s / 3) {
       const double cost = ceil(tiles * s / num_sms()) * (10 + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
       if (cost < best_cost) best_cost = cost, best = {true, s, 1};
       if (tiles * s > 2 * num_sms()) break;
@@ -480,10 +489,10 @@ extern "C" PI05_API int pi05_fp8_quantize(int64_t rows, int64_t cols, const void
     return fail(err, err_len, PI05_ERR_ARG,
                 "pi05_fp8_quantize: q must be 16-byte aligned with rows a multiple of 16 bytes apart, rows of x, q and "
                 "scales at least cols, cols and ceil(cols / 128) elements apart");
-  // 16-byte loads where every row starts on a 16-byte boundary and ends on a whole 8-value piece
-  const bool vec = aligned(x, 16) && (ldx * xb) % 16 == 0 && cols % 8 == 0;
-  constexpr int ITEMS = 4;
-  const uint32_t items = (uint32_t)(rows * blocks), per = 256 / 16 * ITEMS;
+  // 16-byte loads where every row starts on a 16-byte boundary and ends on a whole 16-value piece
+  const bool vec = aligned(x, 16) && (ldx * xb) % 16 == 0 && cols % 16 == 0;
+  constexpr int ITEMS = 2;
+  const uint32_t items = (uint32_t)(rows * blocks), per = 256 / 8 * ITEMS;
   const unsigned grid = (items + per - 1) / per;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* q8 = static_cast<uint8_t*>(q);

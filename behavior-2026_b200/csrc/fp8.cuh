@@ -50,69 +50,86 @@ __device__ __forceinline__ float2 fp8_to_f2(uint16_t c2) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// Eight values as they lie in memory.  Magnitudes are compared as bit patterns (of one sign they order like the values,
-// infinities and NaNs above all finite ones).
+// Sixteen values as they lie in memory.  Magnitudes are compared as bit patterns of bf16 or fp32 (infinities and NaNs are
+// above all finite ones).  These kernels are bound by instruction issue before memory, so the work on a value is
+// kept to about five instructions.
 template <typename X>
 struct Fp8Raw;
 template <>
 struct Fp8Raw<bf16> {
-  uint32_t w[4];
-  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
-  __device__ __forceinline__ void load(const bf16* p) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-  }
-  __device__ __forceinline__ void load_some(const bf16* p, int n) {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) w[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
-  }
-  __device__ __forceinline__ uint32_t top() const {  // as an fp32 bit pattern
-    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-    return max(m << 16, m & 0xffff0000u);
-  }
-  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
-};
-template <>
-struct Fp8Raw<float> {
   uint32_t w[8];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0u;
   }
-  __device__ __forceinline__ void load(const float* p) {
+  __device__ __forceinline__ void load(const bf16* p) {
     const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
     w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
   }
+  __device__ __forceinline__ void load_some(const bf16* p, int n) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < n) w[i / 2] |= (uint32_t)h[i] << (16 * (i & 1));
+  }
+  __device__ __forceinline__ uint32_t top() const {  // the largest magnitude's bf16 pattern (any NaN: 0x7fff)
+    auto m2 = [](uint32_t a, uint32_t b) {
+      const __nv_bfloat162 r = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+      return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    const uint32_t m = m2(m2(m2(w[0], w[1]), m2(w[2], w[3])), m2(m2(w[4], w[5]), m2(w[6], w[7])));
+    return max(m >> 16, m & 0xffffu);
+  }
+  // the scale byte of a largest magnitude 1.m * 2^x: x - 8 + 127, one more where 1.m > 1.75 (448 = 1.75 * 2^8)
+  static constexpr uint32_t BAD = 0x7f80u;
+  __device__ __forceinline__ static int byte(uint32_t top) { return max((int)((top + 0x1fu) >> 7) - 8, 0); }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+};
+template <>
+struct Fp8Raw<float> {
+  uint32_t w[16];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = a.x, w[4 * i + 1] = a.y, w[4 * i + 2] = a.z, w[4 * i + 3] = a.w;
+    }
+  }
   __device__ __forceinline__ void load_some(const float* p, int n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 16; ++i)
       if (i < n) w[i] = __float_as_uint(p[i]);
   }
   __device__ __forceinline__ uint32_t top() const {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+    for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
     return m;
   }
+  static constexpr uint32_t BAD = 0x7f800000u;
+  __device__ __forceinline__ static int byte(uint32_t top) { return max((int)((top + 0x1fffffu) >> 23) - 8, 0); }
   __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
 };
 
-// The codes of a lane's eight values and the exponent byte of the block that LANES consecutive lanes hold.
+// The codes of a lane's sixteen values and the exponent byte of the block that LANES consecutive lanes hold.
 // Every lane of the warp calls it.
 template <int LANES, typename X>
-__device__ __forceinline__ uint2 fp8_encode8(const Fp8Raw<X>& x, int& byte) {
-  const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
-  const uint32_t m = __reduce_max_sync(mask, x.top());
-  if (m >= 0x7f800000u) {  // an infinity or a NaN
-    byte = 255;
-    return make_uint2(0u, 0u);
-  }
-  byte = fp8_scale_byte(__uint_as_float(m));
-  const float r = fp8_scale_inverse(byte);
-  return make_uint2(fp8_pack4(x.at(0) * r, x.at(1) * r, x.at(2) * r, x.at(3) * r),
-                    fp8_pack4(x.at(4) * r, x.at(5) * r, x.at(6) * r, x.at(7) * r));
+__device__ __forceinline__ uint4 fp8_encode16(const Fp8Raw<X>& x, int& byte) {
+  uint32_t m = x.top();
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const bool bad = m >= Fp8Raw<X>::BAD;  // an infinity or a NaN: codes 0
+  const int b = Fp8Raw<X>::byte(m);      // at most 247
+  byte = bad ? 255 : b;
+  const float r = __uint_as_float((uint32_t)(254 - b) << 23);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = fp8_pack4(x.at(4 * i) * r, x.at(4 * i + 1) * r, x.at(4 * i + 2) * r, x.at(4 * i + 3) * r);
+  return bad ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(c[0], c[1], c[2], c[3]);
 }
 
 }  // namespace p5
