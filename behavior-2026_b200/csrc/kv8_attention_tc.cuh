@@ -11,9 +11,10 @@
 //                 chain (load, scale, maximum, exponentials, store) runs beside the next one's.  They share the running maximum
 //                 of a row through shared memory: a tile's warp waits for its turn, raises the maximum if it must, and passes
 //                 the turn on before its exponentials.  Each keeps its own sum.
-//   O += P V      kind::f16, P in fp16 with the V row's scale folded in (11 bits, as in kv8_attention.cuh), V widened to
-//                 fp16 by four converter warps (exact; keys that no row sees become zeros, whatever the cache holds there).
-//                 An e4m3 P would need three operands to keep the small weights of a long cache.
+//   O += P V      kind::f16, P in fp16 (11 bits; as 2^7 p, which keeps weights down to 2^-31 of the largest), V widened to fp16
+//                 and scaled by its row's power of two relative to a running exponent eb by four converter warps (exact;
+//                 keys that no row sees become zeros, whatever the cache holds there).  An e4m3 P would need three
+//                 operands to keep the small weights of a long cache.
 // The running maximum moves only when a tile exceeds it by 2^8 and the V exponent eb only when a scale exceeds it by 2^7;
 // both rescale O through tcgen05.ld/st.  eb is the same for all rows and kept by the warp that loads the scales.
 //   warp 0 TMA, warp 1 MMA issue, warp 2 TMEM, warp 3 scales, warps 4-11 softmax, warps 12-15 V
@@ -34,7 +35,7 @@ struct Kv8TcCfg {
   static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8;
   static constexpr int Q_BYTES = ROWS * (HD * 2 + 16);  // query rows on their way in, over the widened V
   static constexpr int SC_OFF = W_OFF + (2 * TILE16 > Q_BYTES ? 2 * TILE16 : (Q_BYTES + 127) / 128 * 128);
-  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64], vf[64], rescale factor of O
+  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64] (fp32), vf[64] (fp16, twice), rescale factor of O
   static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
   static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
   static constexpr int SMEM = 1024 + BAR_OFF + 512;
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* w_full = v_empty + C::NK;                                // [2] widened V in place (4 warps)
   uint64_t* w_empty = w_full + 2;                                    // [2] P V product done
   uint64_t* sc_full = w_empty + 2;                                   // [NSC] scales in place
-  uint64_t* sc_empty = sc_full + C::NSC;                             // [NSC] read by the tile's 4 softmax warps
+  uint64_t* sc_empty = sc_full + C::NSC;                             // [NSC] read by the tile's 4 softmax warps and the 4 of V
   uint64_t* s_full = sc_empty + C::NSC;                              // [2] of the even and the odd tiles
   uint64_t* s_empty = s_full + 2;                                    // [2] (4 warps)
   uint64_t* p_full = s_empty + 2;                                    // [2] (4 warps)
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(512, 1)
     }
     for (int i = 0; i < C::NSC; ++i) {
       mbar_init(&sc_full[i], 1);
-      mbar_init(&sc_empty[i], 4);
+      mbar_init(&sc_empty[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&w_full[i], 4);
@@ -288,7 +289,8 @@ __global__ void __launch_bounds__(512, 1)
     load(0);
     for (int i = 0; i < n; ++i) {
       const int s = i % C::NSC;
-      float kf[2], vf[2];
+      float kf[2];
+      uint32_t vf[2];
       int ev[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -303,7 +305,10 @@ __global__ void __launch_bounds__(512, 1)
         eb = em;
       }
 #pragma unroll
-      for (int q = 0; q < 2; ++q) vf[q] = exp2_int(ev[q] - eb);
+      for (int q = 0; q < 2; ++q) {  // 2^(ev - eb) <= 2^7 in fp16, for two dims at a time
+        const int e = ev[q] - eb;
+        vf[q] = (e < -24 ? 0u : (e < -14 ? 1u << (e + 24) : (uint32_t)(e + 15) << 10)) * 0x10001u;
+      }
       bool ok = !flags[0] && mbar_wait(&sc_empty[s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
       if (!__all_sync(0xffffffffu, ok)) {
         flags[0] = 1;
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(512, 1)
       }
       float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
       *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
-      *reinterpret_cast<float2*>(sc + C::KT + 2 * lane) = make_float2(vf[0], vf[1]);
+      *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
       if (lane == 0) {
         sc[2 * C::KT] = rescale;
         flags[1] = eb;
@@ -328,7 +333,9 @@ __global__ void __launch_bounds__(512, 1)
     if (!mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN)) flags[0] = 1;  // Q is staged where widened V goes
     for (int i = 0; i < n; ++i) {
       const int s = i % C::NK, wb = i & 1;
+      const int ss = i % C::NSC;
       const bool ok = !flags[0] && mbar_wait(&v_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                      mbar_wait(&sc_full[ss], (uint32_t)(i / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
                       mbar_wait(&w_empty[wb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
       if (!__all_sync(0xffffffffu, ok)) {
         flags[0] = 1;
@@ -336,6 +343,7 @@ __global__ void __launch_bounds__(512, 1)
       }
       const int valid = top - (j0 + i) * C::KT;  // rows from here on become zeros
       const uint8_t* src = smem + C::V_OFF + s * C::TILE8;
+      const uint32_t* vf = reinterpret_cast<const uint32_t*>(smem + C::SC_OFF + ss * C::SC_SLOT) + C::KT;
       uint8_t* dst = smem + C::W_OFF + wb * C::TILE16;
 #pragma unroll
       for (int k = 0; k < C::KT * HD / 16 / 128; ++k) {
@@ -346,16 +354,21 @@ __global__ void __launch_bounds__(512, 1)
         const int piece = group * 4 + j4;  // 16-byte piece of the key's codes
         uint4 u = *reinterpret_cast<const uint4*>(src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
         if (row >= valid) u = make_uint4(0, 0, 0, 0);
+        const uint32_t f = vf[row];
+        auto two = [&](uint32_t c) {
+          const uint32_t h = fp8_to_h2((uint16_t)c);
+          const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&f));
+          return *reinterpret_cast<const uint32_t*>(&x);
+        };
         uint8_t* d = dst + group * (C::KT * 128) + row * 128;
-        *reinterpret_cast<uint4*>(d + (((2 * j4) ^ (row & 7)) << 4)) =
-            make_uint4(fp8_to_h2((uint16_t)u.x), fp8_to_h2((uint16_t)(u.x >> 16)), fp8_to_h2((uint16_t)u.y), fp8_to_h2((uint16_t)(u.y >> 16)));
-        *reinterpret_cast<uint4*>(d + (((2 * j4 + 1) ^ (row & 7)) << 4)) =
-            make_uint4(fp8_to_h2((uint16_t)u.z), fp8_to_h2((uint16_t)(u.z >> 16)), fp8_to_h2((uint16_t)u.w), fp8_to_h2((uint16_t)(u.w >> 16)));
+        *reinterpret_cast<uint4*>(d + (((2 * j4) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.x >> 16), two(u.y), two(u.y >> 16));
+        *reinterpret_cast<uint4*>(d + (((2 * j4 + 1) ^ (row & 7)) << 4)) = make_uint4(two(u.z), two(u.z >> 16), two(u.w), two(u.w >> 16));
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&v_empty[s]);
+        mbar_arrive(&sc_empty[ss]);
         mbar_arrive(&w_full[wb]);
       }
     }
@@ -469,6 +482,8 @@ __global__ void __launch_bounds__(512, 1)
       // in base 2: rf carries the row's power of two, the softmax scale and log2 e
       const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
       const float rescale = sc[2 * C::KT];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc_empty[ss]);
       bool need = rescale != 1.f;
       float alpha = rescale, m = mt;
       if (j > 0) {  // the turn: the maximum after tile j - 1
@@ -486,26 +501,22 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(&turn[4 * (g ^ 1) + sub]);
       l_run *= m_run == m ? 1.f : (m_run == -INFINITY ? 0.f : ex2_approx(m_run - m));
       m_run = m;
-      const float msc = m == -INFINITY ? 0.f : m;
+      const float msc = m == -INFINITY ? 0.f : m - 7.f;  // p and l as 2^7 of themselves, which O / l forgets
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       const float2 rf2 = make_float2(rf, rf), nm2 = make_float2(-msc, -msc);
       uint32_t pk[C::KT / 2];
 #pragma unroll
       for (int c = 0; c < C::KT; c += 4) {
-        const float4 v4 = *reinterpret_cast<const float4*>(sc + C::KT + c);
         const float2 x0 = fma2(make_float2(x[c], x[c + 1]), rf2, nm2);
         const float2 x1 = fma2(make_float2(x[c + 2], x[c + 3]), rf2, nm2);
         const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
         ls[0] = add2(ls[0], p0);
         ls[1] = add2(ls[1], p1);
-        const float2 w0 = mul2(p0, make_float2(v4.x, v4.y)), w1 = mul2(p1, make_float2(v4.z, v4.w));
-        const __half2 h0 = __floats2half2_rn(w0.x, w0.y), h1 = __floats2half2_rn(w1.x, w1.y);
+        const __half2 h0 = __floats2half2_rn(p0.x, p0.y), h1 = __floats2half2_rn(p1.x, p1.y);
         pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
         pk[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
       }
       l_run += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sc_empty[ss]);
       // P buffer g was last read by the P V product of tile j - 2
       ok = ok && mbar_wait(&p_empty[g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
       __syncwarp();
