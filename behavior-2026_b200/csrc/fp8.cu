@@ -197,6 +197,8 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
     return fail(err, err_len, PI05_ERR_ARG,
                 "%s: k, v and the caches must be 16-byte aligned device pointers, rows at least kv_heads * head_dim "
                 "elements and a multiple of 8 apart", what);
+  if (!WRITE && a.batch > 1 && a.b_stride < a.t_stride * (a.T - 1) + (long)a.kv_heads * head_dim)
+    return fail(err, err_len, PI05_ERR_ARG, "%s: samples of k, v overlap", what);
   if (!a.slots && a.batch > a.n_slots)
     return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
   const long head_rows = (long)a.T * a.kv_heads;
@@ -378,7 +380,10 @@ int linear(Fp8Args& a, const void* x, long ldx, const void* w, long ldw, int K, 
                : cudaSuccess;
   }
   if (!mapped) return fail(err, err_len, PI05_ERR_ARG, "pi05_fp8_linear: tensor map rejected the operands");
-  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_fp8_linear: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(err, err_len, PI05_ERR_CUDA, "pi05_fp8_linear: %s", cudaGetErrorString(e));
+  }
   return launched("pi05_fp8_linear", err, err_len);
 }
 
@@ -467,7 +472,10 @@ int attention(const Kv8Args& a, int batch, int cluster, cudaStream_t st, char* e
   cfg.numAttrs = 1;
   void* params[] = {const_cast<Kv8Args*>(&a)};
   const cudaError_t e = cudaLaunchKernelExC(&cfg, (const void*)kv8_attn_rows_kernel<HD>, params);
-  if (e != cudaSuccess) return fail(err, err_len, PI05_ERR_CUDA, "pi05_kv8_attention: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(err, err_len, PI05_ERR_CUDA, "pi05_kv8_attention: %s", cudaGetErrorString(e));
+  }
   if (a.groups > 1) {
     const long rows = (long)batch * a.T * a.heads;
     kv8_attn_combine_kernel<HD><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, batch);
@@ -602,10 +610,10 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
                                            int64_t out_sample_stride, int64_t out_token_stride, void* workspace,
                                            int64_t workspace_bytes, void* stream, char* err, size_t err_len) {
   if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || n_slots < 1 || capacity < 1 ||
-      (int64_t)batch * kv_heads > 65535 || (int64_t)T * (heads / kv_heads) > (1 << 30) || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+      (int64_t)batch * kv_heads > 65535 || (int64_t)T * (heads / kv_heads) > (1 << 30) || (int64_t)batch * T > 0x7fffffff / heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return fail(err, err_len, PI05_ERR_ARG,
                 "pi05_kv8_attention: needs batch, T, n_slots, capacity >= 1, heads a multiple of kv_heads, head_dim 64, 128 "
-                "or 256, batch * kv_heads <= 65535");
+                "or 256, batch * kv_heads <= 65535, batch * T * heads < 2^31");
   const int64_t width = (int64_t)heads * head_dim;
   if (!q || !k8 || !k_scales || !v8 || !v_scales || !lens || !out || !aligned(q, 16) || !aligned(k8, 16) || !aligned(v8, 16) ||
       !aligned(out, 16) || q_sample_stride % 8 || q_token_stride % 8 || out_sample_stride % 8 || out_token_stride % 8 ||

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
     const bool in = r < rows;
     const int t = in ? r / a.G : 0, h = kvh * a.G + (in ? r % a.G : 0);
     const bf16* src = a.q + (long)b * a.q_b + (long)t * a.q_t + (long)h * HD;
-    float m = 0.f;
+    uint32_t mb = 0;
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
@@ -163,14 +163,12 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 f = unpack_bf2(qf[i][j]);
-        m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      for (int j = 0; j < 8; ++j) mb = __vmaxu2(mb, qf[i][j] & 0x7fff7fffu);  // magnitudes as bf16 patterns
+    mb = max(mb >> 16, mb & 0xffffu);
+    mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+    mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
     // |q| < 2^(e + 1); the row is scaled by 2^(14 - e) (kept within the float range)
-    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -112), 127);
+    const int e = min(max((int)(mb >> 7) - 127, -112), 127);
     const float up = exp2_int(14 - e);
 #pragma unroll
     for (int i = 0; i < KI; ++i)
@@ -180,7 +178,8 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
         const __half2 hh = __floats2half2_rn(f.x * up, f.y * up);
         qf[i][j] = *reinterpret_cast<const uint32_t*>(&hh);
       }
-    const float down = a.scale_log2 * exp2_int(e - 14);
+    // a query with a NaN or an infinity: its row is NaN, unless it sees no key
+    const float down = mb >= 0x7f80u ? NAN : a.scale_log2 * exp2_int(e - 14);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       rf[j] = __shfl_sync(0xffffffffu, down, (2 * c + j) * 4);

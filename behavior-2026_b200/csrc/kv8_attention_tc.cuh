@@ -377,6 +377,7 @@ __global__ void __launch_bounds__(512, 1)
     // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
     // Q and O at the start and the end
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
+    const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
     float rf;
     {
       const uint8_t* sq = smem + C::W_OFF;
@@ -393,14 +394,14 @@ __global__ void __launch_bounds__(512, 1)
       exch[g * 128 + r] = __uint_as_float(mb << 16);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       mb = max(__float_as_uint(exch[r]), __float_as_uint(exch[128 + r]));
-      const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN
+      const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN, unless it sees no key
       const int byte = bad ? 127 : fp8_scale_byte(__uint_as_float(mb));
       // rf > 0, so that a masked logit of -inf stays one: the sign of the softmax scale goes into Q, and a scale of 0 makes
       // Q zero
       const float sign = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
       const float up = bad ? 0.f : sign * fp8_scale_inverse(byte);
       const float2 up2 = make_float2(up, up);
-      rf = bad ? NAN : (sign == 0.f ? 1.f : fp8_scale_value(byte) * fabsf(a.scale_log2));
+      rf = bad && lim > 0 ? NAN : (sign == 0.f ? 1.f : fp8_scale_value(byte) * fabsf(a.scale_log2));
       constexpr int NC = HD / 8;  // columns of this half: four codes each
 #pragma unroll 1
       for (int i = 0; i < NC; i += 16) {
@@ -430,7 +431,6 @@ __global__ void __launch_bounds__(512, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
     float* m_ref = exch + 4 * C::ROWS + r;  // the row's running maximum
     float m_run = -INFINITY, l_run = 0.f;
     bool alive = true;

@@ -272,7 +272,8 @@ PI05_API int pi05_linear_static_status(void* stream, char* err, size_t err_len);
  * model is 17.8 MB an environment, this cache 9 MB).  They need no engine: like pi05_linear_static each call takes the
  * caller's stream (a cudaStream_t, NULL = legacy default stream) and device pointers of the current device, allocates
  * nothing, is asynchronous, may be captured into a CUDA graph, and writes a message to err when it refuses.  Calls share
- * no state, so they may overlap on the GPU as long as their buffers (a workspace among them) are their own.
+ * no state, so they may overlap on the GPU as long as their buffers (a workspace among them) are their own.  The first call on
+ * a device prepares the kernels there and should come before any stream capture.
  * No counterpart in the reference's ABI (its engine was bf16, π05_네이티브엔진.md:102-105).
  *
  * Format: an e4m3 code c (finite, 1 byte) and one exponent byte s for each block stand for c * 2^(s - 127); s - 127 is
@@ -303,12 +304,13 @@ PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
  * outside [0, n_slots) is passed over, as are positions outside [0, capacity).
  * pi05_kv8_write: rows t < count[b] (count NULL: T; clamped to [0, T]) of k, v (bf16, sample b's token t at
  *   b * sample_stride + t * token_stride elements, its kv_heads * head_dim values contiguous, 16-byte aligned) go to positions
- *   start[b] + t (start NULL: t).  Everything else in the cache stays as it was.  Where two samples name the same
+ *   start[b] + t (start NULL: t).  Samples of k, v may overlap (a stride of 0).  Everything else in the cache stays as it was.  Where two samples name the same
  *   slot and position the later sample's row is kept.
  * pi05_kv8_read: the reverse; rows that are passed over stay as they were in k and v.
  * pi05_kv8_attention: out[b][t][h] = sum_j p_j V_j, p = softmax over j < lens[b] (clamped to [0, capacity]) of
  *   scale * q[b][t][h] . K_j; causal != 0: token t sees j < lens[b] - T + t + 1 (the last token sees all, as after a write of
- *   the T tokens).  A row that sees nothing gives 0.  heads is a multiple of kv_heads; query head h reads K/V head
+ *   the T tokens).  A row that sees nothing gives 0; one that sees a NaN row of the cache, or whose query holds a NaN or an
+ *   infinity, gives NaN.  heads is a multiple of kv_heads; query head h reads K/V head
  *   h / (heads / kv_heads).  q and out bf16, token t of sample b at b * sample stride + t * token stride elements, heads
  *   contiguous, 16-byte aligned.  workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
  *   of no importance before and after. */

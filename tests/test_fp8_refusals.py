@@ -72,12 +72,17 @@ def test_cache_rows_refuse(pn, name, kw):
     assert rc == ERR_ARG and msg.startswith(name + ":")
 
 
+def test_reading_into_overlapping_samples_is_refused(pn):
+    rc, msg = call(pn, "pi05_kv8_read", *rows_args(sb=768))
+    assert rc == ERR_ARG and "overlap" in msg
+
+
 @pytest.mark.parametrize("kw", [dict(batch=0), dict(T=0), dict(heads=0), dict(kvh=0), dict(heads=7), dict(hd=80), dict(n_slots=0),
                                 dict(capacity=0), dict(batch=40000), dict(q=None), dict(k8=None), dict(ks=None), dict(v8=None),
                                 dict(vs=None), dict(lens=None), dict(out=None), dict(q=A + 8), dict(k8=A + 8), dict(v8=A + 8),
                                 dict(out=A + 8), dict(qb=1020), dict(qt=1020), dict(qt=1016), dict(ot=1016), dict(ob=1020),
                                 dict(ob=512), dict(T=2, ob=1024), dict(batch=5, slots=None), dict(scale=float("inf")),
-                                dict(scale=float("nan"))])
+                                dict(scale=float("nan")), dict(T=1 << 24, heads=512, ob=1 << 62)])
 def test_attention_refuses(pn, kw):
     rc, msg = call(pn, "pi05_kv8_attention", *attention_args(**kw))
     assert rc == ERR_ARG and msg.startswith("pi05_kv8_attention:")

@@ -510,6 +510,75 @@ def test_attention_small_weights_add_up(pn):
         assert (got.float() - ref).abs().max() <= (2.0**-4 + 2.0**-8) * ref
 
 
+@pytest.mark.parametrize("T", [2, 40, 130])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_query_with_nan_or_infinity(pn, T, hd):
+    """its rows are NaN where they see a key and 0 where they see none; all others are as without it"""
+    g = gen(27)
+    cache = filled(pn, g, 2, 90, 1, hd)
+    q = randn(g, 2, T, 8, hd, dtype=BF)
+    lens = i32(90, T - 1)  # causal: the second sample's first token sees nothing
+    want = pn.kv8_attention(q, *cache, lens=lens, causal=True)
+    bad = q.clone()
+    bad[0, 1, 2, 5], bad[0, T - 1, 7, 0] = math.nan, math.inf
+    bad[1, 0, 1, 3], bad[1, T - 1, 0, 9] = -math.inf, math.nan
+    got = pn.kv8_attention(bad, *cache, lens=lens, causal=True)
+    sees = (lens[:, None] - T + 1 + torch.arange(T, device="cuda")) > 0
+    isbad = ~torch.isfinite(bad).all(-1) & sees[..., None]
+    assert torch.equal(torch.isnan(got).all(-1), isbad) and torch.equal(torch.isnan(got).any(-1), isbad)
+    assert torch.equal(got[~isbad], want[~isbad]) and (got[~sees] == 0).all() and isbad.any()
+
+
+@pytest.mark.parametrize("T", [1, 60])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0])
+def test_attention_other_scales(pn, T, scale):
+    g = gen(28)
+    cache = filled(pn, g, 2, 150, 1, 256)
+    check_attention(pn, randn(g, 2, T, 8, 256, dtype=BF) * 0.3, cache, i32(150, 70), scale=scale, causal=True)
+
+
+def test_attention_one_query_for_all_samples(pn):
+    """a query broadcast over the batch (sample stride 0)"""
+    g = gen(29)
+    cache = filled(pn, g, 4, 100, 2, 128)
+    for T in (1, 40):
+        q = randn(g, 1, T, 8, 128, dtype=BF).expand(4, -1, -1, -1)
+        got = pn.kv8_attention(q, *cache, lens=i32(100, 5, 64, 0))
+        assert torch.equal(got, pn.kv8_attention(q.contiguous(), *cache, lens=i32(100, 5, 64, 0)))
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_attention_with_workspaces_on_two_streams_and_in_graphs(pn, T):
+    g = gen(30)
+    cap = 40000
+    assert pn.lib.pi05_kv8_attention_workspace(1, T, 8, 1, 256, cap) > 0
+    runs = []
+    for i in range(2):
+        runs.append((randn(g, 1, T, 8, 256, dtype=BF), filled(pn, g, 1, cap, 1, 256), i32(cap - 3 * i)))
+    want = [pn.kv8_attention(q, *c, lens=n) for q, c, n in runs]
+    side = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for (q, c, n), s in zip(runs, side):
+            with torch.cuda.stream(s):
+                got.append(pn.kv8_attention(q, *c, lens=n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+    graphs, outs = [], []
+    for q, c, n in runs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(pn.kv8_attention(q, *c, lens=n))
+        graphs.append(gr)
+    for _ in range(3):
+        for gr, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 @pytest.mark.parametrize("T", [1, 50])
 def test_attention_strided_query_and_out(pn, T):
     g = gen(25)
@@ -650,6 +719,10 @@ def test_offsets_past_32_bits(pn):
     got = pn.kv8_attention(q, *cache, lens=i32(cap), slots=i32(8), causal=True)
     small = pn.kv8_attention(q, *(c[8:, cap - 70 :].contiguous() for c in cache), lens=i32(70), causal=True)
     assert ((got.float() - small.float()).abs() <= 2.0**-7 * small.float().abs() + 1e-6).all()  # keys of zeros weigh e^-100s
+    q = (40 * k[:, -60:].repeat_interleave(4, 2)).contiguous()
+    got = pn.kv8_attention(q, *cache, lens=i32(cap), slots=i32(8), causal=True)
+    small = pn.kv8_attention(q, *(c[8:, cap - 70 :].contiguous() for c in cache), lens=i32(70), causal=True)
+    assert ((got.float() - small.float()).abs() <= 2.0**-7 * small.float().abs() + 1e-6).all()
     del cache, k8, ks
     x = torch.zeros(1 << 17, 17000, device="cuda", dtype=BF)
     x[-1] = randn(g, 17000, dtype=BF)
