@@ -319,15 +319,16 @@ struct LinearPlan {
 
 // Picks the kernel and its tile by an estimate of its time in microseconds, fitted to measurements of 27 shapes (tokens
 // 1 to 7744, features 1024 to 32768, K 1024 to 16384; each plan forced in turn).  A K block costs an SM what its operand
-// bytes take to arrive; a cluster's exchange grows with its CTAs.  E.g. 50 x 8192 x 1024: 32-token tiles 6.4, 64 8.2, pair
-// kernel 12.5; 968 x 2560 x 2048: pair 11.8 (160 features), 12.9 (240), 64-token tiles 18.3; 50 x 1024 x 4096: one
-// CTA a tile 13.2, clusters of four 7.4; 7744 x 2048 x 16384: pair 204 (240), 262 (128), 128-token tiles 413.
+// bytes take to arrive; a cluster's exchange grows with its CTAs and its tile.  E.g. 50 x 8192 x 1024: 32-token tiles 6.9, 64
+// 8.1, pair kernel 11.4; 968 x 2560 x 2048: pair 11.8 (160 features), 12.9 (240), 64-token tiles 18.3; 50 x 1024 x 4096:
+// one CTA a tile 13.2, clusters of four 7.4; 768 x 1152 x 4304: 128-token tiles in clusters of two 14.8, of one 18.6, pair
+// 18.9; 7744 x 2048 x 16384: pair 204 (240), 262 (128), 128-token tiles 413.
 LinearPlan linear_plan(int T, int F, int blocks, int sms) {
   LinearPlan best = {0, 0, 1};
   double best_cost = 1e300;
   for (int bn = 240; bn >= 128; bn -= 16) {
     const double units = (double)((T + 255) / 256) * ((F + bn - 1) / bn);
-    const double cost = 5.5 + ceil(units / (sms / 2)) * (blocks * (0.26 + 0.0005 * bn) + 0.3);
+    const double cost = 5.5 + 0.012 * bn + ceil(units / (sms / 2)) * (blocks * (0.26 + 0.0005 * bn) + 0.3);
     if (cost < best_cost) best_cost = cost, best = {0, bn, 1};
   }
   for (int bn = 32; bn <= 128; bn *= 2) {
@@ -335,8 +336,10 @@ LinearPlan linear_plan(int T, int F, int blocks, int sms) {
     const double tiles = (double)((F + 127) / 128) * ((T + bn - 1) / bn);
     const double block = bn == 32 ? 0.36 : (bn == 64 ? 0.47 : 0.42);
     for (int s = 1; s <= 8 && s <= blocks; s *= 2) {
-      const double on_an_sm = ceil(tiles * s / sms);
-      const double cost = 3.7 + on_an_sm * ((blocks + s - 1) / s * block + (s > 1 ? 0.3 + 0.4 * s : 0));
+      const double exchange = s == 1 ? 0 : (bn == 32 ? 0.3 + 0.3 * s : (bn == 64 ? 0.6 + 0.4 * s : 3.0 + 0.5 * s));
+      // two CTAs of the smaller tiles share an SM, so a second one's fill and epilogue are hidden; of the largest they add up
+      const double work = (blocks + s - 1) / s * block + exchange;
+      const double cost = bn == 128 ? 0.2 + ceil(tiles * s / sms) * (work + 4.5) : 3.7 + std::max(1.0, tiles * s / sms) * work;
       if (cost < best_cost) best_cost = cost, best = {bn, bn, s};
     }
   }
