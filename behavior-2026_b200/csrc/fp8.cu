@@ -609,7 +609,8 @@ extern "C" PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int h
 extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_heads, int head_dim, const void* q,
                                            int64_t q_sample_stride, int64_t q_token_stride, int n_slots, int capacity,
                                            const void* k8, const uint8_t* k_scales, const void* v8, const uint8_t* v_scales,
-                                           const int32_t* lens, const int32_t* slots, int causal, float scale, void* out,
+                                           const int32_t* lens, const int32_t* count, const int32_t* slots, int causal, float scale,
+                                           void* out,
                                            int64_t out_sample_stride, int64_t out_token_stride, void* workspace,
                                            int64_t workspace_bytes, void* stream, char* err, size_t err_len) {
   if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || n_slots < 1 || capacity < 1 ||
@@ -638,6 +639,7 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
   a.v = static_cast<const uint8_t*>(v8);
   a.vs = v_scales;
   a.lens = lens;
+  a.count = count;
   a.slots = slots;
   a.out = static_cast<bf16*>(out);
   a.o_b = out_sample_stride;

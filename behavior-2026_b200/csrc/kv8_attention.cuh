@@ -1,6 +1,7 @@
 // kv8_attention.cuh — attention over the 8-bit K/V cache (fp8.cuh) for few query rows.
 //
-//   out[b][t][h][:] = sum_j p_j V_j,  p = softmax_j(scale * q . K_j),  j < lens[b] (causal: j < lens[b] - T + t + 1)
+//   out[b][t][h][:] = sum_j p_j V_j,  p = softmax_j(scale * q . K_j),  j < lens[b] (causal: j < lens[b] - n + t + 1)
+// for the tokens t < n of sample b, n = count[b] (T without counts)
 //
 // The query heads of a K/V head and the T tokens of a sample are folded into rows r = t * G + g.  A CTA owns 8 of the
 // rows of one (sample, K/V head) and one key split; its warps walk steps of 32 keys, each warp the steps w, w + W, ... of the
@@ -36,6 +37,7 @@ struct Kv8Args {
   long q_b, q_t;  // elements between samples, tokens; heads are head_dim apart
   const uint8_t *k, *ks, *v, *vs;
   const int* lens;
+  const int* count;  // query tokens of a sample; NULL: T
   const int* slots;  // NULL: sample b is slot b
   bf16* out;
   long o_b, o_t;
@@ -45,6 +47,9 @@ struct Kv8Args {
   float* ws_o;         // [groups][batch][heads * T][head_dim], O in units of the group's 2^m
   float2* ws_ml;       // [groups][batch][heads * T] (m, l)
 };
+
+// query tokens of sample b
+__device__ __forceinline__ int kv8_tokens(const Kv8Args& a, int b) { return a.count ? max(0, min(a.count[b], a.T)) : a.T; }
 
 __device__ __forceinline__ uint32_t movmatrix_b16(uint32_t v) {
   uint32_t r;
@@ -100,13 +105,13 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-  const int rows = a.T * a.G, row0 = blockIdx.x * 8;
+  const int tokens = kv8_tokens(a, b), rows = tokens * a.G, row0 = blockIdx.x * 8;
   const int split = blockIdx.z;
   const int slot = a.slots ? a.slots[b] : b;
   const int len = (slot < 0 || slot >= a.n_slots) ? 0 : max(0, min(a.lens[b], a.capacity));
   // keys that any of the CTA's rows sees
   const int t_last = min(row0 + 8, rows) - 1;
-  const int top = a.causal ? max(0, min(len, len - a.T + t_last / a.G + 1)) : len;
+  const int top = row0 >= rows ? 0 : (a.causal ? max(0, min(len, len - tokens + t_last / a.G + 1)) : len);
   // the split's steps
   const int steps = (top + C::KEYS - 1) / C::KEYS;
   const int per = (steps + a.splits - 1) / a.splits;
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
     for (int j = 0; j < 2; ++j) {
       rf[j] = __shfl_sync(0xffffffffu, down, (2 * c + j) * 4);
       const int rr = row0 + 2 * c + j;
-      lim[j] = rr >= rows ? 0 : (a.causal ? min(len, len - a.T + rr / a.G + 1) : len);
+      lim[j] = rr >= rows ? 0 : (a.causal ? min(len, len - tokens + rr / a.G + 1) : len);
     }
   }
 
@@ -445,7 +450,7 @@ __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
   const int lane = threadIdx.x & 31;
   const long rows = (long)batch * a.T * a.heads;
   const long i = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (i >= rows) return;
+  if (i >= rows || (a.count && (int)(i % a.T) >= kv8_tokens(a, (int)(i / ((long)a.T * a.heads))))) return;
   float m = -INFINITY;
   for (int s = 0; s < a.groups; ++s) m = fmaxf(m, a.ws_ml[s * rows + i].x);
   float l = 0.f, acc[HD / 32];

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(512, 1)
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-  const int rows = a.T * a.G;
+  const int tokens = kv8_tokens(a, b), rows = tokens * a.G;
   // the last rows first: under a causal mask they have the most keys
   const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * C::ROWS;
   const int split = blockIdx.z;
@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(512, 1)
   const int slot = a.slots ? a.slots[b] : b;
   const int len = (slot < 0 || slot >= a.n_slots) ? 0 : max(0, min(a.lens[b], a.capacity));
   const int t_last = (min(row0 + C::ROWS, rows) - 1) / a.G;
-  const int top = a.causal ? max(0, min(len, len - a.T + t_last + 1)) : len;  // keys that any of the rows sees
+  // keys that any of the rows sees
+  const int top = row0 >= rows ? 0 : (a.causal ? max(0, min(len, len - tokens + t_last + 1)) : len);
   const int tiles = (top + C::KT - 1) / C::KT;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int j0 = min(split * per, tiles), n = min(j0 + per, tiles) - j0;
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(512, 1)
     // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
     // Q and O at the start and the end
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
-    const int lim = !in ? 0 : (a.causal ? min(len, len - a.T + t + 1) : len);
+    const int lim = !in ? 0 : (a.causal ? min(len, len - tokens + t + 1) : len);
     float rf;
     {
       const uint8_t* sq = smem + C::W_OFF;

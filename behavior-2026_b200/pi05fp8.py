@@ -200,10 +200,11 @@ def kv8_read(k8, k_scales, v8, v_scales, start=None, T=None, count=None, slots=N
     return k, v
 
 
-def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False, scale=None, out=None):
+def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False, scale=None, out=None, count=None):
     """pi05_kv8_attention: attention of q (bf16 [batch][T][heads][head_dim], samples and tokens may be strided) over the
-    first lens[b] positions of slot slots[b]; causal: token t sees lens[b] - T + t + 1 of them.  scale defaults to
-    head_dim^-0.5.  Returns bf16 [batch][T][heads][head_dim]."""
+    first lens[b] positions of slot slots[b]; causal: token t sees lens[b] - n + t + 1 of them, n = count[b] (T without counts).
+    Rows t >= n keep what `out` held (0 in a new tensor).  scale defaults to head_dim^-0.5.  Returns bf16 [batch][T][heads]
+    [head_dim]."""
     dev = q.get_device()
     (n, cap, kvh, d), at = _cache("kv8_attention", dev, k8, k_scales, v8, v_scales)
     shape = q.shape
@@ -212,7 +213,7 @@ def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False,
     batch, T, heads, _ = shape
     qb, qt = _strides("kv8_attention", q, shape)
     if out is None:
-        out = _empty(shape, dtype=BF, device=q.device)
+        out = (_empty if count is None else torch.zeros)(shape, dtype=BF, device=q.device)
         ob, ot = T * heads * d, heads * d
     else:
         if out.dtype != BF or out.shape != shape or out.get_device() != dev:
@@ -221,12 +222,13 @@ def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False,
     if lens is None:
         _bad("kv8_attention: lens is required")
     lens, slots = _index(lens, batch, dev, "kv8_attention: lens"), _index(slots, batch, dev, "kv8_attention: slots")
+    count = _index(count, batch, dev, "kv8_attention: count")
     need = lib.pi05_kv8_attention_workspace(batch, T, heads, kvh, d, cap)
     if need > 0:
         ws = _empty(need, dtype=U8, device=q.device)
         ws_at = ws.data_ptr()
     else:
         need = ws_at = 0
-    _call(lib.pi05_kv8_attention, dev, batch, T, heads, kvh, d, q.data_ptr(), qb, qt, n, cap, *at, lens, slots, 1 if causal else 0,
+    _call(lib.pi05_kv8_attention, dev, batch, T, heads, kvh, d, q.data_ptr(), qb, qt, n, cap, *at, lens, count, slots, 1 if causal else 0,
           d**-0.5 if scale is None else scale, out.data_ptr(), ob, ot, ws_at, need)
     return out

@@ -155,7 +155,7 @@ def _load():
         f.argtypes = [i32, i32, i32, i32, vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp] + tail
     L.pi05_kv8_attention_workspace.argtypes = [i32] * 6
     L.pi05_kv8_attention_workspace.restype = i64
-    L.pi05_kv8_attention.argtypes = [i32, i32, i32, i32, i32, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, i32,
+    L.pi05_kv8_attention.argtypes = [i32, i32, i32, i32, i32, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, i32,
                                      ctypes.c_float, vp, i64, i64, vp, i64] + tail
     L.pi05_lora_default_config.argtypes = [P(LoraConfig)]
     L.pi05_lora_default_config.restype = None

@@ -308,8 +308,8 @@ PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
  *   slot and position the later sample's row is kept.
  * pi05_kv8_read: the reverse; rows that are passed over stay as they were in k and v.
  * pi05_kv8_attention: out[b][t][h] = sum_j p_j V_j, p = softmax over j < lens[b] (clamped to [0, capacity]) of
- *   scale * q[b][t][h] . K_j; causal != 0: token t sees j < lens[b] - T + t + 1 (the last token sees all, as after a write of
- *   the T tokens).  A row that sees nothing gives 0; one that sees a NaN row of the cache, or whose query holds a NaN or an
+ *   scale * q[b][t][h] . K_j for the tokens t < n, n = count[b] (count NULL: T; clamped to [0, T]); rows from n on are left as they
+ *   were in out.  causal != 0: token t sees j < lens[b] - n + t + 1 (the last one sees all, as after a write of the n tokens).  A row that sees nothing gives 0; one that sees a NaN row of the cache, or whose query holds a NaN or an
  *   infinity, gives NaN.  heads is a multiple of kv_heads; query head h reads K/V head
  *   h / (heads / kv_heads).  q and out bf16, token t of sample b at b * sample stride + t * token stride elements, heads
  *   contiguous, 16-byte aligned.  workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
@@ -326,7 +326,7 @@ PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int heads, int k
 PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_heads, int head_dim, const void* q,
                                 int64_t q_sample_stride, int64_t q_token_stride, int n_slots, int capacity, const void* k8,
                                 const uint8_t* k_scales, const void* v8, const uint8_t* v_scales, const int32_t* lens,
-                                const int32_t* slots, int causal, float scale, void* out, int64_t out_sample_stride,
+                                const int32_t* count, const int32_t* slots, int causal, float scale, void* out, int64_t out_sample_stride,
                                 int64_t out_token_stride, void* workspace, int64_t workspace_bytes, void* stream, char* err,
                                 size_t err_len);
 

@@ -37,7 +37,7 @@ def rows_args(**kw):
 
 def attention_args(**kw):
     a = dict(batch=2, T=1, heads=8, kvh=2, hd=128, q=A, qb=1024, qt=1024, n_slots=4, capacity=16, k8=A, ks=A, v8=A, vs=A, lens=A,
-             slots=A, causal=0, scale=1.0, out=A, ob=1024, ot=1024, ws=A, ws_bytes=1 << 40)
+             count=A, slots=A, causal=0, scale=1.0, out=A, ob=1024, ot=1024, ws=A, ws_bytes=1 << 40)
     a.update(kw)
     return list(a.values())
 

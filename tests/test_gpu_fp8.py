@@ -529,6 +529,29 @@ def test_attention_query_with_nan_or_infinity(pn, T, hd):
     assert torch.equal(got[~isbad], want[~isbad]) and (got[~sees] == 0).all() and isbad.any()
 
 
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 1, 256), (8, 2, 64), (6, 2, 128)])
+@pytest.mark.parametrize("T,cap", [(3, 200), (50, 300), (150, 260), (40, 30000)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_a_padded_batch(pn, heads, kvh, hd, T, cap, causal):
+    """samples with fewer query tokens than T: their tokens give what they give alone, rows behind stay as they were"""
+    g = gen(34)
+    cache = filled(pn, g, 5, cap, kvh, hd)
+    q = randn(g, 5, T, heads, hd, dtype=BF)
+    q[:, T // 2 + 1 :, 0] = math.nan  # in padding too
+    counts, lens = [T, T // 2 + 1, 0, 1, T + 7], [cap, cap - 5, 100, 1, T // 2]
+    q[0] = q[4] = randn(g, T, heads, hd, dtype=BF)
+    out = torch.full_like(q, 3)
+    got = pn.kv8_attention(q, *cache, lens=i32(*lens), count=i32(*counts), causal=causal, out=out)
+    assert got is out
+    for b, n in enumerate(counts):
+        n = min(n, T)
+        assert (out[b, n:] == 3).all()
+        if n:
+            alone = check_attention(pn, q[b : b + 1, :n].contiguous(), cache, i32(lens[b]), slots=i32(b), causal=causal)
+            assert ((out[b, :n].float() - alone[0].float()).abs() <= 2.0**-7 * alone[0].float().abs() + 2.0**-8).all()
+    assert (pn.kv8_attention(q, *cache, lens=i32(*lens), count=i32(*counts), causal=causal)[2] == 0).all()
+
+
 @pytest.mark.parametrize("T", [1, 60])
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1.0])
 def test_attention_other_scales(pn, T, scale):
