@@ -208,129 +208,129 @@ __global__ void __launch_bounds__(512, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp < 4) {
-  regs_dec<C::REG_ROLE>();
-  if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < n && !flags[0]; ++i) {
-        const int s = i % C::NK;
-        const uint32_t ph = (uint32_t)(i / C::NK) & 1u;
-        const int key0 = (j0 + i) * C::KT;
-        if (!mbar_wait(&k_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
-          flags[0] = 1;
-          break;
-        }
-        mbar_arrive_expect_tx(&k_full[s], C::TILE8);
-        for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * 128, &tk, &k_full[s], c * 128, kvh, key0, slot);
-        if (!mbar_wait(&v_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
-          flags[0] = 1;
-          mbar_wait(&k_full[s], ph, status, P5_ERR_WAIT_ATTN);
-          break;
-        }
-        mbar_arrive_expect_tx(&v_full[s], C::TILE8);
-        for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * 128, &tv, &v_full[s], c * 128, kvh, key0, slot);
-        issued = i + 1;
-      }
-      fp8_drain(k_full, C::NK, issued, flags, status);
-      fp8_drain(v_full, C::NK, issued, flags, status);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::KT >> 3) << 17) | (8u << 24);
-    constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // fp16, B MN-major
-    const uint32_t base = smem_u32(smem);
-    bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
-    // S runs two tiles ahead of P V: its buffer is free as soon as the softmax has read it, long before P is there
-    for (int i = 0; i < n + 2 && ok; ++i) {
-      if (i < n) {
-        const int s = i % C::NK, sb = i & 1;
-        ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
-             (i < C::NS || mbar_wait_warp(&s_empty[(i - C::NS) & 1], (uint32_t)((i - C::NS) >> 1) & 1u, status, P5_ERR_WAIT_ATTN));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t ka = base + C::K_OFF + s * C::TILE8;
-        const uint32_t d = tmem + (uint32_t)(C::S_COL + sb % C::NS * C::KT);
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int kk = 0; kk < HD / 32; ++kk)
-            tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
-                         sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
-        tc_commit_warp(&k_empty[s]);
-        tc_commit_warp(&s_full[sb]);
-      }
-      if (i >= 2) {
-        const int j = i - 2, pb = j & 1;
-        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-        ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t va = base + C::W_OFF + pb * C::TILE16;
-#pragma unroll
-        for (int kk = 0; kk < C::KT / 16; ++kk)
-          tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
-                             sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
-        tc_commit_warp(&w_empty[pb]);
-        tc_commit_warp(&p_empty[pb]);
-      }
-    }
-    if (!ok) flags[0] = 1;
-    tc_commit_warp(o_full);
-  } else if (warp == 3) {
-    // ---- scales: two keys a lane, loaded a tile ahead
-    const long c0 = (long)slot * a.capacity * a.kv_heads + kvh;
-    int kb[2], vb[2];
-    auto load = [&](int i) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int key = (j0 + i) * C::KT + 2 * lane + q;
-        const bool in = i < n && key < top;
-        kb[q] = in ? (int)a.ks[c0 + (long)key * a.kv_heads] : 127;
-        vb[q] = in ? (int)a.vs[c0 + (long)key * a.kv_heads] : -1;  // no key
-      }
-    };
-    int eb = -1000;
-    load(0);
-    for (int i = 0; i < n; ++i) {
-      const int s = i % C::NSC;
-      float kf[2];
-      uint32_t vf[2];
-      int ev[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
-        ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
-      }
-      load(i + 1);
-      const int em = __reduce_max_sync(0xffffffffu, max(ev[0], ev[1]));
-      float rescale = 1.f;
-      if (em > eb + 7) {
-        if (i > 0) rescale = exp2_int(eb - em);  // 0 where there was no exponent yet: O is 0
-        eb = em;
-      }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {  // 2^(ev - eb) <= 2^7 in fp16, for two dims at a time
-        const int e = ev[q] - eb;
-        vf[q] = (e < -24 ? 0u : (e < -14 ? 1u << (e + 24) : (uint32_t)(e + 15) << 10)) * 0x10001u;
-      }
-      bool ok = !flags[0] && mbar_wait(&sc_empty[s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
-      if (!__all_sync(0xffffffffu, ok)) {
-        flags[0] = 1;
-        break;
-      }
-      float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
-      *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
-      *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
+    regs_dec<C::REG_ROLE>();
+    if (warp == 0) {
       if (lane == 0) {
-        sc[2 * C::KT] = rescale;
-        flags[1] = eb;
+        int issued = 0;
+        for (int i = 0; i < n && !flags[0]; ++i) {
+          const int s = i % C::NK;
+          const uint32_t ph = (uint32_t)(i / C::NK) & 1u;
+          const int key0 = (j0 + i) * C::KT;
+          if (!mbar_wait(&k_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+            flags[0] = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&k_full[s], C::TILE8);
+          for (int c = 0; c < C::ATOMS; ++c)
+            tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * 128, &tk, &k_full[s], c * 128, kvh, key0, slot);
+          if (!mbar_wait(&v_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+            flags[0] = 1;
+            mbar_wait(&k_full[s], ph, status, P5_ERR_WAIT_ATTN);
+            break;
+          }
+          mbar_arrive_expect_tx(&v_full[s], C::TILE8);
+          for (int c = 0; c < C::ATOMS; ++c)
+            tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * 128, &tv, &v_full[s], c * 128, kvh, key0, slot);
+          issued = i + 1;
+        }
+        fp8_drain(k_full, C::NK, issued, flags, status);
+        fp8_drain(v_full, C::NK, issued, flags, status);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sc_full[s]);
+    } else if (warp == 1) {
+      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::KT >> 3) << 17) | (8u << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // fp16, B MN-major
+      const uint32_t base = smem_u32(smem);
+      bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
+      // S runs two tiles ahead of P V: its buffer is free as soon as the softmax has read it, long before P is there
+      for (int i = 0; i < n + 2 && ok; ++i) {
+        if (i < n) {
+          const int s = i % C::NK, sb = i & 1;
+          ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+               (i < C::NS || mbar_wait_warp(&s_empty[(i - C::NS) & 1], (uint32_t)((i - C::NS) >> 1) & 1u, status, P5_ERR_WAIT_ATTN));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ka = base + C::K_OFF + s * C::TILE8;
+          const uint32_t d = tmem + (uint32_t)(C::S_COL + sb % C::NS * C::KT);
+  #pragma unroll
+          for (int half = 0; half < 2; ++half)
+  #pragma unroll
+            for (int kk = 0; kk < HD / 32; ++kk)
+              tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
+                           sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
+          tc_commit_warp(&k_empty[s]);
+          tc_commit_warp(&s_full[sb]);
+        }
+        if (i >= 2) {
+          const int j = i - 2, pb = j & 1;
+          const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+          ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = base + C::W_OFF + pb * C::TILE16;
+  #pragma unroll
+          for (int kk = 0; kk < C::KT / 16; ++kk)
+            tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
+                               sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
+          tc_commit_warp(&w_empty[pb]);
+          tc_commit_warp(&p_empty[pb]);
+        }
+      }
+      if (!ok) flags[0] = 1;
+      tc_commit_warp(o_full);
+    } else if (warp == 3) {
+      // ---- scales: two keys a lane, loaded a tile ahead
+      const long c0 = (long)slot * a.capacity * a.kv_heads + kvh;
+      int kb[2], vb[2];
+      auto load = [&](int i) {
+  #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int key = (j0 + i) * C::KT + 2 * lane + q;
+          const bool in = i < n && key < top;
+          kb[q] = in ? (int)a.ks[c0 + (long)key * a.kv_heads] : 127;
+          vb[q] = in ? (int)a.vs[c0 + (long)key * a.kv_heads] : -1;  // no key
+        }
+      };
+      int eb = -1000;
+      load(0);
+      for (int i = 0; i < n; ++i) {
+        const int s = i % C::NSC;
+        float kf[2];
+        uint32_t vf[2];
+        int ev[2];
+  #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
+          ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
+        }
+        load(i + 1);
+        const int em = __reduce_max_sync(0xffffffffu, max(ev[0], ev[1]));
+        float rescale = 1.f;
+        if (em > eb + 7) {
+          if (i > 0) rescale = exp2_int(eb - em);  // 0 where there was no exponent yet: O is 0
+          eb = em;
+        }
+  #pragma unroll
+        for (int q = 0; q < 2; ++q) {  // 2^(ev - eb) <= 2^7 in fp16, for two dims at a time
+          const int e = ev[q] - eb;
+          vf[q] = (e < -24 ? 0u : (e < -14 ? 1u << (e + 24) : (uint32_t)(e + 15) << 10)) * 0x10001u;
+        }
+        bool ok = !flags[0] && mbar_wait(&sc_empty[s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+        if (!__all_sync(0xffffffffu, ok)) {
+          flags[0] = 1;
+          break;
+        }
+        float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
+        *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
+        *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
+        if (lane == 0) {
+          sc[2 * C::KT] = rescale;
+          flags[1] = eb;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_full[s]);
+      }
     }
-  }
   } else if (warp >= 12) {
     regs_dec<C::REG_V>();
     // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
@@ -402,12 +402,12 @@ __global__ void __launch_bounds__(512, 1)
       mb = max(__float_as_uint(exch[r]), __float_as_uint(exch[128 + r]));
       const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN, unless it sees no key
       const int byte = bad ? 127 : fp8_scale_byte(__uint_as_float(mb));
-      // rf > 0, so that a masked logit of -inf stays one: the sign of the softmax scale goes into Q, and a scale of 0 makes
-      // Q zero
+      // rf > 0, so that a masked logit of -inf stays one: the sign of the softmax scale goes into Q, a scale of 0 makes Q zero,
+      // and a factor below the float range (a query of zeros, a tiny scale) is the smallest normal one
       const float sign = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
       const float up = bad ? 0.f : sign * fp8_scale_inverse(byte);
       const float2 up2 = make_float2(up, up);
-      rf = bad && lim > 0 ? NAN : (sign == 0.f ? 1.f : fp8_scale_value(byte) * fabsf(a.scale_log2));
+      rf = bad && lim > 0 ? NAN : (sign == 0.f ? 1.f : fmaxf(fp8_scale_value(byte) * fabsf(a.scale_log2), 1.17549435e-38f));
       constexpr int NC = HD / 8;  // columns of this half: four codes each
 #pragma unroll 1
       for (int i = 0; i < NC; i += 16) {

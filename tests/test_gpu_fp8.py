@@ -553,11 +553,14 @@ def test_attention_of_a_padded_batch(pn, heads, kvh, hd, T, cap, causal):
 
 
 @pytest.mark.parametrize("T", [1, 60])
-@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 1e-12, -1e-30])
 def test_attention_other_scales(pn, T, scale):
     g = gen(28)
     cache = filled(pn, g, 2, 150, 1, 256)
-    check_attention(pn, randn(g, 2, T, 8, 256, dtype=BF) * 0.3, cache, i32(150, 70), scale=scale, causal=True)
+    q = randn(g, 2, T, 8, 256, dtype=BF) * 0.3
+    q[:, :, 3] = 0
+    q[:, :, 4] *= 2.0**-120
+    check_attention(pn, q, cache, i32(150, 70), scale=scale, causal=True)
 
 
 def test_attention_one_query_for_all_samples(pn):
