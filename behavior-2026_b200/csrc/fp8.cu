@@ -286,7 +286,7 @@ int setup(char* err, size_t err_len, int* sms) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2 || !linear_attributes<FP8_STORE>() ||
         !linear_attributes<FP8_GELU>() || !linear_attributes<FP8_RESID>() || !linear_attributes<FP8_GATED>() ||
         !linear_attributes<FP8_GEGLU>() || !linear_attributes<FP8_F32>() ||
-        !attention_attributes<128>() || !attention_attributes<256>() ||
+        !attention_attributes<64>() || !attention_attributes<128>() || !attention_attributes<256>() ||
         !set_smem((const void*)kv8_attn_rows_kernel<64>, Kv8RowsCfg<64>::SMEM) ||
         !set_smem((const void*)kv8_attn_rows_kernel<128>, Kv8RowsCfg<128>::SMEM) ||
         !set_smem((const void*)kv8_attn_rows_kernel<256>, Kv8RowsCfg<256>::SMEM))
@@ -416,17 +416,18 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
   {  // a step: 32 keys of one of four warps
     const double tiles = pairs * ceil(rows / 8), steps = ceil(capacity / 128.0);
     const double places = (double)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
-    const double step = head_dim == 256 ? 1.8 : (head_dim == 128 ? 1.0 : 0.7);
+    const double step = head_dim == 256 ? 1.8 : (head_dim == 128 ? 1.0 : 0.9);
     for (int s = 1; s <= 256 && (s == 1 || s <= steps); s *= 2) {
       const double cost = ceil(tiles * s / places) * (6 + ceil(steps / s) * step) + (s > 8 ? 3 : 0);
       if (cost < best_cost) best_cost = cost, best = {false, s, s < 8 ? s : 8};
       if (tiles * s > 2 * places) break;
     }
   }
-  if (head_dim >= 128) {  // a step: 64 keys
-    const double tiles = pairs * ceil(rows / 128), steps = ceil(capacity / 64.0), step = head_dim == 256 ? 0.9 : 0.65;
+  {  // a step: 64 keys
+    const double tiles = pairs * ceil(rows / 128), steps = ceil(capacity / 64.0);
+    const double fixed = head_dim == 256 ? 10 : (head_dim == 128 ? 8 : 6), step = head_dim == 256 ? 0.9 : 0.65;
     for (int s = 1; s <= 64 && (s == 1 || 2 * s <= steps); s += 1 + s / 3) {
-      const double cost = ceil(tiles * s / num_sms()) * (10 + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
+      const double cost = ceil(tiles * s / num_sms()) * (fixed + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
       if (cost < best_cost) best_cost = cost, best = {true, s, 1};
       if (tiles * s > 2 * num_sms()) break;
     }
@@ -434,15 +435,16 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
   return best;
 }
 
-// [slots][capacity][kv_heads][head_dim] codes in boxes of 64 positions x 128 bytes of one head
+// [slots][capacity][kv_heads][head_dim] codes in boxes of 64 positions x 128 (64) bytes of one head, swizzled as wide
 bool cache_map(CUtensorMap* m, const void* base, const Kv8Args& a, int head_dim) {
   const cuuint64_t head = head_dim, pos = head * a.kv_heads;
   cuuint64_t dims[4] = {head, (cuuint64_t)a.kv_heads, (cuuint64_t)a.capacity, (cuuint64_t)a.n_slots};
   cuuint64_t strides[3] = {head, pos, pos * a.capacity};
-  cuuint32_t box[4] = {128, 1, 64, 1};
+  cuuint32_t box[4] = {head_dim < 128 ? 64u : 128u, 1, 64, 1};
   cuuint32_t es[4] = {1, 1, 1, 1};
   return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, head_dim < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -667,7 +669,9 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
   if (rc != PI05_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (plan.tc)
-    return head_dim == 128 ? attention_tc<128>(a, batch, st, err, err_len) : attention_tc<256>(a, batch, st, err, err_len);
+    return head_dim == 64    ? attention_tc<64>(a, batch, st, err, err_len)
+           : head_dim == 128 ? attention_tc<128>(a, batch, st, err, err_len)
+                             : attention_tc<256>(a, batch, st, err, err_len);
   if (head_dim == 64) return attention<64>(a, batch, plan.cluster, st, err, err_len);
   if (head_dim == 128) return attention<128>(a, batch, plan.cluster, st, err, err_len);
   return attention<256>(a, batch, plan.cluster, st, err, err_len);

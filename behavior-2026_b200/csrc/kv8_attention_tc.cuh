@@ -1,5 +1,5 @@
 // kv8_attention_tc.cuh — attention over the 8-bit K/V cache for many query rows, on the 5th-generation tensor cores
-// (head_dim 128 and 256; the mathematics and the arguments are kv8_attention.cuh's).
+// (the mathematics and the arguments are kv8_attention.cuh's).
 //
 // A CTA owns 128 folded query rows (r = t * G + g) of one (sample, K/V head) and one key split, and walks its keys in
 // tiles of 64:
@@ -32,7 +32,8 @@ namespace p5 {
 template <int HD>
 struct Kv8TcCfg {
   static constexpr int ROWS = 128, KT = 64;
-  static constexpr int ATOMS = HD / 128;           // 128-byte blocks of a key row
+  static constexpr int ROWB = HD < 128 ? HD : 128;  // bytes of a key row in one swizzled block
+  static constexpr int ATOMS = HD / ROWB;           // such blocks
   static constexpr int TILE8 = KT * HD;            // codes of a K or V tile
   static constexpr int TILE16 = KT * HD * 2;       // a widened V tile
   static constexpr int NK = HD == 256 ? 3 : 4;     // K and V code rings
@@ -74,6 +75,15 @@ __device__ __forceinline__ void tc_mma_f16_ta_warp(uint32_t d, uint32_t a_tmem, 
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// descriptor of a K-major tile of 64-byte rows written by TMA with the 64-byte swizzle: 8-row groups 512 bytes apart
+__device__ __forceinline__ uint64_t sw64_kmajor_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+__device__ __forceinline__ void tmem_st_n(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+__device__ __forceinline__ void tmem_st_n(uint32_t taddr, const uint32_t (&r)[8]) {
+  tmem_st4(taddr, r[0], r[1], r[2], r[3]);
+  tmem_st4(taddr + 4, r[4], r[5], r[6], r[7]);
 }
 // Each warpgroup sets its share of the block's registers once.
 template <int N>
@@ -222,7 +232,7 @@ __global__ void __launch_bounds__(512, 1)
           }
           mbar_arrive_expect_tx(&k_full[s], C::TILE8);
           for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * 128, &tk, &k_full[s], c * 128, kvh, key0, slot);
+            tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tk, &k_full[s], c * C::ROWB, kvh, key0, slot);
           if (!mbar_wait(&v_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
             flags[0] = 1;
             mbar_wait(&k_full[s], ph, status, P5_ERR_WAIT_ATTN);
@@ -230,7 +240,7 @@ __global__ void __launch_bounds__(512, 1)
           }
           mbar_arrive_expect_tx(&v_full[s], C::TILE8);
           for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * 128, &tv, &v_full[s], c * 128, kvh, key0, slot);
+            tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tv, &v_full[s], c * C::ROWB, kvh, key0, slot);
           issued = i + 1;
         }
         fp8_drain(k_full, C::NK, issued, flags, status);
@@ -257,7 +267,7 @@ __global__ void __launch_bounds__(512, 1)
   #pragma unroll
             for (int kk = 0; kk < HD / 32; ++kk)
               tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
-                           sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
+                           HD == 64 ? sw64_kmajor_desc(ka + kk * 32) : sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
           tc_commit_warp(&k_empty[s]);
           tc_commit_warp(&s_full[sb]);
         }
@@ -358,7 +368,8 @@ __global__ void __launch_bounds__(512, 1)
         const int group = rest % (HD / 64), pair = rest / (HD / 64);  // 64-dim box, pair of rows of an 8-row group
         const int row = (pair >> 2) * 8 + ((pair & 3) ^ (hi ? 5 : 0));
         const int piece = group * 4 + j4;  // 16-byte piece of the key's codes
-        uint4 u = *reinterpret_cast<const uint4*>(src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+        uint4 u = *reinterpret_cast<const uint4*>(HD == 64 ? src + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)
+                                                           : src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
         if (row >= valid) u = make_uint4(0, 0, 0, 0);
         const uint32_t f = vf[row];
         auto two = [&](uint32_t c) {
@@ -409,11 +420,12 @@ __global__ void __launch_bounds__(512, 1)
       const float2 up2 = make_float2(up, up);
       rf = bad && lim > 0 ? NAN : (sign == 0.f ? 1.f : fmaxf(fp8_scale_value(byte) * fabsf(a.scale_log2), 1.17549435e-38f));
       constexpr int NC = HD / 8;  // columns of this half: four codes each
+      constexpr int CH = NC < 16 ? NC : 16;
 #pragma unroll 1
-      for (int i = 0; i < NC; i += 16) {
-        uint32_t hi[16], lo[16];
+      for (int i = 0; i < NC; i += CH) {
+        uint32_t hi[CH], lo[CH];
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
+        for (int k = 0; k < CH; k += 2) {
           const uint4 u = src[(i + k) / 2];
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -429,8 +441,8 @@ __global__ void __launch_bounds__(512, 1)
           }
         }
         __syncwarp();
-        tmem_st16(t_lane + (uint32_t)(C::Q_COL + g * NC + i), hi);
-        tmem_st16(t_lane + (uint32_t)(C::Q_COL + HD / 4 + g * NC + i), lo);
+        tmem_st_n(t_lane + (uint32_t)(C::Q_COL + g * NC + i), hi);
+        tmem_st_n(t_lane + (uint32_t)(C::Q_COL + HD / 4 + g * NC + i), lo);
       }
       tmem_wait_st();
       tc_fence_before();
