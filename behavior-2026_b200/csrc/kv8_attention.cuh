@@ -11,7 +11,7 @@
 //
 // One new token reads the whole cache once for a handful of products, so what counts is bytes in flight: each warp
 // keeps a ring of its own of STAGES steps (cp.async, no barrier between warps), 48 to 192 KB an SM.  Measured, 16 samples of 32
-// heads on 8 of 128: 46 us and 5.8 TB/s at 8,192 keys each, 73 us and 4.7 TB/s at 4,000 to 16,387 (the longest sample decides);
+// heads on 8 of 128: 46 us and 5.8 TB/s at 8,192 keys each, 70-73 us and 4.7 TB/s at 4,000 to 16,387 (the longest sample decides);
 // one sample of 1,018 keys 10 us, its chain of latencies.
 //
 // Everything is computed transposed, keys and head dims on the 16-row side of mma.m16n8k16 and query rows on

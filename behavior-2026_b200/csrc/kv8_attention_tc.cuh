@@ -15,8 +15,8 @@
 //                 and scaled by its row's power of two relative to a running exponent eb by four converter warps (exact;
 //                 keys that no row sees become zeros, whatever the cache holds there).  An e4m3 P would need three
 //                 operands to keep the small weights of a long cache.
-// Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 47.6 us (530 TFLOP/s); 8 x 968 x 968 95 us (649); 2 x 2,049
-// tokens, 16 heads on 4 of 128, up to 8,192 keys 293 us (773).  No unit is full (at HD 128 tensor pipes 43 %, exponentials
+// Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 48.5 us (550 TFLOP/s); 8 x 968 x 968 95 us (649); 2 x 2,049
+// tokens, causal over 8,192 keys, 16 heads on 4 of 128 310 us (777) and on 2 of 64 268 us (448).  No unit is full (at HD 128 tensor pipes 43 %, exponentials
 // 43 %, issue 54 %, shared memory 52 %): a tile waits on the chain of its softmax, about 2,400 clocks for two tiles in
 // turn, and at HD 256 a short call on the 10 us that a CTA takes to load its queries and to store.  Three warpgroups were
 // slower than two (349 against 328 us then): they leave a thread 128 registers.
