@@ -23,11 +23,15 @@
 // registers (exact).  P^T goes from the accumulator layout to the operand layout by movmatrix.
 //
 // fp16 operands: a query row is scaled by a power of two so that its largest element is near 2^15 (elements
-// down to 2^-29 of it keep all 8 bits of a bf16); P carries the V row's scale relative to a running exponent
-// eb (p * 2^(ev - eb)), 11 bits of mantissa, against the 8 that bf16 would keep.  Logits, maxima, sums and O are fp32.
-// The running maximum moves only when a logit exceeds it by 2^8, and eb when a scale exceeds it by 2^7, so
-// p * 2^(ev - eb) stays within 2^15 and O is rarely rescaled.
+// down to 2^-29 of it keep all 8 bits of a bf16); P carries the V row's scale relative to an exponent eb of the warp
+// (p * 2^(ev - eb)).  Logits, maxima, sums and O are fp32.
+// The running maximum moves only when a logit exceeds it by 2^4, and eb only when a scale leaves eb .. eb + 11, so
+// p * 2^(ev - eb) stays within 2^15, a weight keeps 11 bits (or 2^-25 of the largest) whatever other keys' scales are, and O is
+// rarely rescaled.  A step whose scales span more than that (a key that a row does not see counts as well: its scale must
+// not push that row's weights below the range) takes V and P in bf16, P as two operands hi + lo (16 bits): any scale fits.
 #pragma once
+#include <type_traits>
+
 #include "fp8.cuh"
 
 namespace p5 {
@@ -62,6 +66,14 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// two fp16 -> two bf16 (exact for widened e4m3 codes: 4 bits)
+__device__ __forceinline__ uint32_t h2_to_bf2(uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack_bf2(f.x, f.y);
+}
+// Exponents of V scales that one accumulator holds: a term is at most 2^15 (weight) * 2^9 (code) * 2^(scale - unit), summed
+// over up to 2^31 keys, so scales up to 2^72 above the unit cannot pass the fp32 range.
+constexpr int KV8_E_SPAN = 72;
 // 2^n for any integer n (0 below 2^-127, 2^127 above)
 __device__ __forceinline__ float exp2_int(int n) {
   return n < -127 ? 0.f : __uint_as_float(n == -127 ? 0x400000u : (uint32_t)(min(n, 127) + 127) << 23);
@@ -197,7 +209,9 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
 
   float o[MT][4];
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-  int eb = -1000;  // exponent of the V scales that O is in units of
+  int eb = -1000;              // O is in units of 2^eb (-1000: no V scale yet, O is 0)
+  int e_top = -1000;           // the largest V exponent so far
+  constexpr int E_WINDOW = 11;  // fp16 steps: eb .. eb + E_WINDOW
 #pragma unroll
   for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
@@ -233,17 +247,13 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
         }
       // ---- logits in base 2; a cached NaN row (scale byte 255) makes the rows that see it NaN
       const int key0 = step * C::KEYS + g;
-      int ev[2][2];
-      bool grow = false;
-      int em = -1000;
+      const int kb = kq[st], vb = vq[st];  // of key `lane`
+      const float kf1 = (kb == 255 || vb == 255) ? NAN : fp8_scale_value(kb);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int kb = __shfl_sync(0xffffffffu, kq[st], 16 * n + 8 * q + g), vb = __shfl_sync(0xffffffffu, vq[st], 16 * n + 8 * q + g);
-          const float kf = (kb == 255 || vb == 255) ? NAN : fp8_scale_value(kb);
-          ev[n][q] = vb == 255 ? -1000 : vb - 127;
-          em = max(em, ev[n][q]);
+          const float kf = __shfl_sync(0xffffffffu, kf1, 16 * n + 8 * q + g);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float x = (s[n][2 * q + j] + s2[n][2 * q + j]) * rf[j] * kf;
@@ -251,18 +261,26 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
           }
         }
       float mt[2];
+      // a scale outside the window; that of a row of zeros (byte 0: or below 2^-117) counts only where there is no window yet
+      bool grow = vb != 255 && (uint32_t)(vb - 127 - eb) > (uint32_t)E_WINDOW && (vb != 0 || eb == -1000);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mt[j] = fmaxf(fmaxf(s[0][j], s[0][2 + j]), fmaxf(s[1][j], s[1][2 + j]));
-        grow |= mt[j] > m_run[j] + 8.f;
+        grow |= mt[j] > m_run[j] + 4.f;
       }
-      grow |= em > eb + 7;
+      bool wide = false;  // this step's products in bf16
       if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) em = max(em, __shfl_xor_sync(0xffffffffu, em, d));
-        em = max(em, eb);
-        const float ealpha = exp2_int(eb - em);  // 0 at first, when O is 0 anyway
-        eb = em;
+        const int em = __reduce_max_sync(0xffffffffu, vb == 255 ? -1000 : vb - 127);
+        int en = __reduce_min_sync(0xffffffffu, vb == 255 || vb == 0 ? 1000 : vb - 127), to = eb;
+        if (em > eb + E_WINDOW || en < eb) {
+          en = min(en, em);
+          e_top = max(e_top, em);
+          to = max(min(en, em - 9), -127);  // a little room above
+          wide = em - en > E_WINDOW || e_top - to > KV8_E_SPAN;
+          if (wide) to = eb == -1000 ? max(en, em - KV8_E_SPAN) : max(eb, em - KV8_E_SPAN);
+        }
+        const float ealpha = exp2_int(eb - to);  // 0 at first, when O is 0 anyway
+        eb = to;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float m = mt[j];
@@ -280,51 +298,75 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
           }
         }
       }
-      // ---- P^T, each key's V scale folded in
-      uint32_t pf[2][2];
+      // ---- P^T, each key's V scale folded in, and O^T += V^T P^T: tile (i, j) holds dims 16 g + 2 j and + 1 of the 128-dim
+      // part i.  WIDE: in bf16, P as hi + lo.
+      auto product = [&](auto in_bf16) {
+        constexpr bool WIDE = decltype(in_bf16)::value;
+        const float vf1 = vb == 255 ? 0.f : __uint_as_float((uint32_t)max(vb - eb, 0) << 23);  // 2^(vb - 127 - eb), at most 2^KV8_E_SPAN
+        uint32_t pf[2][2], pl[2][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const float vf = exp2_int(ev[n][q] - eb);
-          float p[2];
+          for (int q = 0; q < 2; ++q) {
+            const float vf = __shfl_sync(0xffffffffu, vf1, 16 * n + 8 * q + g);
+            float p[2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            p[j] = ex2_approx(s[n][2 * q + j] - (m_run[j] == -INFINITY ? 0.f : m_run[j]));
-            l_run[j] += p[j];
-          }
-          const __half2 h = __floats2half2_rn(p[0] * vf, p[1] * vf);
-          pf[n][q] = movmatrix_b16(*reinterpret_cast<const uint32_t*>(&h));
-        }
-      // ---- O^T += V^T P^T: tile (i, j) holds dims 16 g + 2 j and + 1 of the 128-dim part i
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < VI; ++i) {
-          uint32_t w[4][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int key = 16 * n + 2 * c + (k & 1) + 8 * (k >> 1);
-            if (VB == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sv + kv8_v_at<HD>(key, 8 * i + g));
-              w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+            for (int j = 0; j < 2; ++j) {
+              p[j] = ex2_approx(s[n][2 * q + j] - (m_run[j] == -INFINITY ? 0.f : m_run[j]));
+              l_run[j] += p[j];
+              p[j] *= vf;
+            }
+            if constexpr (WIDE) {
+              const uint32_t hi = pack_bf2(p[0], p[1]);
+              const float2 f = unpack_bf2(hi);
+              pf[n][q] = movmatrix_b16(hi);
+              pl[n][q] = movmatrix_b16(pack_bf2(p[0] - f.x, p[1] - f.y));
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(sv + kv8_v_at<HD>(key, g >> 1) + (g & 1) * 8);
-              w[k][0] = u.x, w[k][1] = u.y;
+              const __half2 h = __floats2half2_rn(p[0], p[1]);
+              pf[n][q] = movmatrix_b16(*reinterpret_cast<const uint32_t*>(&h));
             }
           }
 #pragma unroll
-          for (int q = 0; q < VB / 4; ++q)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int hlf = 0; hlf < 2; ++hlf) {
-              // bytes (2 hlf, 2 hlf + 1) of the word of two keys, interleaved by key
-              const uint32_t lo = __byte_perm(w[0][q], w[1][q], hlf ? 0x7362 : 0x5140);
-              const uint32_t hi = __byte_perm(w[2][q], w[3][q], hlf ? 0x7362 : 0x5140);
-              const uint32_t af[4] = {fp8_to_h2((uint16_t)lo), fp8_to_h2((uint16_t)(lo >> 16)), fp8_to_h2((uint16_t)hi),
-                                      fp8_to_h2((uint16_t)(hi >> 16))};
-              mma_f16_16816(o[i * (VB / 2) + 2 * q + hlf], af, pf[n][0], pf[n][1]);
+          for (int i = 0; i < VI; ++i) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int key = 16 * n + 2 * c + (k & 1) + 8 * (k >> 1);
+              if (VB == 16) {
+                const uint4 u = *reinterpret_cast<const uint4*>(sv + kv8_v_at<HD>(key, 8 * i + g));
+                w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+              } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(sv + kv8_v_at<HD>(key, g >> 1) + (g & 1) * 8);
+                w[k][0] = u.x, w[k][1] = u.y;
+              }
             }
-        }
+#pragma unroll
+            for (int q = 0; q < VB / 4; ++q)
+#pragma unroll
+              for (int hlf = 0; hlf < 2; ++hlf) {
+                // bytes (2 hlf, 2 hlf + 1) of the word of two keys, interleaved by key
+                const uint32_t lo = __byte_perm(w[0][q], w[1][q], hlf ? 0x7362 : 0x5140);
+                const uint32_t hi = __byte_perm(w[2][q], w[3][q], hlf ? 0x7362 : 0x5140);
+                uint32_t af[4] = {fp8_to_h2((uint16_t)lo), fp8_to_h2((uint16_t)(lo >> 16)), fp8_to_h2((uint16_t)hi),
+                                  fp8_to_h2((uint16_t)(hi >> 16))};
+                float(&acc)[4] = o[i * (VB / 2) + 2 * q + hlf];
+                if constexpr (WIDE) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) af[k] = h2_to_bf2(af[k]);
+                  mma_bf16_16816(acc, af, pf[n][0], pf[n][1]);
+                  mma_bf16_16816(acc, af, pl[n][0], pl[n][1]);
+                } else {
+                  mma_f16_16816(acc, af, pf[n][0], pf[n][1]);
+                }
+              }
+          }
+      };
+      if (wide)
+        product(std::true_type());
+      else
+        product(std::false_type());
       step += W;
     }
   }

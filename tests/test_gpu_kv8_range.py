@@ -1,0 +1,135 @@
+"""pi05_kv8_attention over caches whose rows differ widely in size, against 64 bits.
+
+The bound is a sum over the keys that a row sees: each weight is off by its logit's error (the fp32 sum of head_dim products,
+the base-2 exponent's rounding), 2^-22 of the exponential, the fp32 sums over the keys, and one rounding of the weight:
+fp16, 2^-11 of it or 2^-25 of the largest weight where it is subnormal.  A key that a row does not see, or whose weight is 0, adds
+nothing, whatever its size."""
+import math
+
+import pytest
+import torch
+from launched import assert_launches
+from test_gpu_fp8 import BF, decode, gen, i32, new_cache, randn
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16 = 2.0**-11, 2.0**-8  # half a step of a weight
+
+
+@pytest.fixture(autouse=True)
+def _check_device(pn):
+    yield
+    pn.fp8_status()  # no bounded wait gave up
+
+
+def bounded(got, q, cache, lens, slots=None, causal=False, scale=None, weight=FP16, floor=2.0**-110):
+    """asserts got against the definition; returns nothing"""
+    B, T, H, hd = q.shape
+    N, cap, kvh, _ = cache[0].shape
+    scale = hd**-0.5 if scale is None else scale
+    for b in range(B):
+        sl = int(slots[b]) if slots is not None else b
+        n = min(max(int(lens[b]), 0), cap)
+        if n == 0:
+            assert (got[b] == 0).all()
+            continue
+        k, v = decode(cache[0][sl, :n], cache[1][sl, :n].long()), decode(cache[2][sl, :n], cache[3][sl, :n].long())
+        seen = torch.ones(T, n, dtype=torch.bool, device="cuda")
+        if causal:
+            seen = torch.arange(n, device="cuda")[None] < (n - T + 1 + torch.arange(T, device="cuda"))[:, None]
+        for h in range(H):
+            kh, vh, qh = k[:, h // (H // kvh)], v[:, h // (H // kvh)], q[b, :, h].double()
+            s = (qh @ kh.t() * scale).masked_fill(~seen, -math.inf)
+            mag = torch.where(seen, qh.abs() @ kh.abs().t() * abs(scale), 0).amax(-1, keepdim=True)
+            top = torch.where(seen, s.abs(), 0).amax(-1, keepdim=True)
+            p = torch.softmax(s, -1)
+            p[~seen.any(-1)] = 0
+            dl = mag * (hd + 8) * 2.0**-23 + top * 2.0**-22
+            dp = p * (2 * dl + 2.0**-22 + weight + (n + 16) * 2.0**-23) + p.clamp(max=2.0**-25)
+            ref, tol = p @ vh, dp @ vh.abs()
+            tol = tol + 2.0**-8 * (ref.abs() + tol) + floor
+            off = (got[b, :, h].double() - ref).abs()
+            worst = (off / tol).nan_to_num(nan=1e9).max().item()
+            assert worst <= 1, f"sample {b}, head {h}: {worst:.3g} of the tolerance"
+
+
+# (batch, T, heads, kv_heads, head_dim, capacity) that reach each kernel
+ROWS = [(1, 40, 8, 2, 128, 64), (2, 1, 8, 1, 256, 300), (3, 7, 6, 2, 64, 150)]
+ROWS_SPLIT = [(1, 1, 8, 1, 256, 20000), (1, 3, 8, 2, 64, 40000)]
+KERNELS = {"rows": "kv8_attn_rows_kernel", "tc": "kv8_attn_tc_kernel"}
+
+
+def run(pn, kernel, q, cache, lens, **kw):
+    call = lambda: pn.kv8_attention(q, *cache, lens=lens, **kw)  # noqa: E731
+    got = call()
+    assert_launches(call, *([KERNELS[kernel]] if isinstance(kernel, str) else kernel))
+    return got
+
+
+def written(pn, k, v):
+    B, n, kvh, hd = k.shape
+    cache = new_cache(B, n, kvh, hd)
+    pn.kv8_write(k.to(BF), v.to(BF), *cache)
+    return cache
+
+
+def one_large_hidden_value(pn, kernel, shape, large, hi=2.0**-8, floor=0.0):
+    """V rows of 1 and a last one that only the last token sees: all others give exactly the mean of ones"""
+    B, T, H, kvh, hd, n = shape
+    k = torch.zeros(B, n, kvh, hd, device="cuda")
+    v = torch.ones(B, n, kvh, hd, device="cuda")
+    v[:, n - 1] = large
+    q = torch.zeros(B, T, H, hd, device="cuda", dtype=BF)
+    got = run(pn, kernel, q, written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32), causal=True).float()
+    assert ((got[:, :-1] - 1).abs() <= hi).all()
+    last = (n - 1 + float(v[0, -1, 0, 0].to(BF).double())) / n
+    assert ((got[:, -1].double() - last).abs() <= 2.0**-4 * last).all()  # the value itself is rounded to e4m3
+
+
+def far_apart(pn, kernel, shape, causal, seed, spread, weight=FP16, floor=2.0**-110):
+    """every V row of its own size, 2^-spread to 2^spread; some rows of zeros"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(seed)
+    k = randn(g, B, n, kvh, hd)
+    v = randn(g, B, n, kvh, hd) * torch.exp2(torch.randint(-spread, spread + 1, (B, n, kvh, 1), device="cuda", generator=g).float())
+    v[:, 3::7] = 0
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache = written(pn, k, v)
+    lens = torch.arange(n, n - B, -1, device="cuda").int()
+    bounded(run(pn, kernel, q, cache, lens, causal=causal), q, cache, lens, causal=causal, weight=weight, floor=floor)
+
+
+@pytest.mark.parametrize("large", [2.0**9, 2.0**16, 2.0**30, 2.0**90, 3.3e38])
+@pytest.mark.parametrize("shape", [ROWS[0], (2, 5, 8, 1, 256, 300), (3, 9, 6, 2, 64, 150)])
+def test_rows_kernel_large_hidden_value(pn, shape, large):
+    one_large_hidden_value(pn, "rows", shape, large)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("spread", [4, 8, 40])
+@pytest.mark.parametrize("shape", ROWS + ROWS_SPLIT)
+def test_rows_kernel_values_far_apart(pn, shape, spread, causal):
+    far_apart(pn, "rows", shape, causal, 41, spread)
+
+
+def test_rows_kernel_values_growing_and_shrinking(pn):
+    """sizes that wander over 2^-60 .. 2^60 and back along the cache: the window of exponents has to follow both ways"""
+    g = gen(42)
+    B, T, H, kvh, hd, n = 1, 2, 8, 1, 128, 4000
+    e = 60 * torch.sin(torch.arange(n, device="cuda") / 150.0)
+    v = randn(g, B, n, kvh, hd) * torch.exp2(e)[None, :, None, None]
+    k = randn(g, B, n, kvh, hd)
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache = written(pn, k, v)
+    for lens in (i32(n), i32(471), i32(940)):
+        bounded(run(pn, "rows", q, cache, lens), q, cache, lens)
+
+
+def test_rows_kernel_tiny_values(pn):
+    """V rows next to the smallest exponent"""
+    g = gen(43)
+    v = randn(g, 1, 200, 1, 128) * 2.0**-115
+    k = randn(g, 1, 200, 1, 128)
+    q = randn(g, 1, 1, 8, 128, dtype=BF)
+    cache = written(pn, k, v)
+    bounded(run(pn, "rows", q, cache, i32(200)), q, cache, i32(200), floor=2.0**-126)
