@@ -12,15 +12,18 @@
 //                 of a row through shared memory: a tile's warp waits for its turn, raises the maximum if it must, and passes
 //                 the turn on before its exponentials.  Each keeps its own sum.
 //   O += P V      kind::f16, P in fp16 (11 bits; as 2^7 p, which keeps weights down to 2^-31 of the largest), V widened to fp16
-//                 and scaled by its row's power of two relative to a running exponent eb by four converter warps (exact;
-//                 keys that no row sees become zeros, whatever the cache holds there).  An e4m3 P would need three
-//                 operands to keep the small weights of a long cache.
+//                 and scaled by its row's power of two relative to an exponent eb by four converter warps (exact: eb follows the
+//                 tiles so that their scales lie within eb - 15 .. eb + 7; keys that no row sees become zeros, whatever the cache
+//                 holds there).  An e4m3 P would need three operands to keep the small weights of a long cache.
+//                 Where a tile's scales span more (a key that some rows do not see counts as well: it must not cost them
+//                 bits), the CTA goes through its keys again with V and P in bf16, into which any scale fits; V is exact,
+//                 weights keep 8 bits.  A choice of type for each tile made every call 2 to 7 % slower, in each form tried.
 // Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 48.5 us (550 TFLOP/s); 8 x 968 x 968 95 us (649); 2 x 2,049
 // tokens, causal over 8,192 keys, 16 heads on 4 of 128 310 us (777) and on 2 of 64 268 us (448).  No unit is full (at HD 128 tensor pipes 43 %, exponentials
 // 43 %, issue 54 %, shared memory 52 %): a tile waits on the chain of its softmax, about 2,400 clocks for two tiles in
 // turn, and at HD 256 a short call on the 10 us that a CTA takes to load its queries and to store.  Three warpgroups were
 // slower than two (349 against 328 us then): they leave a thread 128 registers.
-// The running maximum moves only when a tile exceeds it by 2^8 and the V exponent eb only when a scale exceeds it by 2^7;
+// The running maximum moves only when a tile exceeds it by 2^8 and the V exponent eb only when a scale leaves its window;
 // both rescale O through tcgen05.ld/st.  eb is the same for all rows and kept by the warp that loads the scales.
 //   warp 0 TMA, warp 1 MMA issue, warp 2 TMEM, warp 3 scales, warps 4-11 softmax, warps 12-15 V
 #pragma once
@@ -41,10 +44,11 @@ struct Kv8TcCfg {
   static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8;
   static constexpr int Q_BYTES = ROWS * (HD * 2 + 16);  // query rows on their way in, over the widened V
   static constexpr int SC_OFF = W_OFF + (2 * TILE16 > Q_BYTES ? 2 * TILE16 : (Q_BYTES + 127) / 128 * 128);
-  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64] (fp32), vf[64] (fp16, twice), rescale factor of O
+  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64] (fp32), vf[64] (fp16 or bf16, twice), rescale factor of O
   static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
   static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
-  static constexpr int SMEM = 1024 + BAR_OFF + 512;
+  static constexpr int BARS = 4 * NK + 2 * NSC + 21;  // barriers of a pass
+  static constexpr int SMEM = 1024 + BAR_OFF + 2 * BARS * 8 + 64;
   // Tensor memory: Q hi | lo, S, P[2], O.  P lies here because all of this competes for the shared memory; at HD 256 that
   // leaves room for one S buffer only (two, and P in shared memory: 64 chunks 49.7 us).
   static constexpr int NS = HD == 256 ? 1 : 2;
@@ -124,6 +128,7 @@ __global__ void __launch_bounds__(512, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  // barriers, those of a second pass over the keys C::BARS behind them
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [NK] codes landed
   uint64_t* k_empty = k_full + C::NK;                                // [NK] S product done
   uint64_t* v_full = k_empty + C::NK;                                // [NK]
@@ -137,10 +142,10 @@ __global__ void __launch_bounds__(512, 1)
   uint64_t* p_full = s_empty + 2;                                    // [2] (4 warps)
   uint64_t* p_empty = p_full + 2;                                    // [2] P V product done
   uint64_t* turn = p_empty + 2;                                      // [2][4] the other warpgroup's warp has passed the turn
-  uint64_t* q_full = turn + 8;                                       // Q in tensor memory (8 warps)
-  uint64_t* o_full = q_full + 1;                                     // every MMA complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
-  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort, [1] eb at the end
+  uint64_t* o_full = turn + 8;                                       // every MMA complete
+  uint64_t* q_full = k_full + 2 * C::BARS;                           // Q in tensor memory (8 warps)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort, [1] eb at the end, [2] go through the keys again
   float* exch = reinterpret_cast<float*>(smem + C::X_OFF);
   int* status = &g_fp8_status;
 
@@ -200,9 +205,9 @@ __global__ void __launch_bounds__(512, 1)
       mbar_init(&p_empty[i], 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
-    mbar_init(q_full, 8);
     mbar_init(o_full, 1);
-    flags[0] = 0;
+    mbar_init(q_full, 8);
+    flags[0] = flags[2] = 0;
     flags[1] = -1000;
     fence_barrier_init();
     tma_prefetch_desc(&tk);
@@ -217,83 +222,112 @@ __global__ void __launch_bounds__(512, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
+  // A role's pass over the keys, and a second one in bf16 where a tile needs it, on barriers of its own.  The softmax, the scales and the
+  // V warps have a copy of their code for each; one copy of the issuing loop runs twice (a second copy made head_dim 128 a third
+  // slower).  What the second pass costs the calls that do not need it: at head_dim 128 1.5 %, at 256 4 %.
+  auto met = [&]() -> bool {  // every thread; true: once more
+    tc_fence_before();
+    asm volatile("bar.sync 2, 512;" ::: "memory");
+    tc_fence_after();
+    return __builtin_expect(flags[2] && !flags[0], 0);
+  };
+  auto meet = [&]() -> bool {
+    if (__builtin_expect(!met(), 1)) return false;
+    asm volatile("bar.sync 2, 512;" ::: "memory");  // warp 2 has set the second pass' barriers up
+    return true;
+  };
+  auto passes = [&](auto role) {
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      role(pass);
+      if (pass || __builtin_expect(!meet(), 1)) break;
+    }
+  };
+
   if (warp < 4) {
     regs_dec<C::REG_ROLE>();
     if (warp == 0) {
-      if (lane == 0) {
-        int issued = 0;
-        for (int i = 0; i < n && !flags[0]; ++i) {
-          const int s = i % C::NK;
-          const uint32_t ph = (uint32_t)(i / C::NK) & 1u;
-          const int key0 = (j0 + i) * C::KT;
-          if (!mbar_wait(&k_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
-            flags[0] = 1;
-            break;
+      passes([&](int pass) {
+        const int of = pass * C::BARS;
+        if (lane == 0) {
+          int issued = 0;
+          for (int i = 0; i < n && !flags[0]; ++i) {
+            const int s = i % C::NK;
+            const uint32_t ph = (uint32_t)(i / C::NK) & 1u;
+            const int key0 = (j0 + i) * C::KT;
+            if (!mbar_wait(&k_empty[of + s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+              flags[0] = 1;
+              break;
+            }
+            mbar_arrive_expect_tx(&k_full[of + s], C::TILE8);
+            for (int c = 0; c < C::ATOMS; ++c)
+              tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tk, &k_full[of + s], c * C::ROWB, kvh, key0, slot);
+            if (!mbar_wait(&v_empty[of + s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
+              flags[0] = 1;
+              mbar_wait(&k_full[of + s], ph, status, P5_ERR_WAIT_ATTN);
+              break;
+            }
+            mbar_arrive_expect_tx(&v_full[of + s], C::TILE8);
+            for (int c = 0; c < C::ATOMS; ++c)
+              tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tv, &v_full[of + s], c * C::ROWB, kvh, key0, slot);
+            issued = i + 1;
           }
-          mbar_arrive_expect_tx(&k_full[s], C::TILE8);
-          for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_4d(smem + C::K_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tk, &k_full[s], c * C::ROWB, kvh, key0, slot);
-          if (!mbar_wait(&v_empty[s], ph ^ 1u, status, P5_ERR_WAIT_ATTN)) {
-            flags[0] = 1;
-            mbar_wait(&k_full[s], ph, status, P5_ERR_WAIT_ATTN);
-            break;
-          }
-          mbar_arrive_expect_tx(&v_full[s], C::TILE8);
-          for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_4d(smem + C::V_OFF + s * C::TILE8 + c * C::KT * C::ROWB, &tv, &v_full[s], c * C::ROWB, kvh, key0, slot);
-          issued = i + 1;
+          fp8_drain(k_full + of, C::NK, issued, flags, status);
+          fp8_drain(v_full + of, C::NK, issued, flags, status);
         }
-        fp8_drain(k_full, C::NK, issued, flags, status);
-        fp8_drain(v_full, C::NK, issued, flags, status);
-      }
-      __syncwarp();
+        __syncwarp();
+      });
     } else if (warp == 1) {
-      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::KT >> 3) << 17) | (8u << 24);
-      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // fp16, B MN-major
-      const uint32_t base = smem_u32(smem);
-      bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
-      // S runs two tiles ahead of P V: its buffer is free as soon as the softmax has read it, long before P is there
-      for (int i = 0; i < n + 2 && ok; ++i) {
-        if (i < n) {
-          const int s = i % C::NK, sb = i & 1;
-          ok = mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
-               (i < C::NS || mbar_wait_warp(&s_empty[(i - C::NS) & 1], (uint32_t)((i - C::NS) >> 1) & 1u, status, P5_ERR_WAIT_ATTN));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ka = base + C::K_OFF + s * C::TILE8;
-          const uint32_t d = tmem + (uint32_t)(C::S_COL + sb % C::NS * C::KT);
-  #pragma unroll
-          for (int half = 0; half < 2; ++half)
-  #pragma unroll
-            for (int kk = 0; kk < HD / 32; ++kk)
-              tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
-                           HD == 64 ? sw64_kmajor_desc(ka + kk * 32) : sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
-          tc_commit_warp(&k_empty[s]);
-          tc_commit_warp(&s_full[sb]);
+      passes([&](int pass) {
+        const int of = pass * C::BARS;
+        constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::KT >> 3) << 17) | (8u << 24);
+        // fp16 or bf16, B MN-major
+        const uint32_t idesc_o = (1u << 4) | (pass ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
+        const uint32_t base = smem_u32(smem);
+        bool ok = mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN);
+        // S runs two tiles ahead of P V: its buffer is free as soon as the softmax has read it, long before P is there
+        for (int i = 0; i < n + 2 && ok; ++i) {
+          if (i < n) {
+            const int s = i % C::NK, sb = i & 1;
+            ok = mbar_wait_warp(&k_full[of + s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                 (i < C::NS || mbar_wait_warp(&s_empty[of + ((i - C::NS) & 1)], (uint32_t)((i - C::NS) >> 1) & 1u, status, P5_ERR_WAIT_ATTN));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ka = base + C::K_OFF + s * C::TILE8;
+            const uint32_t d = tmem + (uint32_t)(C::S_COL + sb % C::NS * C::KT);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int kk = 0; kk < HD / 32; ++kk)
+                tc_mma_f8_ta(d, tmem + (uint32_t)(C::Q_COL + half * (HD / 4) + kk * 8),
+                             HD == 64 ? sw64_kmajor_desc(ka + kk * 32) : sw128_kmajor_desc(ka + (kk >> 2) * (C::KT * 128) + (kk & 3) * 32), idesc_s, (half | kk) ? 1u : 0u);
+            tc_commit_warp(&k_empty[of + s]);
+            tc_commit_warp(&s_full[of + sb]);
+          }
+          if (i >= 2) {
+            const int j = i - 2, pb = j & 1;
+            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+            ok = mbar_wait_warp(&w_full[of + pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[of + pb], ph, status, P5_ERR_WAIT_ATTN);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t va = base + C::W_OFF + pb * C::TILE16;
+#pragma unroll
+            for (int kk = 0; kk < C::KT / 16; ++kk)
+              tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
+                                 sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
+            tc_commit_warp(&w_empty[of + pb]);
+            tc_commit_warp(&p_empty[of + pb]);
+          }
         }
-        if (i >= 2) {
-          const int j = i - 2, pb = j & 1;
-          const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-          ok = mbar_wait_warp(&w_full[pb], ph, status, P5_ERR_WAIT_ATTN) && mbar_wait_warp(&p_full[pb], ph, status, P5_ERR_WAIT_ATTN);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = base + C::W_OFF + pb * C::TILE16;
-  #pragma unroll
-          for (int kk = 0; kk < C::KT / 16; ++kk)
-            tc_mma_f16_ta_warp(tmem + C::O_COL, tmem + (uint32_t)(C::P_COL + pb * (C::KT / 2) + kk * 8),
-                               sw128_mnmajor_desc(va + kk * 2048, C::KT * 128), idesc_o, (j | kk) ? 1u : 0u);
-          tc_commit_warp(&w_empty[pb]);
-          tc_commit_warp(&p_empty[pb]);
-        }
-      }
-      if (!ok) flags[0] = 1;
-      tc_commit_warp(o_full);
+        if (!ok) flags[0] = 1;
+        tc_commit_warp(&o_full[of]);
+      });
     } else if (warp == 3) {
       // ---- scales: two keys a lane, loaded a tile ahead
       const long c0 = (long)slot * a.capacity * a.kv_heads + kvh;
       int kb[2], vb[2];
       auto load = [&](int i) {
-  #pragma unroll
+#pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int key = (j0 + i) * C::KT + 2 * lane + q;
           const bool in = i < n && key < top;
@@ -301,94 +335,133 @@ __global__ void __launch_bounds__(512, 1)
           vb[q] = in ? (int)a.vs[c0 + (long)key * a.kv_heads] : -1;  // no key
         }
       };
-      int eb = -1000;
-      load(0);
+      int e_top = -1000, e_low = 1000;      // the largest and the smallest V exponent of the keys
+      constexpr int E_UP = 7, E_DOWN = 15;  // an fp16 tile: eb - E_DOWN .. eb + E_UP
+      auto scales = [&](auto in_bf16) {
+        constexpr bool WIDE = decltype(in_bf16)::value;
+        constexpr int of = WIDE ? C::BARS : 0;
+        // O's unit: none yet, or one for all tiles
+        int eb = WIDE ? max(min(e_low, e_top), e_top - KV8_E_SPAN) : -1000;
+        load(0);
+        for (int i = 0; i < n; ++i) {
+          const int s = i % C::NSC;
+          float kf[2];
+          uint32_t vf[2];
+          int ev[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
+            ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
+          }
+          load(i + 1);
+          float rescale = 1.f;
+          if constexpr (!WIDE) {
+            // the largest and the smallest exponent; that of a row of zeros (byte 0: or below 2^-117) is never the smallest
+            const int em = __reduce_max_sync(0xffffffffu, max(ev[0], ev[1]));
+            const int en = __reduce_min_sync(0xffffffffu, min(ev[0] > -127 ? ev[0] : 1000, ev[1] > -127 ? ev[1] : 1000));
+            e_top = max(e_top, em);
+            e_low = min(e_low, en);
+            if (em > eb + E_UP || en < eb - E_DOWN) {
+              const int to = en >= em - E_DOWN ? em : em - E_UP;
+              if (em - en > E_UP + E_DOWN || e_top - to > KV8_E_SPAN) flags[2] = 1;
+              if (i > 0) rescale = exp2_int(eb - to);  // 0 where there was no exponent yet: O is 0
+              eb = to;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {  // 2^(ev - eb) for two dims at a time: fp16, at most 2^E_UP, or bf16, at most 2^KV8_E_SPAN
+            const int e = ev[q] - eb;
+            const uint32_t f = WIDE ? (e < -133 ? 0u : (e < -126 ? 1u << (e + 133) : (uint32_t)(e + 127) << 7))
+                                    : (e < -24 ? 0u : (e < -14 ? 1u << (e + 24) : (uint32_t)(e + 15) << 10));
+            vf[q] = f * 0x10001u;
+          }
+          bool ok = !flags[0] && mbar_wait(&sc_empty[of + s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+          if (!__all_sync(0xffffffffu, ok)) {
+            flags[0] = 1;
+            break;
+          }
+          float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
+          *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
+          *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
+          if (lane == 0) {
+            sc[2 * C::KT] = rescale;
+            flags[1] = eb;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[of + s]);
+        }
+      };
+      scales(std::false_type());
+      if (__builtin_expect(meet(), 0)) scales(std::true_type());
+    } else if (met()) {  // the second pass' barriers, in the first's order
+      for (int i = lane; i < C::BARS; i += 32) {
+        const uint64_t* b = k_full + i;
+        const int count = b >= sc_empty && b < s_full ? 8 : ((b >= v_empty && b < w_empty) || (b >= s_empty && b < p_empty) ? 4 : 1);
+        mbar_init(k_full + C::BARS + i, count);
+      }
+      fence_barrier_init();
+      asm volatile("bar.sync 2, 512;" ::: "memory");
+    }
+  } else if (warp >= 12) {
+    regs_dec<C::REG_V>();
+    // ---- V codes -> fp16 or bf16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
+    // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
+    const int cw = warp - 12;
+    auto widen = [&](auto in_bf16) {
+      constexpr bool WIDE = decltype(in_bf16)::value;
+      constexpr int of = WIDE ? C::BARS : 0;
+      if (!mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN)) flags[0] = 1;  // Q is staged where widened V goes
       for (int i = 0; i < n; ++i) {
-        const int s = i % C::NSC;
-        float kf[2];
-        uint32_t vf[2];
-        int ev[2];
-  #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
-          ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
-        }
-        load(i + 1);
-        const int em = __reduce_max_sync(0xffffffffu, max(ev[0], ev[1]));
-        float rescale = 1.f;
-        if (em > eb + 7) {
-          if (i > 0) rescale = exp2_int(eb - em);  // 0 where there was no exponent yet: O is 0
-          eb = em;
-        }
-  #pragma unroll
-        for (int q = 0; q < 2; ++q) {  // 2^(ev - eb) <= 2^7 in fp16, for two dims at a time
-          const int e = ev[q] - eb;
-          vf[q] = (e < -24 ? 0u : (e < -14 ? 1u << (e + 24) : (uint32_t)(e + 15) << 10)) * 0x10001u;
-        }
-        bool ok = !flags[0] && mbar_wait(&sc_empty[s], ((uint32_t)(i / C::NSC) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
+        const int s = i % C::NK, wb = i & 1;
+        const int ss = i % C::NSC;
+        const bool ok = !flags[0] && mbar_wait(&v_full[of + s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                        mbar_wait(&sc_full[of + ss], (uint32_t)(i / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                        mbar_wait(&w_empty[of + wb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
         if (!__all_sync(0xffffffffu, ok)) {
           flags[0] = 1;
           break;
         }
-        float* sc = reinterpret_cast<float*>(smem + C::SC_OFF + s * C::SC_SLOT);
-        *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
-        *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
-        if (lane == 0) {
-          sc[2 * C::KT] = rescale;
-          flags[1] = eb;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_full[s]);
-      }
-    }
-  } else if (warp >= 12) {
-    regs_dec<C::REG_V>();
-    // ---- V codes -> fp16, MN-major boxes of 64 dims with the 128-byte swizzle.  Eight lanes take four neighbouring
-    // 16-byte pieces of rows r and r ^ 5: their reads and their two writes each hit different banks.
-    const int cw = warp - 12;
-    if (!mbar_wait_warp(q_full, 0, status, P5_ERR_WAIT_ATTN)) flags[0] = 1;  // Q is staged where widened V goes
-    for (int i = 0; i < n; ++i) {
-      const int s = i % C::NK, wb = i & 1;
-      const int ss = i % C::NSC;
-      const bool ok = !flags[0] && mbar_wait(&v_full[s], (uint32_t)(i / C::NK) & 1u, status, P5_ERR_WAIT_ATTN) &&
-                      mbar_wait(&sc_full[ss], (uint32_t)(i / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
-                      mbar_wait(&w_empty[wb], ((uint32_t)(i >> 1) & 1u) ^ 1u, status, P5_ERR_WAIT_ATTN);
-      if (!__all_sync(0xffffffffu, ok)) {
-        flags[0] = 1;
-        break;
-      }
-      const int valid = top - (j0 + i) * C::KT;  // rows from here on become zeros
-      const uint8_t* src = smem + C::V_OFF + s * C::TILE8;
-      const uint32_t* vf = reinterpret_cast<const uint32_t*>(smem + C::SC_OFF + ss * C::SC_SLOT) + C::KT;
-      uint8_t* dst = smem + C::W_OFF + wb * C::TILE16;
+        const int valid = top - (j0 + i) * C::KT;  // rows from here on become zeros
+        const uint8_t* src = smem + C::V_OFF + s * C::TILE8;
+        const uint32_t* vf = reinterpret_cast<const uint32_t*>(smem + C::SC_OFF + ss * C::SC_SLOT) + C::KT;
+        uint8_t* dst = smem + C::W_OFF + wb * C::TILE16;
 #pragma unroll
-      for (int k = 0; k < C::KT * HD / 16 / 128; ++k) {
-        const int id = k * 128 + cw * 32 + lane;  // [row pair][4 pieces of a group][2 rows] ...
-        const int j4 = id & 3, hi = (id >> 2) & 1, rest = id >> 3;
-        const int group = rest % (HD / 64), pair = rest / (HD / 64);  // 64-dim box, pair of rows of an 8-row group
-        const int row = (pair >> 2) * 8 + ((pair & 3) ^ (hi ? 5 : 0));
-        const int piece = group * 4 + j4;  // 16-byte piece of the key's codes
-        uint4 u = *reinterpret_cast<const uint4*>(HD == 64 ? src + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)
-                                                           : src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
-        if (row >= valid) u = make_uint4(0, 0, 0, 0);
-        const uint32_t f = vf[row];
-        auto two = [&](uint32_t c) {
-          const uint32_t h = fp8_to_h2((uint16_t)c);
-          const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&f));
-          return *reinterpret_cast<const uint32_t*>(&x);
-        };
-        uint8_t* d = dst + group * (C::KT * 128) + row * 128;
-        *reinterpret_cast<uint4*>(d + (((2 * j4) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.x >> 16), two(u.y), two(u.y >> 16));
-        *reinterpret_cast<uint4*>(d + (((2 * j4 + 1) ^ (row & 7)) << 4)) = make_uint4(two(u.z), two(u.z >> 16), two(u.w), two(u.w >> 16));
+        for (int k = 0; k < C::KT * HD / 16 / 128; ++k) {
+          const int id = k * 128 + cw * 32 + lane;  // [row pair][4 pieces of a group][2 rows] ...
+          const int j4 = id & 3, hi = (id >> 2) & 1, rest = id >> 3;
+          const int group = rest % (HD / 64), pair = rest / (HD / 64);  // 64-dim box, pair of rows of an 8-row group
+          const int row = (pair >> 2) * 8 + ((pair & 3) ^ (hi ? 5 : 0));
+          const int piece = group * 4 + j4;  // 16-byte piece of the key's codes
+          uint4 u = *reinterpret_cast<const uint4*>(HD == 64 ? src + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)
+                                                             : src + (piece >> 3) * (C::KT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+          if (row >= valid) u = make_uint4(0, 0, 0, 0);
+          const uint32_t f = vf[row];
+          auto two = [&](uint32_t c) {
+            const uint32_t h = fp8_to_h2((uint16_t)c);
+            if constexpr (WIDE) {
+              const uint32_t w = h2_to_bf2(h);
+              const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&f));
+              return *reinterpret_cast<const uint32_t*>(&x);
+            } else {
+              const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&f));
+              return *reinterpret_cast<const uint32_t*>(&x);
+            }
+          };
+          uint8_t* d = dst + group * (C::KT * 128) + row * 128;
+          *reinterpret_cast<uint4*>(d + (((2 * j4) ^ (row & 7)) << 4)) = make_uint4(two(u.x), two(u.x >> 16), two(u.y), two(u.y >> 16));
+          *reinterpret_cast<uint4*>(d + (((2 * j4 + 1) ^ (row & 7)) << 4)) = make_uint4(two(u.z), two(u.z >> 16), two(u.w), two(u.w >> 16));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&v_empty[of + s]);
+          mbar_arrive(&sc_empty[of + ss]);
+          mbar_arrive(&w_full[of + wb]);
+        }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&v_empty[s]);
-        mbar_arrive(&sc_empty[ss]);
-        mbar_arrive(&w_full[wb]);
-      }
-    }
+    };
+    widen(std::false_type());
+    if (__builtin_expect(meet(), 0)) widen(std::true_type());
   } else {
     regs_inc<C::REG_SOFT>();
     // ---- softmax: thread = row = TMEM lane; warpgroup g takes the tiles j with j % 2 == g, and half of the head dims of
@@ -450,129 +523,142 @@ __global__ void __launch_bounds__(512, 1)
       if (lane == 0) mbar_arrive(q_full);
     }
     float* m_ref = exch + 4 * C::ROWS + r;  // the row's running maximum
-    float m_run = -INFINITY, l_run = 0.f;
-    bool alive = true;
-    for (int j = g; j < n; j += 2) {
-      const int ss = j % C::NSC;
-      const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-      bool ok = !flags[0] && mbar_wait(&sc_full[ss], (uint32_t)(j / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
-                mbar_wait(&s_full[g], ph, status, P5_ERR_WAIT_ATTN);
-      if (!__all_sync(0xffffffffu, ok)) {
-        flags[0] = 1;
-        alive = false;
-        break;
-      }
-      tc_fence_after();
-      const float* sc = reinterpret_cast<const float*>(smem + C::SC_OFF + ss * C::SC_SLOT);
-      float x[C::KT];
-      {
-        uint32_t lo[32], hi[32];
-        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT), lo);
-        tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT + 32), hi);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(lo[c]), x[32 + c] = __uint_as_float(hi[c]);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[g]);
-      const int valid = lim - (j0 + j) * C::KT;  // columns of the tile that this row sees (may be <= 0)
-      // each column by its key's power of two
-#pragma unroll
-      for (int c = 0; c < C::KT; c += 4) {
-        const float4 k = *reinterpret_cast<const float4*>(sc + c);
-        const float2 a0 = mul2(make_float2(x[c], x[c + 1]), make_float2(k.x, k.y));
-        const float2 a1 = mul2(make_float2(x[c + 2], x[c + 3]), make_float2(k.z, k.w));
-        x[c] = a0.x, x[c + 1] = a0.y, x[c + 2] = a1.x, x[c + 3] = a1.y;
-      }
-      if (valid < C::KT) {
-#pragma unroll
-        for (int c = 0; c < C::KT; ++c)
-          if (c >= valid) x[c] = -INFINITY;
-      }
-      float mx[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mx[k] = fmaxf(x[k], x[8 + k]);
-#pragma unroll
-      for (int c = 16; c < C::KT; c += 16)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], x[c + k], x[c + 8 + k]);
-      // in base 2: rf carries the row's power of two, the softmax scale and log2 e
-      const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
-      const float rescale = sc[2 * C::KT];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sc_empty[ss]);
-      bool need = rescale != 1.f;
-      float alpha = rescale, m = mt;
-      if (j > 0) {  // the turn: the maximum after tile j - 1
-        ok = mbar_wait(&turn[4 * g + sub], (uint32_t)((j >> 1) - 1 + g) & 1u, status, P5_ERR_WAIT_ATTN);
-        const float before = *m_ref;
-        m = before;
-        if (mt > before + 8.f) {
-          need = true;
-          m = mt;
-          alpha *= before == -INFINITY ? 0.f : ex2_approx(before - mt);
+    float m_run, l_run;
+    bool alive;
+    auto softmax = [&](auto in_bf16) {
+      constexpr bool WIDE = decltype(in_bf16)::value;
+      constexpr int of = WIDE ? C::BARS : 0;
+      m_run = -INFINITY, l_run = 0.f;
+      alive = true;
+      for (int j = g; j < n; j += 2) {
+        const int ss = j % C::NSC;
+        const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+        bool ok = !flags[0] && mbar_wait(&sc_full[of + ss], (uint32_t)(j / C::NSC) & 1u, status, P5_ERR_WAIT_ATTN) &&
+                  mbar_wait(&s_full[of + g], ph, status, P5_ERR_WAIT_ATTN);
+        if (!__all_sync(0xffffffffu, ok)) {
+          flags[0] = 1;
+          alive = false;
+          break;
         }
-      }
-      *m_ref = m;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&turn[4 * (g ^ 1) + sub]);
-      l_run *= m_run == m ? 1.f : (m_run == -INFINITY ? 0.f : ex2_approx(m_run - m));
-      m_run = m;
-      const float msc = m == -INFINITY ? 0.f : m - 7.f;  // p and l as 2^7 of themselves, which O / l forgets
-      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const float2 rf2 = make_float2(rf, rf), nm2 = make_float2(-msc, -msc);
-      uint32_t pk[C::KT / 2];
+        tc_fence_after();
+        const float* sc = reinterpret_cast<const float*>(smem + C::SC_OFF + ss * C::SC_SLOT);
+        float x[C::KT];
+        {
+          uint32_t lo[32], hi[32];
+          tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT), lo);
+          tmem_ld32(t_lane + (uint32_t)(C::S_COL + g % C::NS * C::KT + 32), hi);
+          tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < C::KT; c += 4) {
-        const float2 x0 = fma2(make_float2(x[c], x[c + 1]), rf2, nm2);
-        const float2 x1 = fma2(make_float2(x[c + 2], x[c + 3]), rf2, nm2);
-        const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
-        ls[0] = add2(ls[0], p0);
-        ls[1] = add2(ls[1], p1);
-        const __half2 h0 = __floats2half2_rn(p0.x, p0.y), h1 = __floats2half2_rn(p1.x, p1.y);
-        pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-        pk[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
-      }
-      l_run += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
-      // P buffer g was last read by the P V product of tile j - 2
-      ok = ok && mbar_wait(&p_empty[g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
-      __syncwarp();
-      tc_fence_after();
-      tmem_st32(t_lane + (uint32_t)(C::P_COL + g * (C::KT / 2)), pk);
-      tmem_wait_st();
-      if (j > 0 && __any_sync(0xffffffffu, need)) {
-        // wait for the P V product of tile j - 1, then rescale this warp's rows of O
-        ok = ok && mbar_wait(&p_empty[g ^ 1], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
-        if (__all_sync(0xffffffffu, ok)) {
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(t_lane + (uint32_t)(C::O_COL + c), o);
-            tmem_wait_ld();
+          for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(lo[c]), x[32 + c] = __uint_as_float(hi[c]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[of + g]);
+        const int valid = lim - (j0 + j) * C::KT;  // columns of the tile that this row sees (may be <= 0)
+        // each column by its key's power of two
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(t_lane + (uint32_t)(C::O_COL + c), o);
+        for (int c = 0; c < C::KT; c += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(sc + c);
+          const float2 a0 = mul2(make_float2(x[c], x[c + 1]), make_float2(k.x, k.y));
+          const float2 a1 = mul2(make_float2(x[c + 2], x[c + 3]), make_float2(k.z, k.w));
+          x[c] = a0.x, x[c + 1] = a0.y, x[c + 2] = a1.x, x[c + 3] = a1.y;
+        }
+        if (valid < C::KT) {
+#pragma unroll
+          for (int c = 0; c < C::KT; ++c)
+            if (c >= valid) x[c] = -INFINITY;
+        }
+        float mx[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx[k] = fmaxf(x[k], x[8 + k]);
+#pragma unroll
+        for (int c = 16; c < C::KT; c += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], x[c + k], x[c + 8 + k]);
+        // in base 2: rf carries the row's power of two, the softmax scale and log2 e
+        const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
+        const float rescale = sc[2 * C::KT];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_empty[of + ss]);
+        bool need = rescale != 1.f;
+        float alpha = rescale, m = mt;
+        if (j > 0) {  // the turn: the maximum after tile j - 1
+          ok = mbar_wait(&turn[of + 4 * g + sub], (uint32_t)((j >> 1) - 1 + g) & 1u, status, P5_ERR_WAIT_ATTN);
+          const float before = *m_ref;
+          m = before;
+          if (mt > before + 8.f) {
+            need = true;
+            m = mt;
+            alpha *= before == -INFINITY ? 0.f : ex2_approx(before - mt);
           }
-          tmem_wait_st();
         }
+        *m_ref = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&turn[of + 4 * (g ^ 1) + sub]);
+        l_run *= m_run == m ? 1.f : (m_run == -INFINITY ? 0.f : ex2_approx(m_run - m));
+        m_run = m;
+        const float msc = m == -INFINITY ? 0.f : m - 7.f;  // p and l as 2^7 of themselves, which O / l forgets
+        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 rf2 = make_float2(rf, rf), nm2 = make_float2(-msc, -msc);
+        uint32_t pk[C::KT / 2];
+#pragma unroll
+        for (int c = 0; c < C::KT; c += 4) {
+          const float2 x0 = fma2(make_float2(x[c], x[c + 1]), rf2, nm2);
+          const float2 x1 = fma2(make_float2(x[c + 2], x[c + 3]), rf2, nm2);
+          const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
+          ls[0] = add2(ls[0], p0);
+          ls[1] = add2(ls[1], p1);
+          if constexpr (WIDE) {
+            pk[c / 2] = pack_bf2(p0.x, p0.y);
+            pk[c / 2 + 1] = pack_bf2(p1.x, p1.y);
+          } else {
+            const __half2 h0 = __floats2half2_rn(p0.x, p0.y), h1 = __floats2half2_rn(p1.x, p1.y);
+            pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+            pk[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          }
+        }
+        l_run += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+        // P buffer g was last read by the P V product of tile j - 2
+        ok = ok && mbar_wait(&p_empty[of + g], ph ^ 1u, status, P5_ERR_WAIT_ATTN);
+        __syncwarp();
+        tc_fence_after();
+        tmem_st32(t_lane + (uint32_t)(C::P_COL + g * (C::KT / 2)), pk);
+        tmem_wait_st();
+        if (j > 0 && __any_sync(0xffffffffu, need)) {
+          // wait for the P V product of tile j - 1, then rescale this warp's rows of O
+          ok = ok && mbar_wait(&p_empty[of + (g ^ 1)], (uint32_t)((j - 1) >> 1) & 1u, status, P5_ERR_WAIT_ATTN);
+          if (__all_sync(0xffffffffu, ok)) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_lane + (uint32_t)(C::O_COL + c), o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st32(t_lane + (uint32_t)(C::O_COL + c), o);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+          flags[0] = 1;
+          alive = false;
+          break;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[of + g]);
       }
-      if (!__all_sync(0xffffffffu, ok)) {
-        flags[0] = 1;
-        alive = false;
-        break;
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g]);
-    }
+      alive = mbar_wait(&o_full[of], 0, status, P5_ERR_WAIT_ATTN) && alive;
+    };
+    softmax(std::false_type());
+    if (__builtin_expect(meet(), 0)) softmax(std::true_type());
     const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
 
     // ---- O / l, or the split's partial
-    const bool done = mbar_wait(o_full, 0, status, P5_ERR_WAIT_ATTN);
     tc_fence_after();
-    const bool good = __all_sync(0xffffffffu, done && alive) && !flags[0];
+    const bool good = __all_sync(0xffffffffu, alive) && !flags[0];
     // the later tile's maximum is the larger; O is in units of it
     exch[g * 128 + r] = l_run;
     exch[(2 + g) * 128 + r] = m_run;

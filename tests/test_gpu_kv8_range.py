@@ -73,15 +73,16 @@ def written(pn, k, v):
     return cache
 
 
-def one_large_hidden_value(pn, kernel, shape, large, hi=2.0**-8, floor=0.0):
-    """V rows of 1 and a last one that only the last token sees: all others give exactly the mean of ones"""
+def one_large_hidden_value(pn, kernel, shape, large):
+    """V rows of 1 and a last one that only the last token sees: all others give the mean of ones"""
     B, T, H, kvh, hd, n = shape
     k = torch.zeros(B, n, kvh, hd, device="cuda")
     v = torch.ones(B, n, kvh, hd, device="cuda")
     v[:, n - 1] = large
     q = torch.zeros(B, T, H, hd, device="cuda", dtype=BF)
     got = run(pn, kernel, q, written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32), causal=True).float()
-    assert ((got[:, :-1] - 1).abs() <= hi).all()
+    first = max(T - n, 0)  # the first token that sees a key
+    assert (got[:, :first] == 0).all() and ((got[:, first:-1] - 1).abs() <= 2.0**-8).all()
     last = (n - 1 + float(v[0, -1, 0, 0].to(BF).double())) / n
     assert ((got[:, -1].double() - last).abs() <= 2.0**-4 * last).all()  # the value itself is rounded to e4m3
 
@@ -133,3 +134,62 @@ def test_rows_kernel_tiny_values(pn):
     q = randn(g, 1, 1, 8, 128, dtype=BF)
     cache = written(pn, k, v)
     bounded(run(pn, "rows", q, cache, i32(200)), q, cache, i32(200), floor=2.0**-126)
+
+
+# ---- the tcgen05 kernel: weights of a tile whose scales span more than 2^22 are bf16
+TC = [(2, 130, 8, 1, 256, 150), (8, 200, 8, 2, 128, 64), (4, 200, 8, 1, 128, 150), (8, 400, 8, 1, 64, 300)]
+TC_SPLIT = [(1, 968, 8, 1, 256, 968)]
+
+
+@pytest.mark.parametrize("large", [2.0**9, 2.0**16, 2.0**30, 2.0**90, 3.3e38])
+@pytest.mark.parametrize("shape", TC)
+def test_tcgen05_kernel_large_hidden_value(pn, shape, large):
+    one_large_hidden_value(pn, "tc", shape, large)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("spread", [4, 8, 40])
+@pytest.mark.parametrize("shape", TC + TC_SPLIT)
+def test_tcgen05_kernel_values_far_apart(pn, shape, spread, causal):
+    far_apart(pn, "tc", shape, causal, 44, spread, weight=BF16 if spread > 8 else FP16)
+
+
+def test_tcgen05_kernel_values_growing_and_shrinking(pn):
+    g = gen(45)
+    B, T, H, kvh, hd, n = 2, 150, 8, 1, 128, 4000
+    e = 60 * torch.sin(torch.arange(n, device="cuda") / 400.0)
+    v = randn(g, B, n, kvh, hd) * torch.exp2(e)[None, :, None, None]
+    k = randn(g, B, n, kvh, hd)
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache = written(pn, k, v)
+    for lens in (i32(n, 1256), i32(471, 940)):
+        bounded(run(pn, "tc", q, cache, lens), q, cache, lens, weight=BF16)
+
+
+def test_tcgen05_kernel_wide_tiles_among_others(pn):
+    """tiles of 64 keys by turns of one size, far apart, and of another size: the weights' type changes from tile to tile"""
+    g = gen(46)
+    B, T, H, kvh, hd, n = 4, 200, 8, 1, 128, 64 * 9 + 5
+    v = randn(g, B, n, kvh, hd)
+    e = torch.zeros(n, device="cuda")
+    e[64:128] = torch.randint(-30, 30, (64,), device="cuda", generator=g).float()
+    e[256:320] = 40
+    e[384:448] = torch.randint(-60, 60, (64,), device="cuda", generator=g).float()
+    e[576] = 100
+    v *= torch.exp2(e)[None, :, None, None]
+    k = randn(g, B, n, kvh, hd)
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache = written(pn, k, v)
+    for causal in (False, True):
+        lens = i32(n, 577, 380, 250)
+        bounded(run(pn, "tc", q, cache, lens, causal=causal), q, cache, lens, causal=causal, weight=BF16)
+
+
+def test_tcgen05_kernel_tiny_values(pn):
+    g = gen(47)
+    v = randn(g, 4, 150, 1, 128) * 2.0**-115
+    k = randn(g, 4, 150, 1, 128)
+    q = randn(g, 4, 200, 8, 128, dtype=BF)
+    cache = written(pn, k, v)
+    lens = i32(150, 100, 64, 3)
+    bounded(run(pn, "tc", q, cache, lens), q, cache, lens, weight=BF16, floor=2.0**-126)
