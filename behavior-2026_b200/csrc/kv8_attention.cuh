@@ -48,7 +48,7 @@ struct Kv8Args {
   float scale_log2;  // scale * log2(e)
   int n_slots, capacity, T, heads, kv_heads, G, causal;
   int splits, groups;  // key splits, and clusters of them: splits = groups * CTAs of a cluster
-  float* ws_o;         // [groups][batch][heads * T][head_dim], O in units of the group's 2^m
+  float* ws_o;         // [groups][batch][heads * T][head_dim], O / l of the group: never above the largest |V|
   float2* ws_ml;       // [groups][batch][heads * T] (m, l)
 };
 
@@ -464,9 +464,9 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
     }
     const float unit = exp2_int(e);
     const int t = row / a.G, h = kvh * a.G + row % a.G;
+    // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
+    const float inv = l == 0.f ? 0.f : unit / l;
     if (a.groups == 1) {
-      // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
-      const float inv = l == 0.f ? 0.f : unit / l;
       bf16* dst = a.out + (long)b * a.o_b + (long)t * a.o_t + (long)h * HD;
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k)
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
       const long i = ((long)group * (gridDim.y / a.kv_heads) + b) * out_rows + (long)h * a.T + t;
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k)
-        *reinterpret_cast<float2*>(a.ws_o + i * HD + 64 * k + 2 * lane) = make_float2(x[2 * k] * unit, x[2 * k + 1] * unit);
+        *reinterpret_cast<float2*>(a.ws_o + i * HD + 64 * k + 2 * lane) = make_float2(x[2 * k] * inv, x[2 * k + 1] * inv);
       if (lane == 0) a.ws_ml[i] = make_float2(m, l);
     }
   }
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
   }
 }
 
-// Joins the groups of key splits of a row: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, in order.
+// Joins the groups of key splits of a row: out = sum_s w_s O_s / sum_s w_s with w_s = 2^(m_s - m) l_s, in order.
 // One warp a row.
 template <int HD>
 __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
@@ -493,16 +493,25 @@ __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
   const long rows = (long)batch * a.T * a.heads;
   const long i = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (i >= rows || (a.count && (int)(i % a.T) >= kv8_tokens(a, (int)(i / ((long)a.T * a.heads))))) return;
-  float m = -INFINITY;
-  for (int s = 0; s < a.groups; ++s) m = fmaxf(m, a.ws_ml[s * rows + i].x);
-  float l = 0.f, acc[HD / 32];
+  float2 ml[2];  // lane: groups lane and lane + 32 (there are at most 64)
+#pragma unroll
+  for (int k = 0; k < 2; ++k) ml[k] = lane + 32 * k < a.groups ? a.ws_ml[(lane + 32 * k) * rows + i] : make_float2(-INFINITY, 0.f);
+  float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float w[2], l;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) w[k] = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ml[k].y * ex2_approx(ml[k].x - m);
+  l = w[0] + w[1];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float acc[HD / 32];
 #pragma unroll
   for (int k = 0; k < HD / 32; ++k) acc[k] = 0.f;
   for (int s = 0; s < a.groups; ++s) {
-    const float2 ml = a.ws_ml[s * rows + i];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = ex2_approx(ml.x - m);
-    l += ml.y * f;
+    const float f = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31) * inv;
+    if (f == 0.f) continue;
 #pragma unroll
     for (int k = 0; k < HD / 64; ++k) {
       const float2 x = *reinterpret_cast<const float2*>(a.ws_o + (s * rows + i) * HD + 64 * k + 2 * lane);
@@ -510,14 +519,13 @@ __global__ void kv8_attn_combine_kernel(const Kv8Args a, int batch) {
       acc[2 * k + 1] += x.y * f;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   const long per = (long)a.T * a.heads;
   const long b = i / per;
   const int h = (int)(i % per / a.T), t = (int)(i % a.T);
   bf16* dst = a.out + b * a.o_b + (long)t * a.o_t + (long)h * HD;
 #pragma unroll
   for (int k = 0; k < HD / 64; ++k)
-    *reinterpret_cast<uint32_t*>(dst + 64 * k + 2 * lane) = pack_bf2(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+    *reinterpret_cast<uint32_t*>(dst + 64 * k + 2 * lane) = pack_bf2(acc[2 * k], acc[2 * k + 1]);
 }
 
 }  // namespace p5

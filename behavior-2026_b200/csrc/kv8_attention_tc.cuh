@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(512, 1)
     if (__builtin_expect(meet(), 0)) softmax(std::true_type());
     const uint32_t t_o = t_lane + (uint32_t)(C::O_COL + g * (HD / 2));
 
-    // ---- O / l, or the split's partial
+    // ---- O / l, of the split where there are more
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, alive) && !flags[0];
     // the later tile's maximum is the larger; O is in units of it
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(512, 1)
     const float l = (m0 == m_run ? 1.f : ex2_approx(m0 - m_run)) * exch[r] + (m1 == m_run ? 1.f : ex2_approx(m1 - m_run)) * exch[128 + r];
     const float unit = exp2_int(n > 0 ? (int)flags[1] : 0);
     // l is 0 for a row without keys (its output is 0), NaN for one that sees a NaN
-    const float f = a.groups == 1 ? (l == 0.f ? 0.f : unit / l) : unit;
+    const float f = l == 0.f ? 0.f : unit / l;
     const long part = ((long)split * (gridDim.y / a.kv_heads) + b) * ((long)a.T * a.heads);
 #pragma unroll 1
     for (int c = 0; c < HD / 2; c += 32) {

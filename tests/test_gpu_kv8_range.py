@@ -193,3 +193,24 @@ def test_tcgen05_kernel_tiny_values(pn):
     cache = written(pn, k, v)
     lens = i32(150, 100, 64, 3)
     bounded(run(pn, "tc", q, cache, lens), q, cache, lens, weight=BF16, floor=2.0**-126)
+
+
+# ---- key splits joined through a workspace
+@pytest.mark.parametrize("shape,kernel", [(ROWS_SPLIT[0], ["kv8_attn_rows", "kv8_attn_combine"]), (TC_SPLIT[0], ["kv8_attn_tc", "kv8_attn_combine"])])
+@pytest.mark.parametrize("size", [1.0, 2.0**120, 3.0e38])
+def test_partials_of_the_largest_values_are_finite(pn, shape, kernel, size):
+    """V next to the largest finite number: no weighted average of it is larger"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(48)
+    v = (0.5 + 0.5 * torch.rand(B, n, kvh, hd, device="cuda", generator=g)) * size
+    k = randn(g, B, n, kvh, hd)
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache = written(pn, k, v)
+    got = run(pn, kernel, q, cache, i32(n))
+    assert torch.isfinite(got).all()
+    bounded(got / size, q, (cache[0], cache[1], cache[2], (cache[3].int() - int(math.log2(size))).to(torch.uint8)), i32(n)) if size < 3e38 else None
+
+
+@pytest.mark.parametrize("large", [2.0**30, 3.3e38])
+def test_large_hidden_value_with_splits(pn, large):
+    one_large_hidden_value(pn, "tc", TC_SPLIT[0], large)
