@@ -66,6 +66,12 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the smaller one; NaN if either is
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // two fp16 -> two bf16 (exact for widened e4m3 codes: 4 bits)
 __device__ __forceinline__ uint32_t h2_to_bf2(uint32_t h) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
@@ -188,7 +194,8 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
     mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
     // |q| < 2^(e + 1); the row is scaled by 2^(14 - e) (kept within the float range)
     const int e = min(max((int)(mb >> 7) - 127, -112), 127);
-    const float up = exp2_int(14 - e);
+    // a query with a NaN or an infinity: its row is NaN, unless it sees no key.  The sign of the softmax scale goes into Q.
+    const float up = mb >= 0x7f80u ? NAN : (a.scale_log2 < 0.f ? -exp2_int(14 - e) : exp2_int(14 - e));
 #pragma unroll
     for (int i = 0; i < KI; ++i)
 #pragma unroll
@@ -197,8 +204,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
         const __half2 hh = __floats2half2_rn(f.x * up, f.y * up);
         qf[i][j] = *reinterpret_cast<const uint32_t*>(&hh);
       }
-    // a query with a NaN or an infinity: its row is NaN, unless it sees no key
-    const float down = mb >= 0x7f80u ? NAN : a.scale_log2 * exp2_int(e - 14);
+    const float down = fminf(fabsf(a.scale_log2) * exp2_int(e - 14), 3.4028235e38f);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       rf[j] = __shfl_sync(0xffffffffu, down, (2 * c + j) * 4);
@@ -256,7 +262,9 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
           const float kf = __shfl_sync(0xffffffffu, kf1, 16 * n + 8 * q + g);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float x = (s[n][2 * q + j] + s2[n][2 * q + j]) * rf[j] * kf;
+            // the row's and the key's factors first: each may be near the float range where their product is not (and where
+            // that passes it, a sum of 0 is still a logit of 0)
+            const float x = (s[n][2 * q + j] + s2[n][2 * q + j]) * min_nan(rf[j] * kf, 3.4028235e38f);
             s[n][2 * q + j] = key0 + 16 * n + 8 * q < lim[j] ? x : -INFINITY;
           }
         }

@@ -44,7 +44,7 @@ struct Kv8TcCfg {
   static constexpr int K_OFF = 0, V_OFF = NK * TILE8, W_OFF = 2 * NK * TILE8;
   static constexpr int Q_BYTES = ROWS * (HD * 2 + 16);  // query rows on their way in, over the widened V
   static constexpr int SC_OFF = W_OFF + (2 * TILE16 > Q_BYTES ? 2 * TILE16 : (Q_BYTES + 127) / 128 * 128);
-  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64] (fp32), vf[64] (fp16 or bf16, twice), rescale factor of O
+  static constexpr int SC_SLOT = (2 * KT + 4) * 4;  // kf[64] (fp32), vf[64] (fp16 or bf16, twice), rescale factor of O, unit of kf
   static constexpr int X_OFF = SC_OFF + NSC * SC_SLOT;  // [5][128] floats between the two softmax warpgroups
   static constexpr int BAR_OFF = X_OFF + 5 * ROWS * 4;
   static constexpr int BARS = 4 * NK + 2 * NSC + 21;  // barriers of a pass
@@ -347,12 +347,18 @@ __global__ void __launch_bounds__(512, 1)
           const int s = i % C::NSC;
           float kf[2];
           uint32_t vf[2];
-          int ev[2];
+          int ev[2], kt = 0;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : fp8_scale_value(kb[q]);  // a NaN row: NaN for the rows that see it
+            kt = max(kt, kb[q] == 255 ? 0 : kb[q]);
             ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
           }
+          // A tile's largest K factor is kept to 2^64, with the rest (kh) for the row's own factor: codes and K factor alone, up to
+          // 2^146, would leave the float range where the logit does not.
+          const int kh = max(__reduce_max_sync(0xffffffffu, kt) - (127 + 64), 0);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : exp2_int(kb[q] - 127 - kh);  // a NaN row: NaN for the rows that see it
           load(i + 1);
           float rescale = 1.f;
           if constexpr (!WIDE) {
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(512, 1)
           *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(kf[0], kf[1]);
           *reinterpret_cast<uint2*>(sc + C::KT + 2 * lane) = make_uint2(vf[0], vf[1]);
           if (lane == 0) {
-            sc[2 * C::KT] = rescale;
+            *reinterpret_cast<float2*>(sc + 2 * C::KT) = make_float2(rescale, exp2_int(kh));
             flags[1] = eb;
           }
           __syncwarp();
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(512, 1)
     // Q and O at the start and the end
     const uint32_t t_lane = tmem + ((uint32_t)(sub * 32) << 16);
     const int lim = !in ? 0 : (a.causal ? min(len, len - tokens + t + 1) : len);
-    float rf;
+    float row_factor;
     {
       const uint8_t* sq = smem + C::W_OFF;
       cp_async_wait<0>();
@@ -486,12 +492,12 @@ __global__ void __launch_bounds__(512, 1)
       mb = max(__float_as_uint(exch[r]), __float_as_uint(exch[128 + r]));
       const bool bad = mb >= 0x7f800000u;  // a query with a NaN or an infinity: its row is NaN, unless it sees no key
       const int byte = bad ? 127 : fp8_scale_byte(__uint_as_float(mb));
-      // rf > 0, so that a masked logit of -inf stays one: the sign of the softmax scale goes into Q, a scale of 0 makes Q zero,
-      // and a factor below the float range (a query of zeros, a tiny scale) is the smallest normal one
+      // the row's factor is >= 0: the sign of the softmax scale goes into Q, and a scale of 0 makes Q zero.  A query with a NaN or an
+      // infinity has NaN codes, which make every logit of its row NaN.
       const float sign = a.scale_log2 < 0.f ? -1.f : (a.scale_log2 == 0.f ? 0.f : 1.f);
       const float up = bad ? 0.f : sign * fp8_scale_inverse(byte);
       const float2 up2 = make_float2(up, up);
-      rf = bad && lim > 0 ? NAN : (sign == 0.f ? 1.f : fmaxf(fp8_scale_value(byte) * fabsf(a.scale_log2), 1.17549435e-38f));
+      row_factor = fp8_scale_value(byte) * fabsf(a.scale_log2);
       constexpr int NC = HD / 8;  // columns of this half: four codes each
       constexpr int CH = NC < 16 ? NC : 16;
 #pragma unroll 1
@@ -575,9 +581,12 @@ __global__ void __launch_bounds__(512, 1)
         for (int c = 16; c < C::KT; c += 16)
 #pragma unroll
           for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], x[c + k], x[c + 8 + k]);
-        // in base 2: rf carries the row's power of two, the softmax scale and log2 e
+        // in base 2: rf carries the row's power of two, the softmax scale, log2 e and the unit of the K factors.  It is positive
+        // and finite, so that a masked logit of -inf stays one and a sum of 0 gives 0.
+        const float2 tile = *reinterpret_cast<const float2*>(sc + 2 * C::KT);
+        const float rf = fminf(fmaxf(row_factor * tile.y, 1.17549435e-38f), 3.4028235e38f);
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
-        const float rescale = sc[2 * C::KT];
+        const float rescale = tile.x;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_empty[of + ss]);
         bool need = rescale != 1.f;

@@ -214,3 +214,33 @@ def test_partials_of_the_largest_values_are_finite(pn, shape, kernel, size):
 @pytest.mark.parametrize("large", [2.0**30, 3.3e38])
 def test_large_hidden_value_with_splits(pn, large):
     one_large_hidden_value(pn, "tc", TC_SPLIT[0], large)
+
+
+# ---- logits of ordinary size from very large and very small factors
+@pytest.mark.parametrize("qe,ke", [(116, -114), (-114, 116), (-60, 62), (62, -60), (100, -100), (-100, 100)])
+@pytest.mark.parametrize("kernel,shape", [("rows", ROWS[0]), ("rows", ROWS[1]), ("tc", TC[0]), ("tc", TC[2]), ("tc", TC[3])])
+def test_large_keys_and_small_queries_or_the_reverse(pn, kernel, shape, qe, ke):
+    B, T, H, kvh, hd, n = shape
+    g = gen(49)
+    q = (randn(g, B, T, H, hd) * 2.0**qe).to(BF)
+    k = randn(g, B, n, kvh, hd) * 2.0**ke
+    k[:, 5::9] *= 2.0**-8  # smaller rows beside them
+    v = randn(g, B, n, kvh, hd)
+    cache = written(pn, k, v)
+    lens = torch.arange(n, n - B, -1, device="cuda").int()
+    bounded(run(pn, kernel, q, cache, lens, causal=True), q, cache, lens, causal=True)
+
+
+@pytest.mark.parametrize("kernel,shape", [("rows", ROWS[1]), ("tc", TC[0])])
+def test_queries_and_keys_both_large_but_orthogonal(pn, kernel, shape):
+    """products of zeros: the weights are equal however large the factors"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(50)
+    q, k = torch.zeros(B, T, H, hd, device="cuda"), torch.zeros(B, n, kvh, hd, device="cuda")
+    q[..., : hd // 2] = randn(g, B, T, H, hd // 2) * 2.0**100
+    k[..., hd // 2 :] = randn(g, B, n, kvh, hd // 2) * 2.0**100
+    v = randn(g, B, n, kvh, hd)
+    cache = written(pn, k, v)
+    lens = torch.full((B,), n, device="cuda", dtype=torch.int32)
+    q = q.to(BF)
+    bounded(run(pn, kernel, q, cache, lens), q, cache, lens)
