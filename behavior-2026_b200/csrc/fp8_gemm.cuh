@@ -396,13 +396,13 @@ __global__ void __launch_bounds__(256, Fp8FewCfg<BN>::PER_SM)
 // ------------------------------------------------------------------ many tokens
 // A cluster of two CTAs owns 256 tokens x bn features (bn <= 240, a multiple of 16): each stages 128 token rows and
 // bn / 2 weight rows per K block, and one thread of the even CTA issues tcgen05.mma.cta_group::2 over both, as in
-// gemm_pair.cuh (the same ring, relay and commit protocol).  Measured: 7744 x 32768 x 2048 GeGLU 400 us, 2.6 PFLOP/s in short
-// bursts (tensor pipes 72 % busy); run for seconds the power cap holds it at 478 us, 2.17, where a library product with one
-// scale a tensor and no epilogue gets 2.26.  7744 x 2048 x 16384 200 us.  Its scale words are never waited for (without
-// them 472 us against 479 when that was measured).  Tensor memory holds two accumulators of bn columns and, in the
+// gemm_pair.cuh (the same ring, relay and commit protocol).  Measured: 7744 x 32768 x 2048 GeGLU 411 us, 2.5 PFLOP/s in short
+// bursts (tensor pipes 72 % busy); run for seconds the power cap holds it near 2.2, where a library product with one
+// scale a tensor and no epilogue gets 2.26.  7744 x 2048 x 16384 211 us.  Announcing the odd CTA's scale words soundly is 2 and 6 %
+// of these.  Tensor memory holds two accumulators of bn columns and, in the
 // rest, chunks of scale words (4 columns of tokens, 8 of features); bn = 256 would leave room for one accumulator only,
 // and its epilogue could not run under the next tile's products.
-//   warp 0 TMA, warp 1 MMA (odd CTA: relay), warp 2 TMEM, warps 4-11 epilogue, warps 12-15 scales
+//   warp 0 TMA, warp 1 MMA (odd CTA: relay), warp 2 TMEM, warp 3 the odd CTA's scales, warps 4-11 epilogue, warps 12-15 scales
 struct Fp8PairCfg {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = 120 * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 5;
@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
   uint64_t* sf_full = tempty + 2;                // [slots] this CTA's scale words in place (4 warps)
   uint64_t* sf_empty = sf_full + C::MAX_SLOTS;   // [slots] MMAs done with the scale words (multicast commit)
   uint64_t* rows_full = sf_empty + C::MAX_SLOTS;  // [2] sf_rows buffer written by the four scale warps
-  uint64_t* done = rows_full + 2;
+  uint64_t* sf_peer = rows_full + 2;              // [slots] even CTA: the odd CTA's scale words in place (its warp 3)
+  uint64_t* done = sf_peer + C::MAX_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] abort
   int* status = &g_fp8_status;
@@ -458,6 +459,7 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
     }
     for (int i = 0; i < C::MAX_SLOTS; ++i) {
       mbar_init(&sf_full[i], 4);
+      mbar_init(&sf_peer[i], 1);
       mbar_init(&sf_empty[i], 1);
     }
     mbar_init(done, 1);
@@ -520,7 +522,8 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
         if ((i & 3) == 0) {
           if (++slot == slots) slot = 0;
           if (slot == 0) sf_ph ^= 1u;
-          ok = mbar_wait_warp(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL);
+          ok = mbar_wait_warp(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL) &&
+               mbar_wait_cl_warp(&sf_peer[slot], sf_ph, status, P5_ERR_WAIT_FULL);
         }
         ok = ok && mbar_wait_warp(&full[s], ph, status, P5_ERR_WAIT_FULL) && mbar_wait_warp(&pair[s], ph, status, P5_ERR_WAIT_FULL);
         if (!ok) break;
@@ -541,27 +544,40 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
     tc_commit2_mc_warp(done, 3);
   } else if (warp == 1) {
     if (lane == 0) {
+      // relaxed, as in gemm_pair.cuh: nothing but a completion that the TMA has signalled is passed on
       const uint32_t pair0 = map_peer(smem_u32(pair), 0);
-      int it = 0, slot = -1;
-      uint32_t sf_ph = 1;
+      int it = 0;
       for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
         for (int i = 0; i < a.blocks; ++i, ++it) {
           const int s = it % C::STAGES;
-          if ((i & 3) == 0) {  // a chunk's first stage is passed on once its scale words are in place too
-            if (++slot == slots) slot = 0;
-            if (slot == 0) sf_ph ^= 1u;
-            if (!mbar_wait(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL)) {
-              flags[0] = 1;
-              break;
-            }
-            tc_fence_after();
-            tc_fence_before();
-          }
           if (!mbar_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, status, P5_ERR_WAIT_FULL)) {
             flags[0] = 1;
             break;
           }
           mbar_arrive_cluster_relaxed(pair0 + (uint32_t)s * 8u);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // The odd CTA's scale words are written by its warps: this lane announces them with a release at cluster scope, which the
+    // issuer acquires once a chunk.  A warp of its own, because a release holds its thread up (7744 x 32768 x 2048: by the relay
+    // 445 us, by the scale warps 435, here 423).
+    if (!even && lane == 0) {
+      const uint32_t sf_peer0 = map_peer(smem_u32(sf_peer), 0);
+      int slot = -1;
+      uint32_t sf_ph = 1;
+      for (int u = cid; u < n_units && !flags[0]; u += nclusters) {
+        for (int i = 0; i < a.blocks; i += 4) {
+          if (++slot == slots) slot = 0;
+          if (slot == 0) sf_ph ^= 1u;
+          if (!mbar_wait(&sf_full[slot], sf_ph, status, P5_ERR_WAIT_FULL)) {
+            flags[0] = 1;
+            break;
+          }
+          tc_fence_after();
+          tc_fence_before();
+          mbar_arrive_cluster(sf_peer0 + (uint32_t)slot * 8u);
         }
       }
     }
