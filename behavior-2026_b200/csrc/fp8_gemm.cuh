@@ -684,6 +684,7 @@ __global__ void __launch_bounds__(Fp8PairCfg::THREADS, 1)
         for (int q = 0; q < PASS; q += 32) {
           if (q >= width) break;
           uint32_t r[32];
+          __syncwarp();  // lanes behind the last token have skipped the arithmetic below
           if (q + 32 <= width) {
             tmem_ld32(t_acc + (uint32_t)(c + q), r);
           } else {

@@ -148,3 +148,13 @@ def test_two_streams_and_a_graph(pn, T, F, K):
     y.fill_(-1)
     gr.replay()
     assert torch.equal(y, want[0])
+
+
+@pytest.mark.parametrize("T", [1793, 1799, 1823, 1825, 1855])
+def test_pair_with_warps_across_the_last_token(pn, T):
+    """the last token inside a warp's 32: its lanes behind it sit out the epilogue's arithmetic and no more"""
+    F, K = 4306, 640
+    for epi in ("gelu", "f32"):
+        x, w, bias, _, _ = case(pn, 68 + T, T, F, K, epi, True)
+        check_linear(pn, *x, *w, epi, bias)
+        reaches(pn, "fp8_pair_kernel", *x, *w, epi=epi, bias=bias)
