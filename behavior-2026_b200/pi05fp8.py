@@ -2,7 +2,7 @@
 
 Reached as pi05native.fp8_quantize and so on.  Each call runs on torch's current stream of its tensors' device, allocates
 its outputs (and attention's workspace) from torch's allocator, may be captured into a torch.cuda.CUDAGraph, and raises
-Pi05Error where the shapes, types or devices do not fit.  float8_e4m3fn codes and uint8 exponent bytes: a block's values are
+Pi05Error where the shapes, types or devices do not fit, or where autograd would want a gradient (there is no backward pass).  float8_e4m3fn codes and uint8 exponent bytes: a block's values are
 codes * 2^(byte - 127); byte 255 stands for NaN.
 
 The checks are written for a few microseconds a call: a single-token step makes several hundred of these calls.
@@ -17,12 +17,20 @@ from pi05native import ERR_ARG, OK, Engine, Pi05Error, lib
 E4M3, U8, BF, F32, I32 = torch.float8_e4m3fn, torch.uint8, torch.bfloat16, torch.float32, torch.int32
 EPI = Engine.EPI
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-_empty, _empty_strided = torch.empty, torch.empty_strided
+_empty, _empty_strided, _grad_enabled = torch.empty, torch.empty_strided, torch.is_grad_enabled
 _tls = threading.local()
 
 
 def _bad(what):
     raise Pi05Error(ERR_ARG, what)
+
+
+def _no_grad(what, *tensors):
+    """these operators have no backward pass, so a result that autograd expects to follow is refused, not returned without a graph"""
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _bad(f"{what}: no backward pass: call it under torch.no_grad(), or with tensors that need no gradient")
 
 
 def _err():
@@ -60,6 +68,7 @@ def fp8_quantize(x, out=None):
     dt, shape, dev = x.dtype, x.shape, x.get_device()
     if dev < 0 or len(shape) != 2 or (dt != BF and dt != F32) or x.numel() == 0:
         _bad("fp8_quantize: x must be a CUDA tensor [rows][cols], bf16 or fp32, not empty")
+    _no_grad("fp8_quantize", x)
     rows, cols = shape
     blocks = (cols + 127) // 128
     if out is None:
@@ -100,6 +109,7 @@ def fp8_linear(x, x_scales, w, w_scales, epi="store", bias=None, res=None, gate=
         _bad("fp8_linear: x [T][K] and w [F][K] must agree in K, scales must be [rows][ceil(K / 128)]")
     if w.get_device() != dev or x_scales.get_device() != dev or w_scales.get_device() != dev:
         _bad("fp8_linear: operands on different devices")
+    _no_grad("fp8_linear", bias, res, gate, out)
     code = EPI.get(epi)
     if code is None or (code == 4 and F % 2):
         _bad(f"fp8_linear: unknown epilogue {epi!r}, or geglu with an odd F")
@@ -161,6 +171,7 @@ def _rows(what, k, v, h, d, dev):
     if k.dtype != BF or v.dtype != BF or len(shape) != 4 or v.shape != shape or shape[2] != h or shape[3] != d or k.numel() == 0 \
             or k.get_device() != dev or v.get_device() != dev:
         _bad(f"{what}: k, v must be CUDA bf16 tensors [batch][T][kv_heads][head_dim] of the cache's heads and device, not empty")
+    _no_grad(what, k, v)
     strides = _strides(what, k, shape)
     if v.stride() != k.stride() and _strides(what, v, shape) != strides:
         _bad(f"{what}: k and v must be strided alike")
@@ -210,6 +221,7 @@ def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False,
     shape = q.shape
     if q.dtype != BF or len(shape) != 4 or shape[3] != d or shape[2] % kvh or q.numel() == 0:
         _bad("kv8_attention: q must be a CUDA bf16 tensor [batch][T][heads][head_dim], heads a multiple of the cache's, not empty")
+    _no_grad("kv8_attention", q, out)
     batch, T, heads, _ = shape
     qb, qt = _strides("kv8_attention", q, shape)
     if out is None:
