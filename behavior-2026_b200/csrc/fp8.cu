@@ -36,6 +36,10 @@ int launched(const char* what, char* err, size_t err_len) {
   return PI05_OK;
 }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// rows of `width` elements at b * sample + t * token (token >= width): none shares an element with another, whichever axis is outer
+bool apart(int batch, int T, int64_t sample, int64_t token, int64_t width) {
+  return batch == 1 || sample >= token * (T - 1) + width || (sample >= width && token >= sample * (batch - 1) + width);
+}
 
 // ------------------------------------------------------------------ quantisation
 // Eight lanes take a block of 128 values, 16 each, and ITEMS consecutive blocks, whose loads are all issued before the first
@@ -197,7 +201,7 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
     return fail(err, err_len, PI05_ERR_ARG,
                 "%s: k, v and the caches must be 16-byte aligned device pointers, rows at least kv_heads * head_dim "
                 "elements and a multiple of 8 apart", what);
-  if (!WRITE && a.batch > 1 && a.b_stride < a.t_stride * (a.T - 1) + (long)a.kv_heads * head_dim)
+  if (!WRITE && !apart(a.batch, a.T, a.b_stride, a.t_stride, (long)a.kv_heads * head_dim))
     return fail(err, err_len, PI05_ERR_ARG, "%s: samples of k, v overlap", what);
   if (!a.slots && a.batch > a.n_slots)
     return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
@@ -626,7 +630,7 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
   if (!q || !k8 || !k_scales || !v8 || !v_scales || !lens || !out || !aligned(q, 16) || !aligned(k8, 16) || !aligned(v8, 16) ||
       !aligned(out, 16) || q_sample_stride % 8 || q_token_stride % 8 || out_sample_stride % 8 || out_token_stride % 8 ||
       q_token_stride < width || out_token_stride < width || q_sample_stride < 0 || out_sample_stride < 0 ||
-      (batch > 1 && out_sample_stride < out_token_stride * (T - 1) + width))
+      !apart(batch, T, out_sample_stride, out_token_stride, width))
     return fail(err, err_len, PI05_ERR_ARG,
                 "pi05_kv8_attention: q, out and the caches must be 16-byte aligned device pointers, tokens of q and out "
                 "at least heads * head_dim elements and a multiple of 8 apart, samples of out not overlapping");

@@ -124,3 +124,16 @@ def test_python_refuses_host_tensors_and_wrong_types(pn):
         pn.kv8_read(k8, ks, k8, ks)
     with pytest.raises(pn.Pi05Error):
         pn.kv8_attention(k, k8, ks, k8, ks, lens=torch.zeros(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kw", [dict(T=4, sb=256, st=256), dict(T=4, sb=128, st=1024), dict(T=4, sb=264, st=512), dict(batch=3, T=4, sb=256, st=512)])
+def test_reading_into_rows_that_share_elements_is_refused(pn, kw):
+    """neither the samples' nor the tokens' rows clear of each other (256 elements a row)"""
+    rc, msg = call(pn, "pi05_kv8_read", *rows_args(**kw))
+    assert rc == ERR_ARG and "overlap" in msg
+
+
+@pytest.mark.parametrize("kw", [dict(T=2, ob=1024, ot=1024), dict(T=3, ob=512, ot=4096), dict(batch=3, T=2, ob=1024, ot=2048)])
+def test_attention_into_rows_that_share_elements_is_refused(pn, kw):
+    rc, msg = call(pn, "pi05_kv8_attention", *attention_args(**kw))
+    assert rc == ERR_ARG and "overlapping" in msg

@@ -24,3 +24,22 @@ def test_a_tensor_that_needs_a_gradient_is_refused(pn):
         call(lambda t: t)
         with torch.no_grad():
             call(grad)
+
+
+@pytest.mark.parametrize("T,B,kvh,hd", [(5, 3, 2, 128), (140, 4, 1, 256), (40, 8, 2, 64)])
+def test_outputs_with_tokens_outside_samples(pn, T, B, kvh, hd):
+    """[T][batch][heads][head_dim] buffers seen as [batch][T]...: no two rows share an element"""
+    g = gen(72)
+    cache = filled(pn, g, B, T + 7, kvh, hd)
+    lens = torch.arange(T + 7, T + 7 - B, -1, device="cuda").int()
+    q = randn(g, T, B, 4 * kvh, hd, dtype=BF).transpose(0, 1)
+    out = torch.full((T, B, 4 * kvh, hd), 3.0, device="cuda", dtype=BF).transpose(0, 1)
+    got = pn.kv8_attention(q, *cache, lens=lens, causal=True, out=out)
+    assert got is out and torch.equal(got, pn.kv8_attention(q.contiguous(), *cache, lens=lens, causal=True))
+    k, v = (torch.zeros(T, B, kvh, hd, device="cuda", dtype=BF).transpose(0, 1) for _ in range(2))
+    pn.kv8_read(*cache, T=T, start=i32(*range(B)), out=(k, v))
+    want = pn.kv8_read(*cache, T=T, start=i32(*range(B)))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    twice = new_cache(B, T, kvh, hd, fill=0, scale=0)
+    pn.kv8_write(k, v, *twice)
+    assert all(torch.equal(a, b) for a, b in zip(pn.kv8_read(*twice), want))
