@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -36,6 +37,24 @@ int launched(const char* what, char* err, size_t err_len) {
   return PI05_OK;
 }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// SMs of the current device; a B200's where there is none (a host that only asks for sizes)
+int num_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return 148;
+    }
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 // rows of `width` elements at b * sample + t * token (token >= width): none shares an element with another, whichever axis is outer
 bool apart(int batch, int T, int64_t sample, int64_t token, int64_t width) {
   return batch == 1 || sample >= token * (T - 1) + width || (sample >= width && token >= sample * (batch - 1) + width);
@@ -210,7 +229,7 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
   // writing 68 us with 16 values a thread and 2 rows (8 and 4: 95), reading 62 us with 8 and 4 (16 and 2: 71)
   constexpr int MANY = WRITE ? 2 : 4;
   const int threads = 256, per = threads / (head_dim / (WRITE ? 16 : 8));
-  const bool few = head_rows * a.batch < 148L * 8 * per;
+  const bool few = head_rows * a.batch < 8L * num_sms() * per;
   const long gx = (head_rows + per * (few ? 1 : MANY) - 1) / (per * (few ? 1 : MANY));
   if (head_rows > 0x7fffffffL) return fail(err, err_len, PI05_ERR_ARG, "%s: T * kv_heads must be below 2^31", what);
   const dim3 grid((unsigned)gx, a.batch, 2);
@@ -395,14 +414,12 @@ int linear(Fp8Args& a, const void* x, long ldx, const void* w, long ldw, int K, 
 }
 
 // ------------------------------------------------------------------ attention
-int num_sms() {
-  static int n = [] {
-    int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      return 148;
-    return v;
-  }();
-  return n;
+// what attention and the query of its workspace take
+bool attention_shape(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
+  return batch >= 1 && T >= 1 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && capacity >= 1 &&
+         (head_dim == 64 || head_dim == 128 || head_dim == 256) && (int64_t)batch * kv_heads <= 65535 &&
+         (int64_t)T * (heads / kv_heads) <= (1 << 30) && (int64_t)batch * T <= 0x7fffffff / heads &&
+         (int64_t)kv_heads * head_dim * capacity < (1LL << 40);
 }
 
 struct AttentionPlan {
@@ -419,9 +436,10 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
   const double rows = (double)T * (heads / kv_heads), pairs = (double)batch * kv_heads;
   AttentionPlan best = {false, 1, 1};
   double best_cost = 1e300;
+  const int sms = num_sms();
   {  // a step: 32 keys of one of four warps
     const double tiles = pairs * ceil(rows / 8), steps = ceil(capacity / 128.0);
-    const double places = (double)num_sms() * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
+    const double places = (double)sms * (head_dim == 256 ? 1 : (head_dim == 128 ? 2 : 4));
     const double step = head_dim == 256 ? 1.8 : (head_dim == 128 ? 1.0 : 0.9);
     for (int s = 1; s <= 256 && (s == 1 || s <= steps); s *= 2) {
       const double cost = ceil(tiles * s / places) * (6 + ceil(steps / s) * step) + (s > 8 ? 3 : 0);
@@ -433,9 +451,9 @@ AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head
     const double tiles = pairs * ceil(rows / 128), steps = ceil(capacity / 64.0);
     const double fixed = head_dim == 256 ? 10 : (head_dim == 128 ? 8 : 6), step = head_dim == 256 ? 0.9 : 0.65;
     for (int s = 1; s <= 64 && (s == 1 || 2 * s <= steps); s += 1 + s / 3) {
-      const double cost = ceil(tiles * s / num_sms()) * (fixed + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
+      const double cost = ceil(tiles * s / sms) * (fixed + ceil(steps / s) * step) + (s > 1 ? 3 : 0);
       if (cost < best_cost) best_cost = cost, best = {true, s, 1};
-      if (tiles * s > 2 * num_sms()) break;
+      if (tiles * s > 2 * sms) break;
     }
   }
   return best;
@@ -606,9 +624,7 @@ extern "C" PI05_API int pi05_kv8_read(int batch, int T, int kv_heads, int head_d
 }
 
 extern "C" PI05_API int64_t pi05_kv8_attention_workspace(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
-  if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || capacity < 1 ||
-      (head_dim != 64 && head_dim != 128 && head_dim != 256))
-    return PI05_ERR_ARG;
+  if (!attention_shape(batch, T, heads, kv_heads, head_dim, capacity)) return PI05_ERR_ARG;
   const AttentionPlan p = attention_plan(batch, T, heads, kv_heads, head_dim, capacity);
   const int64_t groups = p.splits / p.cluster;
   return groups == 1 ? 0 : groups * batch * T * heads * ((int64_t)head_dim * 4 + 8);
@@ -621,11 +637,11 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
                                            void* out,
                                            int64_t out_sample_stride, int64_t out_token_stride, void* workspace,
                                            int64_t workspace_bytes, void* stream, char* err, size_t err_len) {
-  if (batch < 1 || T < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || n_slots < 1 || capacity < 1 ||
-      (int64_t)batch * kv_heads > 65535 || (int64_t)T * (heads / kv_heads) > (1 << 30) || (int64_t)batch * T > 0x7fffffff / heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+  if (n_slots < 1 || !attention_shape(batch, T, heads, kv_heads, head_dim, capacity))
     return fail(err, err_len, PI05_ERR_ARG,
                 "pi05_kv8_attention: needs batch, T, n_slots, capacity >= 1, heads a multiple of kv_heads, head_dim 64, 128 "
-                "or 256, batch * kv_heads <= 65535, batch * T * heads < 2^31");
+                "or 256, batch * kv_heads <= 65535, T * heads / kv_heads <= 2^30, batch * T * heads < 2^31, a slot of the cache "
+                "smaller than 2^40 bytes");
   const int64_t width = (int64_t)heads * head_dim;
   if (!q || !k8 || !k_scales || !v8 || !v_scales || !lens || !out || !aligned(q, 16) || !aligned(k8, 16) || !aligned(v8, 16) ||
       !aligned(out, 16) || q_sample_stride % 8 || q_token_stride % 8 || out_sample_stride % 8 || out_token_stride % 8 ||
@@ -635,8 +651,6 @@ extern "C" PI05_API int pi05_kv8_attention(int batch, int T, int heads, int kv_h
                 "pi05_kv8_attention: q, out and the caches must be 16-byte aligned device pointers, tokens of q and out "
                 "at least heads * head_dim elements and a multiple of 8 apart, samples of out not overlapping");
   if (!slots && batch > n_slots) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: batch exceeds the cache's slots");
-  if ((int64_t)kv_heads * head_dim * capacity >= (1LL << 40))
-    return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: a slot of the cache must be smaller than 2^40 bytes");
   if (!(scale == scale) || scale - scale != 0.f) return fail(err, err_len, PI05_ERR_ARG, "pi05_kv8_attention: scale must be finite");
   Kv8Args a = {};
   a.q = static_cast<const bf16*>(q);

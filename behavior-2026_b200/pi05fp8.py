@@ -235,7 +235,11 @@ def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False,
         _bad("kv8_attention: lens is required")
     lens, slots = _index(lens, batch, dev, "kv8_attention: lens"), _index(slots, batch, dev, "kv8_attention: slots")
     count = _index(count, batch, dev, "kv8_attention: count")
-    need = lib.pi05_kv8_attention_workspace(batch, T, heads, kvh, d, cap)
+    if dev == _device():
+        need = lib.pi05_kv8_attention_workspace(batch, T, heads, kvh, d, cap)
+    else:
+        with torch.cuda.device(dev):
+            need = lib.pi05_kv8_attention_workspace(batch, T, heads, kvh, d, cap)
     if need > 0:
         ws = _empty(need, dtype=U8, device=q.device)
         ws_at = ws.data_ptr()

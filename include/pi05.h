@@ -314,7 +314,9 @@ PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
  *   infinity, gives NaN.  heads is a multiple of kv_heads; query head h reads K/V head
  *   h / (heads / kv_heads).  q and out bf16, token t of sample b at b * sample stride + t * token stride elements, heads
  *   contiguous, 16-byte aligned.  workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
- *   of no importance before and after. */
+ *   of no importance before and after.  The bytes depend on every size (and on the current device), and not monotonically: fewer
+ *   samples or tokens may need more than many, because few rows are split along the keys.  Ask for each shape that will be
+ *   called and keep the largest.  PI05_ERR_ARG (negative) for sizes that attention refuses. */
 PI05_API int pi05_kv8_write(int batch, int T, int kv_heads, int head_dim, const void* k, const void* v, int64_t sample_stride,
                             int64_t token_stride, int n_slots, int capacity, void* k8, uint8_t* k_scales, void* v8,
                             uint8_t* v_scales, const int32_t* start, const int32_t* count, const int32_t* slots, void* stream,

@@ -137,3 +137,26 @@ def test_reading_into_rows_that_share_elements_is_refused(pn, kw):
 def test_attention_into_rows_that_share_elements_is_refused(pn, kw):
     rc, msg = call(pn, "pi05_kv8_attention", *attention_args(**kw))
     assert rc == ERR_ARG and "overlapping" in msg
+
+
+@pytest.mark.parametrize("bad", [(40000, 1, 8, 2, 128, 64), (1, 1 << 30, 8, 2, 128, 64), (1 << 12, 1 << 12, 512, 1, 64, 64),
+                                 (1, 1, 8, 2, 128, 0x7fffffff), (-1, 1, 8, 1, 256, 64), (1, 1, 8, 0, 256, 64)])
+def test_workspace_is_asked_for_the_shapes_that_attention_takes(pn, bad):
+    """a size is never given for a call that would then be refused"""
+    b, t, h, kvh, hd, cap = bad
+    if (kvh, cap) != (2, 0x7fffffff):  # 2^39 bytes a slot: taken
+        assert pn.lib.pi05_kv8_attention_workspace(*bad) == ERR_ARG
+        rc, _ = call(pn, "pi05_kv8_attention", *attention_args(batch=b, T=t, heads=h, kvh=kvh, hd=hd, capacity=cap, n_slots=1 << 20))
+        assert rc == ERR_ARG
+    else:
+        assert pn.lib.pi05_kv8_attention_workspace(*bad) >= 0
+        assert pn.lib.pi05_kv8_attention_workspace(b, t, h, 8, 128, cap) == ERR_ARG
+
+
+def test_workspaces_are_not_monotone_and_each_is_enough_for_its_own_shape(pn):
+    need = [pn.lib.pi05_kv8_attention_workspace(n, 50, 8, 1, 256, 1024) for n in (2, 8, 64)]
+    assert need[2] == 0 and need[0] > 0 and need[1] > 0
+    for n, bytes_ in zip((2, 8), need):
+        rc, msg = call(pn, "pi05_kv8_attention", *attention_args(batch=n, T=50, heads=8, kvh=1, hd=256, qb=50 * 2048, qt=2048, ob=50 * 2048,
+                                                                ot=2048, n_slots=64, capacity=1024, ws_bytes=bytes_ - 1))
+        assert rc == ERR_ARG and "workspace" in msg
