@@ -222,6 +222,13 @@ int kv8_rows(const char* what, const KvRows& a, int head_dim, void* stream, char
                 "elements and a multiple of 8 apart", what);
   if (!WRITE && !apart(a.batch, a.T, a.b_stride, a.t_stride, (long)a.kv_heads * head_dim))
     return fail(err, err_len, PI05_ERR_ARG, "%s: samples of k, v overlap", what);
+  // what is written must be two things: K and V rows nearer to each other than a row is long, or caches that overlap, are not
+  const auto near = [](const void* p, const void* q, double bytes) {
+    return (double)((uintptr_t)p > (uintptr_t)q ? (uintptr_t)p - (uintptr_t)q : (uintptr_t)q - (uintptr_t)p) < bytes;
+  };
+  const double heads = (double)a.n_slots * a.capacity * a.kv_heads;
+  if (WRITE ? near(a.k8, a.v8, heads * head_dim) || near(a.ks, a.vs, heads) : near(x0, x1, 2.0 * a.kv_heads * head_dim))
+    return fail(err, err_len, PI05_ERR_ARG, "%s: what is written for K and for V overlaps", what);
   if (!a.slots && a.batch > a.n_slots)
     return fail(err, err_len, PI05_ERR_ARG, "%s: batch exceeds the cache's slots", what);
   const long head_rows = (long)a.T * a.kv_heads;

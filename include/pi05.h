@@ -307,7 +307,8 @@ PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
  *   start[b] + t (start NULL: t).  Samples of k, v may overlap (a stride of 0).  Everything else in the cache stays as it was.  Where two samples name the same
  *   slot and position the later sample's row is kept.
  * pi05_kv8_read: the reverse; rows that are passed over stay as they were in k and v.  In k, v (and in attention's out) samples
- *   may lie one behind the other or token by token ([T][batch]...); rows that share elements are refused.
+ *   may lie one behind the other or token by token ([T][batch]...); rows that share elements, and k and v (for a write: caches) that lie over
+ *   each other, are refused.
  * pi05_kv8_attention: out[b][t][h] = sum_j p_j V_j, p = softmax over j < lens[b] (clamped to [0, capacity]) of
  *   scale * q[b][t][h] . K_j for the tokens t < n, n = count[b] (count NULL: T; clamped to [0, T]); rows from n on are left as they
  *   were in out.  causal != 0: token t sees j < lens[b] - n + t + 1 (the last one sees all, as after a write of the n tokens).  A row that sees nothing gives 0; one that sees a NaN row of the cache, or whose query holds a NaN or an

@@ -160,3 +160,13 @@ def test_workspaces_are_not_monotone_and_each_is_enough_for_its_own_shape(pn):
         rc, msg = call(pn, "pi05_kv8_attention", *attention_args(batch=n, T=50, heads=8, kvh=1, hd=256, qb=50 * 2048, qt=2048, ob=50 * 2048,
                                                                 ot=2048, n_slots=64, capacity=1024, ws_bytes=bytes_ - 1))
         assert rc == ERR_ARG and "workspace" in msg
+
+
+@pytest.mark.parametrize("name,kw", [("pi05_kv8_read", dict()), ("pi05_kv8_read", dict(v=A + 496)), ("pi05_kv8_read", dict(k=A + 16)),
+                                     ("pi05_kv8_write", dict()), ("pi05_kv8_write", dict(v8=A + 4 * 16 * 256 - 16, vs=A - 4096)),
+                                     ("pi05_kv8_write", dict(v8=A + (1 << 19), vs=A + 127)), ("pi05_kv8_write", dict(k8=A + (1 << 19), ks=A + 1))])
+def test_k_and_v_written_to_one_place_is_refused(pn, name, kw):
+    a = dict(batch=2, T=4, kvh=2, hd=128, sb=1024, st=256, n_slots=4, capacity=16)
+    a.update(kw)
+    rc, msg = call(pn, name, *rows_args(**a))
+    assert rc == ERR_ARG and "overlaps" in msg

@@ -43,3 +43,16 @@ def test_outputs_with_tokens_outside_samples(pn, T, B, kvh, hd):
     twice = new_cache(B, T, kvh, hd, fill=0, scale=0)
     pn.kv8_write(k, v, *twice)
     assert all(torch.equal(a, b) for a, b in zip(pn.kv8_read(*twice), want))
+
+
+def test_reading_into_the_two_halves_of_a_buffer(pn):
+    g = gen(73)
+    cache = filled(pn, g, 2, 30, 2, 128)
+    both = torch.zeros(2, 30, 4, 128, device="cuda", dtype=BF)
+    k, v = pn.kv8_read(*cache, out=(both[:, :, :2], both[:, :, 2:]))
+    want = pn.kv8_read(*cache)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    with pytest.raises(pn.Pi05Error, match="overlaps"):
+        pn.kv8_read(*cache, out=(want[0], want[0]))
+    with pytest.raises(pn.Pi05Error, match="overlaps"):
+        pn.kv8_write(*want, cache[0], cache[1], cache[0], cache[3])
