@@ -144,8 +144,8 @@ def _index(t, batch, dev, what):
 def _cache(what, dev, k8, k_scales, v8, v_scales):
     """(slots, capacity, kv_heads, head_dim) and the four addresses"""
     shape = k8.shape
-    if len(shape) != 4 or v8.shape != shape or k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
-        _bad(f"{what}: codes must be [slots][capacity][kv_heads][head_dim], scales [slots][capacity][kv_heads]")
+    if len(shape) != 4 or v8.shape != shape or k_scales.shape != shape[:3] or v_scales.shape != shape[:3] or 0 in shape:
+        _bad(f"{what}: codes must be [slots][capacity][kv_heads][head_dim], not empty, scales [slots][capacity][kv_heads]")
     if k8.dtype != E4M3 or v8.dtype != E4M3 or k_scales.dtype != U8 or v_scales.dtype != U8:
         _bad(f"{what}: codes must be float8_e4m3fn, scales uint8")
     if not (k8.is_contiguous() and v8.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
@@ -197,6 +197,8 @@ def kv8_read(k8, k_scales, v8, v_scales, start=None, T=None, count=None, slots=N
     dev = k8.get_device()
     (n, cap, h, d), at = _cache("kv8_read", dev, k8, k_scales, v8, v_scales)
     first = start if start is not None else count if count is not None else slots
+    if first is not None and first.dim() != 1:
+        _bad("kv8_read: start, count and slots must be int32 tensors [batch]")
     batch = n if first is None else first.shape[0]
     T = cap if T is None else T
     if out is None:
@@ -219,7 +221,7 @@ def kv8_attention(q, k8, k_scales, v8, v_scales, lens, slots=None, causal=False,
     dev = q.get_device()
     (n, cap, kvh, d), at = _cache("kv8_attention", dev, k8, k_scales, v8, v_scales)
     shape = q.shape
-    if q.dtype != BF or len(shape) != 4 or shape[3] != d or shape[2] % kvh or q.numel() == 0:
+    if dev < 0 or q.dtype != BF or len(shape) != 4 or shape[3] != d or shape[2] % kvh or q.numel() == 0:
         _bad("kv8_attention: q must be a CUDA bf16 tensor [batch][T][heads][head_dim], heads a multiple of the cache's, not empty")
     _no_grad("kv8_attention", q, out)
     batch, T, heads, _ = shape

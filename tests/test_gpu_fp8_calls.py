@@ -56,3 +56,22 @@ def test_reading_into_the_two_halves_of_a_buffer(pn):
         pn.kv8_read(*cache, out=(want[0], want[0]))
     with pytest.raises(pn.Pi05Error, match="overlaps"):
         pn.kv8_write(*want, cache[0], cache[1], cache[0], cache[3])
+
+
+@pytest.mark.parametrize("shape", [(1, 8, 0, 256), (0, 8, 1, 256), (1, 0, 1, 256)])
+def test_empty_caches_are_refused(pn, shape):
+    """with the library's own error, before anything is divided or allocated"""
+    k8, ks = torch.zeros(shape, device="cuda").to(E4M3), torch.zeros(shape[:3], device="cuda", dtype=torch.uint8)
+    cache = (k8, ks, k8.clone(), ks.clone())
+    q, k = torch.zeros(1, 1, 8, 256, device="cuda", dtype=BF), torch.zeros(1, 1, 1, 256, device="cuda", dtype=BF)
+    for call in (lambda: pn.kv8_attention(q, *cache, lens=i32(1)), lambda: pn.kv8_read(*cache), lambda: pn.kv8_write(k, k, *cache)):
+        with pytest.raises(pn.Pi05Error):
+            call()
+
+
+def test_an_index_that_is_no_vector_is_refused(pn):
+    cache = new_cache(2, 8, 1, 256, fill=0, scale=0)
+    with pytest.raises(pn.Pi05Error):
+        pn.kv8_read(*cache, start=torch.tensor(0, device="cuda", dtype=torch.int32))
+    with pytest.raises(pn.Pi05Error):
+        pn.kv8_read(*cache, slots=torch.zeros(1, 1, device="cuda", dtype=torch.int32))
