@@ -75,3 +75,38 @@ def test_an_index_that_is_no_vector_is_refused(pn):
         pn.kv8_read(*cache, start=torch.tensor(0, device="cuda", dtype=torch.int32))
     with pytest.raises(pn.Pi05Error):
         pn.kv8_read(*cache, slots=torch.zeros(1, 1, device="cuda", dtype=torch.int32))
+
+
+def test_the_engines_prefixes_held_in_8_bits(pn):
+    """a server's path: prefixes of two samples out of the engine into slots of an 8-bit cache, later back into the engine, all by
+    device pointers.  What the engine then holds is the quantised prefix bit for bit, and it denoises as from the same
+    values installed from the host."""
+    import ctypes
+
+    import numpy as np
+    from test_gpu_fp8 import decode, encode
+
+    layers, n = 2, 2
+    eng = pn.Engine(pn.Config.make(siglip_layers=1, gemma_layers=layers, num_steps=2), max_batch=n)
+    eng.init_random_weights(3)
+    imgs = np.stack([pn.synth_images(3, i) for i in range(n)])
+    toks = np.stack([pn.synth_tokens(3, i) for i in range(n)])
+    noise = np.stack([pn.synth_noise(3, i) for i in range(n)])
+    plain = eng.infer(imgs, toks, noise)
+    P = eng.prefix_len
+    k, v = (torch.empty(n, layers, P, 256, device="cuda", dtype=BF) for _ in range(2))
+    for i in range(n):
+        for layer in range(layers):
+            assert pn.lib.pi05_get_prefix_cache(eng._h, i, layer, ctypes.c_void_p(k[i, layer].data_ptr()), ctypes.c_void_p(v[i, layer].data_ptr())) == 0
+    cache = new_cache(7, P, 1, 256)
+    slots = i32(5, 0, 3, 6)
+    pn.kv8_write(k.view(n * layers, P, 1, 256), v.view(n * layers, P, 1, 256), *cache, slots=slots)
+    k2, v2 = pn.kv8_read(*cache, T=P, slots=slots)
+    torch.cuda.synchronize()
+    assert pn.lib.pi05_set_prefix_cache(eng._h, n, ctypes.c_void_p(k2.data_ptr()), ctypes.c_void_p(v2.data_ptr())) == 0
+    got = eng.denoise(noise)
+    host = [decode(*encode(t)).to(BF).cpu() for t in (k, v)]
+    assert torch.equal(k2.view_as(k).cpu(), host[0]) and torch.equal(v2.view_as(v).cpu(), host[1])
+    eng.set_prefix_cache(*(t.view(torch.int16).numpy().view(np.uint16) for t in host))
+    want = eng.denoise(noise)
+    assert np.array_equal(got, want) and np.isfinite(got).all() and not np.array_equal(got, plain)
