@@ -365,7 +365,9 @@ __global__ void __launch_bounds__(256, Fp8FewCfg<BN>::PER_SM)
     if (threadIdx.x < (unsigned)a.splits)
       bulk_copy_to_peer(map_peer(smem_u32(recv) + rank * bytes, threadIdx.x), smem_u32(ring) + threadIdx.x * bytes, bytes,
                         map_peer(smem_u32(got), threadIdx.x));
-    if (!mbar_wait_cl(got, 0, status, P5_ERR_WAIT_SPLITK)) flags[0] = 1;
+    // A peer whose own waits give up still sends, up to four limits later: this CTA must not free what that copy writes, nor
+    // pass the barrier that keeps the peer's copy readable, so it waits for it all the same.
+    for (int k = 0; k < 8 && !mbar_wait_cl(got, 0, status, P5_ERR_WAIT_SPLITK); ++k) flags[0] = 1;
     __syncthreads();
     cluster_arrive_relaxed();
   }
