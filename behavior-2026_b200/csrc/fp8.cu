@@ -436,8 +436,8 @@ struct AttentionPlan {
 
 // By sizes that the host knows (the lengths are on the device): the kernel and its key splits by an estimate in microseconds of
 // waves x (fixed + steps), fitted to measurements.  E.g. 1018 keys, 8 heads on one of 256: one chunk of 50 tokens
-// 14.2 (rows, 2 splits), 18.2 (tc, 8 splits); 64 chunks 365 (rows), 48.5 (tc); 8 x 5 tokens 14.1 (rows), 16.7 (tc).
-// Heads of 64: 8 x 500 tokens, 16 heads, 2,000 keys 322 (rows), 103 (tc); 8 x 50 tokens, 8 on 2, 1,000 keys 14.1 (rows, 1 split),
+// 14.2 (rows, 2 splits), 18.2 (tc, 8 splits); 64 chunks 365 (rows), 50.6 (tc); 8 x 5 tokens 14.1 (rows), 16.7 (tc).
+// Heads of 64: 8 x 500 tokens, 16 heads, 2,000 keys 322 (rows), 105 (tc); 8 x 50 tokens, 8 on 2, 1,000 keys 14.1 (rows, 1 split),
 // 16.4 (tc, 1 split), 13.4 (the plan's).
 AttentionPlan attention_plan(int batch, int T, int heads, int kv_heads, int head_dim, int capacity) {
   const double rows = (double)T * (heads / kv_heads), pairs = (double)batch * kv_heads;

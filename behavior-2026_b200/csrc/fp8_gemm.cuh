@@ -202,8 +202,9 @@ __device__ __forceinline__ void fp8_epilogue8(const Fp8Args& a, float (&v)[8], i
 // are on the 128-row side, so a handful of tokens still reads each weight once and at full width.  The fp32 partial tiles
 // meet over distributed shared memory: CTA p receives the token slice p of every partial in one bulk copy each and adds
 // them in rank order (reruns give the same bits).
-// Bound by what one SM takes in (a block of 20 / 24 / 32 KB every 0.36 / 0.47 / 0.42 us), and below 10 us by its fixed chain:
-// 50 x 8192 x 1024 GeGLU 6.9 us (bytes alone 1.4), 50 x 32768 x 2048 17.6 us, 3.8 TB/s of weights, 1 x 32768 x 2048 15.2 us, 4.4.
+// Below 10 us bound by a CTA's fixed chain and by tiles that do not fill the machine (50 x 8192 x 1024 GeGLU 6.6 us, bytes
+// alone 1.4: 64 CTAs), above by uneven shares: a weight of 32768 rows is 256 tiles, two on 108 SMs and one on 40 (50 x 32768 x 2048
+// 17.8 us, 3.8 TB/s of weights; 1 x 32768 x 2048 15.7 us, 4.3).
 //   warp 0  TMA producer, warp 1  MMA issuer, warp 2  TMEM, warps 4-7  scales, then the accumulator
 template <int BN>
 struct Fp8FewCfg {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(256, Fp8FewCfg<BN>::PER_SM)
 // A cluster of two CTAs owns 256 tokens x bn features (bn <= 240, a multiple of 16): each stages 128 token rows and
 // bn / 2 weight rows per K block, and one thread of the even CTA issues tcgen05.mma.cta_group::2 over both, as in
 // gemm_pair.cuh (the same ring, relay and commit protocol).  Measured: 7744 x 32768 x 2048 GeGLU 411 us, 2.5 PFLOP/s in short
-// bursts (tensor pipes 72 % busy); run for seconds the power cap holds it near 2.2, where a library product with one
+// bursts (tensor pipes 69 % busy); run for seconds the power cap holds it near 2.2, where a library product with one
 // scale a tensor and no epilogue gets 2.26.  7744 x 2048 x 16384 211 us.  Announcing the odd CTA's scale words soundly is 2 and 6 %
 // of these.  Tensor memory holds two accumulators of bn columns and, in the
 // rest, chunks of scale words (4 columns of tokens, 8 of features); bn = 256 would leave room for one accumulator only,

@@ -11,8 +11,8 @@
 //
 // One new token reads the whole cache once for a handful of products, so what counts is bytes in flight: each warp
 // keeps a ring of its own of STAGES steps (cp.async, no barrier between warps), 48 to 192 KB an SM.  Measured, 16 samples of 32
-// heads on 8 of 128: 46 us and 5.8 TB/s at 8,192 keys each, 70-73 us and 4.7 TB/s at 4,000 to 16,387 (the longest sample decides);
-// one sample of 1,018 keys 10 us, its chain of latencies.
+// heads on 8 of 128: 46 us and 5.8 TB/s at 8,192 keys each, 71 us and 4.9 TB/s at 4,000 to 16,387 (the longest sample decides);
+// one sample of 1,018 keys on one head of 256 9.6 us, its chain of latencies, of 30,000 24 us.
 //
 // Everything is computed transposed, keys and head dims on the 16-row side of mma.m16n8k16 and query rows on
 // the 8-column side, because one token of 8 heads has 8 rows, not 16:
@@ -28,7 +28,8 @@
 // The running maximum moves only when a logit exceeds it by 2^4, and eb only when a scale leaves eb .. eb + 11, so
 // p * 2^(ev - eb) stays within 2^15, a weight keeps 11 bits (or 2^-25 of the largest) whatever other keys' scales are, and O is
 // rarely rescaled.  A step whose scales span more than that (a key that a row does not see counts as well: its scale must
-// not push that row's weights below the range) takes V and P in bf16, P as two operands hi + lo (16 bits): any scale fits.
+// not push that row's weights below the range) takes V and P in bf16, P as two operands hi + lo (16 bits): any scale fits
+// (every step so: 60 us for the 46 above).
 #pragma once
 #include <type_traits>
 

@@ -18,9 +18,10 @@
 //                 Where a tile's scales span more (a key that some rows do not see counts as well: it must not cost them
 //                 bits), the CTA goes through its keys again with V and P in bf16, into which any scale fits; V is exact,
 //                 weights keep 8 bits.  A choice of type for each tile made every call 2 to 7 % slower, in each form tried.
-// Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 48.5 us (550 TFLOP/s); 8 x 968 x 968 95 us (649); 2 x 2,049
-// tokens, causal over 8,192 keys, 16 heads on 4 of 128 310 us (777) and on 2 of 64 268 us (448).  No unit is full (at HD 128 tensor pipes 43 %, exponentials
-// 43 %, issue 54 %, shared memory 52 %): a tile waits on the chain of its softmax, about 2,400 clocks for two tiles in
+// Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 50.6 us (527 TFLOP/s); 8 x 968 x 968 98 us (629); 2 x 2,049
+// tokens, causal over 8,192 keys, 16 heads on 4 of 128 315 us (764) and on 2 of 64 270 us (446); where the second pass is needed the
+// chunks take 92 us, the third 683.  No unit is full (at HD 128 tensor pipes 43 %, exponentials
+// 43 %, issue 56 %, shared memory 53 %): a tile waits on the chain of its softmax, about 2,400 clocks for two tiles in
 // turn, and at HD 256 a short call on the 10 us that a CTA takes to load its queries and to store.  Three warpgroups were
 // slower than two (349 against 328 us then): they leave a thread 128 registers.
 // The running maximum moves only when a tile exceeds it by 2^8 and the V exponent eb only when a scale leaves its window;

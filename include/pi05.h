@@ -314,7 +314,8 @@ PI05_API int pi05_fp8_status(void* stream, char* err, size_t err_len);
  *   were in out.  causal != 0: token t sees j < lens[b] - n + t + 1 (the last one sees all, as after a write of the n tokens).  A row that sees nothing gives 0; one that sees a NaN row of the cache, or whose query holds a NaN or an
  *   infinity, gives NaN.  heads is a multiple of kv_heads; query head h reads K/V head
  *   h / (heads / kv_heads).  q and out bf16, token t of sample b at b * sample stride + t * token stride elements, heads
- *   contiguous, 16-byte aligned.  workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
+ *   contiguous, 16-byte aligned.  V rows of a sample may be of any sizes; those below 2^-180 of its largest may count as 0.
+ *   workspace: pi05_kv8_attention_workspace bytes (0: NULL will do), 16-byte aligned, contents
  *   of no importance before and after.  The bytes depend on every size (and on the current device), and not monotonically: fewer
  *   samples or tokens may need more than many, because few rows are split along the keys.  Ask for each shape that will be
  *   called and keep the largest.  PI05_ERR_ARG (negative) for sizes that attention refuses. */

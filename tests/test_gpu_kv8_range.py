@@ -244,3 +244,17 @@ def test_queries_and_keys_both_large_but_orthogonal(pn, kernel, shape):
     lens = torch.full((B,), n, device="cuda", dtype=torch.int32)
     q = q.to(BF)
     bounded(run(pn, kernel, q, cache, lens), q, cache, lens)
+
+
+@pytest.mark.parametrize("kernel,shape", [("rows", ROWS[0]), ("rows", (2, 5, 8, 1, 256, 300)), ("tc", TC[0]), ("tc", TC[2]), ("tc", TC[3]), ("tc", TC_SPLIT[0])])
+def test_values_2_to_the_180_apart(pn, kernel, shape):
+    """the range that the header names: V near 2^-54 beside one row of 2^126 that only the last token sees"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(51)
+    k = randn(g, B, n, kvh, hd)
+    v = (1 + torch.rand(B, n, kvh, hd, device="cuda", generator=g)) * 2.0**-54
+    v[:, n - 1] = 2.0**126
+    q = randn(g, B, T, H, hd, dtype=BF)
+    cache, lens = written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32)
+    got = run(pn, kernel, q, cache, lens, causal=True)
+    bounded(got, q, cache, lens, causal=True, weight=FP16 if kernel == "rows" else BF16, floor=2.0**-85)
