@@ -78,13 +78,16 @@ __device__ __forceinline__ uint32_t h2_to_bf2(uint32_t h) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   return pack_bf2(f.x, f.y);
 }
-// Exponents of V scales that one accumulator holds: a term is at most 2^15 (weight) * 2^9 (code) * 2^(scale - unit), summed
-// over up to 2^31 keys, so scales up to 2^72 above the unit cannot pass the fp32 range.
-constexpr int KV8_E_SPAN = 72;
+// Exponents of V scales that one accumulator holds.  A term is at most 2^15 (weight) * 2^9 (code) * 2^(scale - unit), summed over up
+// to 2^28 keys, so scales up to 2^64 above the unit (and the rest of a window) stay within the fp32 range; and a unit at most
+// 2^64 above the smallest scale leaves rows that see only that one all their bits.
+constexpr int KV8_E_SPAN = 64;
 // 2^n for any integer n (0 below 2^-127, 2^127 above)
 __device__ __forceinline__ float exp2_int(int n) {
   return n < -127 ? 0.f : __uint_as_float(n == -127 ? 0x400000u : (uint32_t)(min(n, 127) + 127) << 23);
 }
+// x 2^n for n from -252 to 127
+__device__ __forceinline__ float mul_exp2(float x, int n) { return x * exp2_int(max(n, -126)) * exp2_int(min(n + 126, 0)); }
 
 template <int HD>
 struct Kv8RowsCfg {
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
   float o[MT][4];
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   int eb = -1000;              // O is in units of 2^eb (-1000: no V scale yet, O is 0)
-  int e_top = -1000;           // the largest V exponent so far
+  int e_top = -1000, e_low = 1000;  // the largest and the smallest V exponent so far, a window's width loose
   constexpr int E_WINDOW = 11;  // fp16 steps: eb .. eb + E_WINDOW
 #pragma unroll
   for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -282,11 +285,14 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
         const int em = __reduce_max_sync(0xffffffffu, vb == 255 ? -1000 : vb - 127);
         int en = __reduce_min_sync(0xffffffffu, vb == 255 || vb == 0 ? 1000 : vb - 127), to = eb;
         if (em > eb + E_WINDOW || en < eb) {
+          e_low = min(e_low, en);
           en = min(en, em);
           e_top = max(e_top, em);
           to = max(min(en, em - 9), -127);  // a little room above
-          wide = em - en > E_WINDOW || e_top - to > KV8_E_SPAN;
+          // what is already summed must fit the new unit as well
+          wide = em - en > E_WINDOW || e_top - to > KV8_E_SPAN || to - e_low > KV8_E_SPAN;
           if (wide) to = eb == -1000 ? max(en, em - KV8_E_SPAN) : max(eb, em - KV8_E_SPAN);
+          else if (e_low < 1000) e_low = min(e_low, to);
         }
         const float ealpha = exp2_int(eb - to);  // 0 at first, when O is 0 anyway
         eb = to;
@@ -393,11 +399,14 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
       sm_l[warp][2 * c + j] = l_run[j];
     }
   }
-  if (lane == 0) sm_e[warp] = eb;
+  if (lane == 0) sm_e[warp] = e_top;
   __syncthreads();
+  // one unit for all: warps that saw only small rows keep their bits beside one that saw only a large one
   int e_all = -1000;
 #pragma unroll
   for (int w = 0; w < W; ++w) e_all = max(e_all, sm_e[w]);
+  e_all = max(e_all - KV8_E_SPAN, -127);
+  const float e1 = exp2_int(max(eb - e_all, -126)), e2 = exp2_int(min(eb - e_all + 126, 0));
   float* tile = reinterpret_cast<float*>(smem);  // [W][8][HD], each warp's in its own ring
   constexpr int TILE = C::STAGES * C::STAGE / 4;
 #pragma unroll
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; ++w) m = fmaxf(m, sm_m[w][2 * c + j]);
-    const float f = m_run[j] == -INFINITY ? 0.f : ex2_approx(m_run[j] - m) * exp2_int(eb - e_all);
+    const float f = m_run[j] == -INFINITY ? 0.f : ex2_approx(m_run[j] - m) * e2;
     float* dst = tile + warp * TILE + (2 * c + j) * HD;
 #pragma unroll
     for (int i = 0; i < VI; ++i)
@@ -413,7 +422,7 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
       for (int q = 0; q < VB; q += 4) {
         const int k = i * (VB / 2) + q / 2;
         *reinterpret_cast<float4*>(dst + 128 * i + VB * g + q) =
-            make_float4(o[k][j] * f, o[k][2 + j] * f, o[k + 1][j] * f, o[k + 1][2 + j] * f);
+            make_float4(o[k][j] * e1 * f, o[k][2 + j] * e1 * f, o[k + 1][j] * e1 * f, o[k + 1][2 + j] * e1 * f);
       }
   }
   if (threadIdx.x < 8) {
@@ -462,13 +471,12 @@ __global__ void __launch_bounds__(32 * Kv8RowsCfg<HD>::W, Kv8RowsCfg<HD>::PER_SM
       const int ep = size > 1 ? __float_as_int(ld_peer_f32(map_peer(smem_u32(&cta_e), p))) : cta_e;
       const float f = mp == -INFINITY ? 0.f : ex2_approx(mp - m);
       l += mp == -INFINITY ? lp : lp * f;
-      const float fe = f * exp2_int(ep - e);
 #pragma unroll
       for (int k = 0; k < HD / 64; ++k) {
         const float* q = tile + r * HD + 64 * k + 2 * lane;
         const uint32_t at = size > 1 ? map_peer(smem_u32(q), p) : 0u;
-        x[2 * k] += fe * (size > 1 ? ld_peer_f32(at) : q[0]);
-        x[2 * k + 1] += fe * (size > 1 ? ld_peer_f32(at + 4) : q[1]);
+        x[2 * k] += f * mul_exp2(size > 1 ? ld_peer_f32(at) : q[0], ep - e);
+        x[2 * k + 1] += f * mul_exp2(size > 1 ? ld_peer_f32(at + 4) : q[1], ep - e);
       }
     }
     const float unit = exp2_int(e);

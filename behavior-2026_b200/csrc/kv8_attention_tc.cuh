@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(512, 1)
             e_low = min(e_low, en);
             if (em > eb + E_UP || en < eb - E_DOWN) {
               const int to = en >= em - E_DOWN ? em : em - E_UP;
-              if (em - en > E_UP + E_DOWN || e_top - to > KV8_E_SPAN) flags[2] = 1;
+              // what is already summed must fit the new unit as well
+              if (em - en > E_UP + E_DOWN || e_top - to > KV8_E_SPAN || to - e_low > KV8_E_SPAN) flags[2] = 1;
               if (i > 0) rescale = exp2_int(eb - to);  // 0 where there was no exponent yet: O is 0
               eb = to;
             }

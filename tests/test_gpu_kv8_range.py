@@ -258,3 +258,34 @@ def test_values_2_to_the_180_apart(pn, kernel, shape):
     cache, lens = written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32)
     got = run(pn, kernel, q, cache, lens, causal=True)
     bounded(got, q, cache, lens, causal=True, weight=FP16 if kernel == "rows" else BF16, floor=2.0**-85)
+
+
+# one key behind whole steps of 32 and tiles of 64, so that it has a step, a warp, a tile, a CTA of a cluster or a split to itself
+ALONE = [("rows", (1, 40, 8, 2, 128, 65)), ("rows", (1, 3, 8, 1, 256, 129)), ("rows", (1, 3, 8, 1, 256, 33)), ("rows", (1, 2, 8, 1, 256, 2049)),
+         ("rows", (1, 2, 8, 2, 64, 1025)), ("rows", (1, 2, 8, 1, 256, 20001)), ("tc", (2, 130, 8, 1, 256, 129)), ("tc", (4, 200, 8, 1, 128, 193)),
+         ("tc", (8, 400, 8, 1, 64, 257)), ("tc", (1, 968, 8, 1, 256, 961)), ("tc", (2, 300, 8, 1, 128, 1025))]
+
+
+@pytest.mark.parametrize("large", [2.0**30, 2.0**70, 2.0**100, 3.3e38])
+@pytest.mark.parametrize("kernel,shape", ALONE)
+def test_large_hidden_value_alone_in_its_step(pn, kernel, shape, large):
+    one_large_hidden_value(pn, kernel, shape, large)
+
+
+@pytest.mark.parametrize("where", ["first", "middle", "last", "a tile"])
+@pytest.mark.parametrize("kernel,shape", ALONE)
+def test_large_values_without_weight(pn, kernel, shape, where):
+    """keys whose logits are e^-900 below the others, with V of 3e38: they count for nothing, before, among and behind the rest"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(52)
+    k, v = randn(g, B, n, kvh, hd), randn(g, B, n, kvh, hd)
+    q = randn(g, B, T, H, hd)
+    q[..., 0] = 30.0
+    at = {"first": [0], "middle": [n // 2], "last": [n - 1], "a tile": list(range(min(64, n - 2)))}[where]
+    k[:, at] = 0
+    k[:, at, :, 0] = -30.0 * math.sqrt(hd)
+    v[:, at] = 2.0**126
+    cache, lens = written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32)
+    q = q.to(BF)
+    got = run(pn, kernel, q, cache, lens)
+    bounded(got, q, cache, lens, weight=FP16 if kernel == "rows" else BF16, floor=2.0**-60)
