@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(512, 1)
             kt = max(kt, kb[q] == 255 ? 0 : kb[q]);
             ev[q] = (vb[q] < 0 || vb[q] == 255) ? -1000 : vb[q] - 127;
           }
-          // A tile's largest K factor is kept to 2^64, with the rest (kh) for the row's own factor: codes and K factor alone, up to
-          // 2^146, would leave the float range where the logit does not.
-          const int kh = max(__reduce_max_sync(0xffffffffu, kt) - (127 + 64), 0);
+          // A tile's largest K factor is kept to 2^100, with the rest (kh) for the row's own factor: codes (2^26) and K factor
+          // alone, up to 2^146, would leave the float range where the logit does not.
+          const int kh = max(__reduce_max_sync(0xffffffffu, kt) - (127 + 100), 0);
 #pragma unroll
           for (int q = 0; q < 2; ++q)
             kf[q] = (kb[q] == 255 || vb[q] == 255) ? NAN : exp2_int(kb[q] - 127 - kh);  // a NaN row: NaN for the rows that see it
@@ -584,9 +584,9 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], x[c + k], x[c + 8 + k]);
         // in base 2: rf carries the row's power of two, the softmax scale, log2 e and the unit of the K factors.  It is positive
-        // and finite, so that a masked logit of -inf stays one and a sum of 0 gives 0.
+        // and finite, so that a masked logit of -inf stays one and a sum of 0 gives 0; the smallest float makes no logit of 2^-23.
         const float2 tile = *reinterpret_cast<const float2*>(sc + 2 * C::KT);
-        const float rf = fminf(fmaxf(row_factor * tile.y, 1.17549435e-38f), 3.4028235e38f);
+        const float rf = fminf(fmaxf(row_factor * tile.y, 1.4012985e-45f), 3.4028235e38f);
         const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], fmax3(mx[5], mx[6], mx[7]))) * rf;
         const float rescale = tile.x;
         __syncwarp();

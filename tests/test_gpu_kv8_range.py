@@ -289,3 +289,19 @@ def test_large_values_without_weight(pn, kernel, shape, where):
     q = q.to(BF)
     got = run(pn, kernel, q, cache, lens)
     bounded(got, q, cache, lens, weight=FP16 if kernel == "rows" else BF16, floor=2.0**-60)
+
+
+@pytest.mark.parametrize("qe,ke,scale", [(-100, 118, 1e-30), (-126, 118, 1e-30), (100, -100, 0.1), (10, 20, 1e-38)])
+@pytest.mark.parametrize("kernel,shape", [("rows", ROWS[0]), ("tc", TC[0]), ("tc", TC[2]), ("tc", TC[3])])
+def test_factors_at_the_ends_of_the_float_range(pn, kernel, shape, qe, ke, scale):
+    """logits that vanish though a factor of theirs is next to the largest, and keys of ordinary logits beside a hidden huge one"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(53)
+    q = (randn(g, B, T, H, hd) * 2.0**qe).to(BF)
+    k = randn(g, B, n, kvh, hd) * 2.0**ke
+    if ke < 0:
+        k[:, n - 1] = randn(g, B, kvh, hd) * 2.0**116
+        q[:, T - 1] = 0  # the token that sees it
+    v = randn(g, B, n, kvh, hd)
+    cache, lens = written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32)
+    bounded(run(pn, kernel, q, cache, lens, causal=True, scale=scale), q, cache, lens, causal=True, scale=scale)
