@@ -12,7 +12,7 @@
 // One new token reads the whole cache once for a handful of products, so what counts is bytes in flight: each warp
 // keeps a ring of its own of STAGES steps (cp.async, no barrier between warps), 48 to 192 KB an SM.  Measured, 16 samples of 32
 // heads on 8 of 128: 46 us and 5.8 TB/s at 8,192 keys each, 71 us and 4.9 TB/s at 4,000 to 16,387 (the longest sample decides);
-// one sample of 1,018 keys on one head of 256 9.6 us, its chain of latencies, of 30,000 24 us.
+// one sample of 1,018 keys on one head of 256 9.9 us, its chain of latencies, of 30,000 25 us.
 //
 // Everything is computed transposed, keys and head dims on the 16-row side of mma.m16n8k16 and query rows on
 // the 8-column side, because one token of 8 heads has 8 rows, not 16:

@@ -15,8 +15,8 @@
 //                 and scaled by its row's power of two relative to an exponent eb by four converter warps (exact: eb follows the
 //                 tiles so that their scales lie within eb - 15 .. eb + 7; keys that no row sees become zeros, whatever the cache
 //                 holds there).  An e4m3 P would need three operands to keep the small weights of a long cache.
-//                 Where a tile's scales span more (a key that some rows do not see counts as well: it must not cost them
-//                 bits), the CTA goes through its keys again with V and P in bf16, into which any scale fits; V is exact,
+//                 Where a tile's scales span more, or lie more than 2^64 from those before (a key that some rows do not see
+//                 counts as well: it must not cost them bits), the CTA goes through its keys again with V and P in bf16, into which any scale fits; V is exact,
 //                 weights keep 8 bits.  A choice of type for each tile made every call 2 to 7 % slower, in each form tried.
 // Measured: 64 chunks of 50 tokens, 8 heads on one of 256, 1,018 keys 50.6 us (527 TFLOP/s); 8 x 968 x 968 98 us (629); 2 x 2,049
 // tokens, causal over 8,192 keys, 16 heads on 4 of 128 315 us (764) and on 2 of 64 270 us (446); where the second pass is needed the

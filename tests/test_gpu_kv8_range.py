@@ -305,3 +305,34 @@ def test_factors_at_the_ends_of_the_float_range(pn, kernel, shape, qe, ke, scale
     v = randn(g, B, n, kvh, hd)
     cache, lens = written(pn, k, v), torch.full((B,), n, device="cuda", dtype=torch.int32)
     bounded(run(pn, kernel, q, cache, lens, causal=True, scale=scale), q, cache, lens, causal=True, scale=scale)
+
+
+@pytest.mark.parametrize("kernel,shape", [("rows", ROWS[0]), ("rows", ROWS_SPLIT[0]), ("tc", TC[1]), ("tc", TC_SPLIT[0])])
+def test_far_apart_values_again_on_streams_and_from_a_graph(pn, kernel, shape):
+    """the bf16 products too give the same bits each time: twice at once, and replayed on a cache that has changed between wide and
+    narrow"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(54)
+    k = randn(g, B, n, kvh, hd)
+    wide = randn(g, B, n, kvh, hd) * torch.exp2(torch.randint(-40, 41, (B, n, kvh, 1), device="cuda", generator=g).float())
+    caches = [written(pn, k, wide), written(pn, k, randn(g, B, n, kvh, hd))]
+    q, lens = randn(g, B, T, H, hd, dtype=BF), torch.full((B,), n, device="cuda", dtype=torch.int32)
+    want = [run(pn, kernel, q, c, lens) for c in caches]
+    side = [torch.cuda.Stream() for _ in caches]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for c, s in zip(caches, side):
+            with torch.cuda.stream(s):
+                got.append(pn.kv8_attention(q, *c, lens=lens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+    live = [t.clone() for t in caches[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pn.kv8_attention(q, *live, lens=lens)
+    for i in (0, 1, 0, 1, 1, 0):
+        for a, b in zip(live, caches[i]):
+            a.copy_(b)
+        graph.replay()
+        assert torch.equal(out, want[i])

@@ -154,3 +154,17 @@ def test_small_weights_add_up(pn, kernel, T):
     # most 2^-11 of itself, or 2^-25 / 2^7 (subnormal); the fp32 sums by 60,000 * 2^-23
     rel = 2.0**-11 + 2.0**-32 / math.exp(-14.5) + cap * 2.0**-23 + 2.0**-20 + 14.5 * 1.45 * 2.0**-22
     assert (got.double() - ref).abs().max() <= (rel + 2.0**-8) * ref
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("kernel,shape", [("tc", (8, 400, 8, 1, 64, 5)), ("tc", (8, 200, 8, 1, 128, 3)), ("tc", (8, 200, 8, 1, 256, 1)),
+                                          ("rows", (3, 1, 40, 8, 128, 1)), ("rows", (2, 3, 71, 1, 64, 300)), ("tc", (16, 2, 96, 1, 128, 700)),
+                                          ("tc", (8, 30, 71, 1, 128, 400)), ("tc", (64, 3, 71, 1, 256, 300))])
+def test_caches_smaller_than_a_tile_and_odd_groups(pn, kernel, shape, causal):
+    """capacities of 1 to 5 positions; 71 and 96 query heads on one, so that tokens straddle the row tiles"""
+    B, T, H, kvh, hd, n = shape
+    g = gen(89)
+    q, cache = randn(g, B, T, H, hd, dtype=BF), filled(pn, g, B, n, kvh, hd)
+    lens = torch.randint(0, n + 2, (B,), device="cuda", generator=g).int()
+    lens[0] = n
+    bounded(run(pn, kernel, q, cache, lens, causal=causal), q, cache, lens, causal=causal)
